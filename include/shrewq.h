@@ -201,6 +201,35 @@ SHREWQ_API int shrewq_dequantize_ex(shrewq_ctx *ctx, const int8_t *q_dev, const 
                          const double *zero_points_dev, size_t rows, size_t cols, int granularity,
                          int out_dtype, void *out_dev);
 
+/* ---- 4-bit microscaled floating point --------------------------------------------------- */
+/*
+ * No counterpart in the reference (its 4-bit type is an integer, quantize.rs:51-58): weights, and activations if asked, as E2M1 codes
+ * (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a scale for every block along a row:
+ *   SHREWQ_FP4_MX  blocks of 32, a power of two as an E8M0 byte b (2^(b - 127), 255 = NaN): 2^(floor(log2 amax) - 2), at least 2^-127;
+ *   SHREWQ_FP4_NV  blocks of 16, an E4M3 byte (448 at most, 0x7F = NaN), and one f32 scale g for the whole tensor:
+ *                  e4m3(amax / (6 g)), at least 2^-9.
+ * amax is the block's largest magnitude.  A block of zeros has the scale 1; a block with an infinity or a NaN has the scale NaN and
+ * codes 0, so that it comes back as NaN.  code = x / scale (NV: (x / g) / scale, with x / g formed as x times the rounded reciprocal of g)
+ * rounded to the nearest E2M1 value, ties to the even code, saturating at 6 (the sign of a zero
+ * code is not specified); a value is code * scale (* g), rounded to f32 for NV.
+ *
+ * Layout of a tensor [rows, cols], with cols padded to Kp = a multiple of 32: codes, rows x Kp / 2 bytes, two a byte, the even column
+ * in the low nibble; scales, rows x Kp / 32 (MX) or Kp / 16 (NV) bytes.  Padding holds code 0 (scale 1 in blocks of padding alone).
+ */
+#define SHREWQ_FP4_MX 0
+#define SHREWQ_FP4_NV 1
+/*
+ * w_dev: [rows, cols] of w_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), rows ldw elements apart.  codes_dev must be 4-byte aligned.
+ * tensor_scale_dev: NULL for MX; for NV one f32 on the device: read if find_tensor_scale is 0 (a positive number), else written: the
+ * smallest power of two g with 2688 g >= the tensor's largest finite magnitude (1 for a tensor of zeros).  Finding it takes a pass over
+ * the tensor of its own.  No workspace grows; up to eight calls that find a scale may be in flight on different streams.
+ */
+SHREWQ_API int shrewq_quantize_fp4(shrewq_ctx *ctx, const void *w_dev, int w_dtype, size_t rows, size_t cols, size_t ldw, int format,
+                                   float *tensor_scale_dev, int find_tensor_scale, uint8_t *codes_dev, uint8_t *scales_dev);
+/* Codes and scales -> values of out_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), [rows, cols] without gaps. */
+SHREWQ_API int shrewq_dequantize_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev,
+                                     size_t rows, size_t cols, int format, int out_dtype, void *out_dev);
+
 /* ---- quantized Linear --------------------------------------------------------------- */
 /*
  * QuantizedLinear::new — quantize.rs:437-447 (from_linear, :413-434, is
@@ -234,6 +263,23 @@ SHREWQ_API int shrewq_pack_int4(shrewq_ctx *ctx, const int8_t *q_dev, size_t row
 SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_dev, const double *scales_dev,
                               const float *bias_dev, size_t out_features, size_t in_features,
                               int granularity, shrewq_linear **out);
+/*
+ * A layer over 4-bit microscaled weights (shrewq_quantize_fp4, or codes and scales of the same layout from elsewhere).
+ * codes_dev must be 16-byte aligned and, like bias_dev, outlive the handle; scales_dev and tensor_scale_dev (one f32 on the device;
+ * NULL for MX) are copied, in the order of the context's stream, into memory of the handle (one byte a block, rows padded to 128,
+ * columns to 256).
+ * The handle goes through shrewq_linear_forward, shrewq_linear_forward_gate_up_silu (both layers of one format and one treatment of
+ * activations), shrewq_linear_forward_host and shrewq_mlp_forward_host; not through peer destinations or the no-allocation forward.  Any
+ * in_features; activations and results f32 or bf16.
+ *   quantize_activations = 0: y = x . dequant(W)^T + bias with f32 sums of exact products.  bf16 activations smaller than 2^-64 of the
+ *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens.
+ *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
+ *     positive number, as the tensor scale), and codes are multiplied by codes on the block-scaled tensor cores.
+ * Both use the context's workspace (staged activations, partial sums): see shrewq_ctx_set_stream.
+ */
+SHREWQ_API int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev,
+                                        const float *bias_dev, size_t out_features, size_t in_features, int format,
+                                        int quantize_activations, float activation_scale, shrewq_linear **out);
 SHREWQ_API void shrewq_linear_destroy(shrewq_linear *lin);
 
 /*
@@ -349,6 +395,50 @@ SHREWQ_API int shrewq_exchange_create(shrewq_ctx *ctx, int rank, int world, void
                                       shrewq_exchange **out);
 SHREWQ_API int shrewq_exchange_barrier(shrewq_exchange *ex);
 SHREWQ_API void shrewq_exchange_destroy(shrewq_exchange *ex);
+
+/* ---- between two blocks ------------------------------------------------------------------- */
+/*
+ * The norms before and after a block, its gate and the residual scale in one pass over the rows (no counterpart in the facade crate, whose
+ * blocks come from shrew-nn):
+ *   b = branch;  b = post_norm(b);  b = gate * b;  r = residual_scale * x + branch_scale * b;  h = pre_norm(r)
+ *   SHREWQ_NORM_RMS:   norm(v) = v / sqrt(mean(v^2) + eps) * weight + bias
+ *   SHREWQ_NORM_LAYER: norm(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
+ * x: [M, D] of x_dtype; branch: NULL (b is left out) or [M, D] of branch_dtype; gate: NULL or of branch_dtype: one value a channel
+ * [D], a token (element m * ldg) or an element [M, D].  Weights and biases: f32 [D], NULL = 1 and 0.  residual_dev (NULL = not
+ * wanted) receives r as [M, D] of x_dtype, normed_dev (NULL = not wanted) h as [M, D] of normed_dtype; h is formed from r in f32,
+ * before that is rounded.  Types: SHREWQ_F32 or SHREWQ_BF16.  Rows ldx / ldb / ldg elements apart.  D up to 32768.  Outputs must not
+ * overlap each other or an input.  Uses no workspace.
+ */
+#define SHREWQ_NORM_NONE 0
+#define SHREWQ_NORM_RMS 1
+#define SHREWQ_NORM_LAYER 2
+#define SHREWQ_GATE_NONE 0
+#define SHREWQ_GATE_CHANNEL 1
+#define SHREWQ_GATE_TOKEN 2
+#define SHREWQ_GATE_FULL 3
+typedef struct shrewq_residual_norm_args {
+    size_t M, D;
+    const void *x_dev;
+    size_t ldx;
+    int x_dtype;
+    const void *branch_dev;
+    size_t ldb;
+    int branch_dtype;
+    const void *gate_dev;
+    size_t ldg;
+    int gate_kind;
+    int post_norm;
+    float post_eps;
+    const float *post_weight_dev, *post_bias_dev;
+    float residual_scale, branch_scale;
+    int pre_norm;
+    float pre_eps;
+    const float *pre_weight_dev, *pre_bias_dev;
+    void *residual_dev;
+    void *normed_dev;
+    int normed_dtype;
+} shrewq_residual_norm_args;
+SHREWQ_API int shrewq_residual_norm(shrewq_ctx *ctx, const shrewq_residual_norm_args *args);
 
 /* Accessors mirroring QuantizedLinear's public fields / methods (quantize.rs:392-394,
  * :455-459). */

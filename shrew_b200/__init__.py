@@ -19,3 +19,5 @@ from .quantize import (  # noqa: F401
     quantize_tensor,
     quantize_tensors,
 )
+from .block import GatedMlp, Norm, NormKind, residual_norm, run_blocks  # noqa: F401
+from .fp4 import Fp4Format, Fp4Linear, Fp4Tensor, dequantize_fp4, quantize_fp4  # noqa: F401

@@ -3,6 +3,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "linear_fp4.cuh"
 
 namespace shrewq {
 
@@ -57,6 +58,8 @@ int ensure_scratch(shrewq_ctx *ctx, size_t bytes) {
 }
 
 int ensure_xsplit(shrewq_ctx *ctx, size_t bytes) { return grow(ctx, &ctx->xsplit, &ctx->xsplit_bytes, bytes, false); }
+
+int ensure_ytmp(shrewq_ctx *ctx, size_t bytes) { return grow(ctx, &ctx->ytmp, &ctx->ytmp_bytes, bytes, false); }
 
 int ensure_stage(shrewq_ctx *ctx, size_t dev_bytes, size_t pinned_bytes) {
     int rc = grow(ctx, &ctx->stage_dev, &ctx->stage_dev_bytes, dev_bytes, false);
@@ -552,6 +555,7 @@ void shrewq_linear_destroy(shrewq_linear *lin) {
     cudaStreamSynchronize(lin->ctx->stream);
     if (lin->scales_f32) cudaFree(lin->scales_f32);
     if (lin->czp) cudaFree(lin->czp);
+    destroy_fp4(lin->fp4);
     delete lin;
 }
 
@@ -560,6 +564,10 @@ size_t shrewq_linear_out_features(const shrewq_linear *lin) { return lin ? lin->
 /* fp32 size minus INT8 size — quantize.rs:455-459 */
 size_t shrewq_linear_memory_savings_bytes(const shrewq_linear *lin) {
     if (!lin) return 0;
+    if (lin->fp4) {  // codes and scales of whole 32s
+        const size_t codes = lin->n * ((lin->k + 31) / 32) * 16, held = codes + codes / (lin->fp4->nv ? 8 : 16);
+        return lin->n * lin->k * 4 > held ? lin->n * lin->k * 4 - held : 0;
+    }
     return lin->n * lin->k * 4 - (lin->int4_packed ? lin->n * lin->k / 2 : lin->n * lin->k);
 }
 const char *shrewq_linear_last_kernel(const shrewq_linear *lin) { return lin ? g_last_kernel : "none"; }
@@ -618,6 +626,26 @@ static int forward_impl(shrewq_linear *lin, shrewq_linear *up, const void *x_dev
     a.extra.n = n_peers;
     a.pdl = ctx->tuning.pdl != 0 && lin->forwarded.load(std::memory_order_relaxed) &&
             (!up || up->forwarded.load(std::memory_order_relaxed));
+
+    if (lin->fp4 || (up && up->fp4)) {
+        if (up && (!lin->fp4 || !up->fp4 || lin->fp4->nv != up->fp4->nv || lin->fp4->round_x != up->fp4->round_x || lin->fp4->x_scale != up->fp4->x_scale))
+            return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "%s: gate and up must both hold 4-bit weights of one format and treat activations alike", who);
+        if (n_peers > 0) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "%s: 4-bit weights take no peer destinations", who);
+        Fp4Forward f;
+        f.w = lin->fp4; f.up = up ? up->fp4 : nullptr;
+        f.bias = lin->bias; f.bias_up = up ? up->bias : nullptr;
+        f.w_tmap = up ? lin->w_tmap64 : lin->w_tmap; f.up_tmap = up ? up->w_tmap64 : nullptr;
+        f.x = x_dev; f.x_dtype = x_dtype; f.y = y_dev; f.y_dtype = y_dtype;
+        f.M = M; f.N = lin->n; f.K = lin->k; f.ldy = ldy; f.epilogue = epilogue; f.pdl = a.pdl;
+        const char *name = "none";
+        rc = forward_fp4(ctx, f, &name);
+        g_last_kernel = name;
+        if (rc == SHREWQ_OK) {
+            lin->forwarded.store(true, std::memory_order_relaxed);
+            if (up) up->forwarded.store(true, std::memory_order_relaxed);
+        }
+        return rc;
+    }
 
     // Packed INT4 rows: only the warp-MMA forward reads them (batch <= 32 for now)
     if (lin->int4_packed || (up && up->int4_packed)) {
@@ -732,8 +760,8 @@ int shrewq_linear_forward_noalloc(shrewq_linear *lin, const void *x_dev, size_t 
         return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "forward_noalloc: y_dtype must be SHREWQ_F32 or SHREWQ_BF16");
     if (epilogue != SHREWQ_EPILOGUE_NONE && epilogue != SHREWQ_EPILOGUE_RELU)
         return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "forward_noalloc: unknown epilogue %d", epilogue);
-    if (lin->czp || lin->int4_packed)
-        return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "forward_noalloc: handles with zero points or packed INT4 rows need shrewq_linear_forward");
+    if (lin->czp || lin->int4_packed || lin->fp4)
+        return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "forward_noalloc: handles with zero points, packed INT4 rows or 4-bit floating point weights need shrewq_linear_forward");
     if (M == 0) return SHREWQ_OK;
     if (!x_dev || !y_dev) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "forward_noalloc: x / y is NULL");
     if (ldy < lin->n) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "forward_noalloc: ldy smaller than out_features");

@@ -34,6 +34,10 @@ struct Tuning {
 
 }  // namespace shrewq
 
+namespace shrewq {
+struct Fp4Weight;
+}
+
 // Opaque in the ABI.
 struct shrewq_ctx {
     int device = 0;
@@ -82,6 +86,7 @@ struct shrewq_linear {
     float *scales_f32 = nullptr;  // owned, out_features entries (per-tensor scale broadcast)
     float *czp = nullptr;         // owned, scale * zero_point per output channel; null = symmetric
     bool int4_packed = false;     // q points at packed INT4 rows (in_features / 2 bytes each)
+    shrewq::Fp4Weight *fp4 = nullptr;  // owned: a layer with 4-bit microscaled weights (q, scales_f32 and czp are null then)
     size_t n = 0, k = 0;
     int granularity = 0;
     // TMA descriptors for the INT8 weight matrix (128 B each, opaque CUtensorMap), valid when
@@ -136,6 +141,7 @@ int launch_dequantize(shrewq_ctx *ctx, const int8_t *q, const double *scales, si
 int launch_scales_to_f32(shrewq_ctx *ctx, const double *scales, int granularity, size_t n, float *out);
 int launch_split_f32(shrewq_ctx *ctx, const float *x, size_t n, void *hi_bf16, void *lo_bf16);
 int ensure_xsplit(shrewq_ctx *ctx, size_t bytes);
+int ensure_ytmp(shrewq_ctx *ctx, size_t bytes);
 int launch_quantize_ex(shrewq_ctx *ctx, const float *w, size_t rows, size_t cols, int granularity, int bits, int mode,
                        int8_t *q, double *scales, double *zps);
 int launch_quantize_any(shrewq_ctx *ctx, const void *w, int w_dtype, size_t rows, size_t cols, int granularity, int bits,
@@ -147,6 +153,10 @@ int launch_row_sums(shrewq_ctx *ctx, const void *x, int x_dtype, size_t M, size_
 int launch_zero_point_fix(shrewq_ctx *ctx, const float *acc, const float *czp, const float *xsum, size_t M, size_t N,
                           size_t ldy, int relu, int y_dtype, void *y);
 
+
+struct Fp4Forward;
+int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel);
+void destroy_fp4(Fp4Weight *w);
 
 struct ForwardArgs {
     const int8_t *q;       // [N,K]

@@ -40,6 +40,9 @@ struct Library {
     decltype(&shrewq_dequantize_ex) dequantize_ex = nullptr;
     decltype(&shrewq_linear_forward) linear_forward = nullptr;
     decltype(&shrewq_linear_forward_gate_up_silu) gate_up_silu = nullptr;
+    decltype(&shrewq_quantize_fp4) quantize_fp4 = nullptr;
+    decltype(&shrewq_dequantize_fp4) dequantize_fp4 = nullptr;
+    decltype(&shrewq_residual_norm) residual_norm = nullptr;
 } L;
 
 PyObject *g_error = nullptr;       // ShrewError(code, message)
@@ -444,6 +447,241 @@ PyObject *dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// ---- 4-bit microscaled floating point --------------------------------------------------------------------------
+int64_t padded32(int64_t cols) { return (cols + 31) / 32 * 32; }
+
+long int_arg(PyObject *o) {
+    const long v = PyLong_AsLong(o);
+    if (v == -1 && PyErr_Occurred()) throw PythonError{};
+    return v;
+}
+double float_arg(PyObject *o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PythonError{};
+    return v;
+}
+
+// one f32 on the device
+void *tensor_scale_arg(PyObject *o, int device, const char *who) {
+    const at::Tensor &t = tensor_arg(o, who);
+    if (!on_device(t) || device_index(t) != device || t.scalar_type() != at::kFloat || t.numel() != 1)
+        fail(SHREWQ_ERR_INVALID_ARG, std::string(who) + ": the tensor scale is one float32 on the tensor's device");
+    return t.data_ptr();
+}
+
+// quantize_fp4(tensor, format, tensor scale or None) -> (codes, scales, tensor scale or None, shape)
+PyObject *quantize_fp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        if (n != 3) {
+            PyErr_SetString(PyExc_TypeError, "quantize_fp4(tensor, format, tensor_scale)");
+            throw PythonError{};
+        }
+        const at::Tensor &t = tensor_arg(args[0], "quantize_fp4");
+        const int wt = storage_code(t.scalar_type());
+        if (wt < 0 || wt == SHREWQ_F64) fail(SHREWQ_ERR_UNSUPPORTED, "quantize_fp4: dtype " + dtype_name(t.scalar_type()) + " not supported (f32, bf16, f16)");
+        const int device = device_index(t);
+        shrewq_ctx *ctx = context_of(device);
+        const int format = (int)int_arg(args[1]);
+        const bool nv = format == SHREWQ_FP4_NV;
+        // a matrix whose rows are dense is read where it is; anything else from a dense copy
+        const at::Tensor w = t.is_contiguous() || (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1)) ? t : t.contiguous();
+        const Rows rc_ = rows_cols(w.sizes());
+        const int64_t ld = w.dim() == 2 && rc_.rows > 1 && !w.is_contiguous() ? w.stride(0) : rc_.cols, kp = padded32(rc_.cols);
+        const int64_t code_shape[2] = {rc_.rows, kp / 2}, scale_shape[2] = {rc_.rows, kp / (nv ? 16 : 32)};
+        at::Tensor codes = empty(code_shape, at::kByte, device), scales = empty(scale_shape, at::kByte, device), whole;
+        float *gp = nullptr;
+        const bool find = nv && args[2] == Py_None;
+        if (find) {
+            whole = empty(1, at::kFloat, device);
+            gp = static_cast<float *>(whole.data_ptr());
+        } else if (args[2] != Py_None) {
+            gp = static_cast<float *>(tensor_scale_arg(args[2], device, "quantize_fp4"));
+        }
+        bind_stream(ctx, device);
+        const void *wp = w.data_ptr();
+        uint8_t *cp = static_cast<uint8_t *>(codes.data_ptr()), *sp = static_cast<uint8_t *>(scales.data_ptr());
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = L.quantize_fp4(ctx, wp, wt, (size_t)rc_.rows, (size_t)rc_.cols, (size_t)ld, format, gp, find ? 1 : 0, cp, sp);
+        Py_END_ALLOW_THREADS
+        check(rc, ctx);
+        PyObject *go;
+        if (find) go = wrap(std::move(whole));
+        else {
+            go = args[2];
+            Py_INCREF(go);
+        }
+        return Py_BuildValue("NNNN", wrap(std::move(codes)), wrap(std::move(scales)), go, shape_list(w.sizes()));
+    });
+}
+
+// codes or scales: bytes on the device, at least `need` of them
+at::Tensor bytes_arg(PyObject *o, int device, int64_t need, const char *who, const char *what) {
+    const at::Tensor &t = tensor_arg(o, who);
+    if (!on_device(t) || device_index(t) != device || t.scalar_type() != at::kByte || t.numel() < need)
+        fail(SHREWQ_ERR_INVALID_ARG, std::string(who) + ": needs " + std::to_string(need) + " uint8 " + what + " on one CUDA device");
+    return t.is_contiguous() ? t : t.contiguous();
+}
+
+// dequantize_fp4(codes, scales, tensor scale or None, shape, format, dtype) -> tensor
+PyObject *dequantize_fp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        if (n != 6) {
+            PyErr_SetString(PyExc_TypeError, "dequantize_fp4(codes, scales, tensor_scale, shape, format, dtype)");
+            throw PythonError{};
+        }
+        const at::Tensor &codes = tensor_arg(args[0], "dequantize_fp4");
+        const at::ScalarType type = dtype_arg(args[5], at::kFloat, "dequantize_fp4: the target dtype");
+        const int ot = storage_code(type);
+        if (ot < 0 || ot == SHREWQ_F64) fail(SHREWQ_ERR_UNSUPPORTED, "dequantize_fp4: target dtype " + dtype_name(type) + " not supported (f32, bf16, f16)");
+        const int device = device_index(codes), format = (int)int_arg(args[4]);
+        shrewq_ctx *ctx = context_of(device);
+        PyObject *seq = PySequence_Fast(args[3], "dequantize_fp4: shape is a list of sizes");
+        if (!seq) throw PythonError{};
+        c10::SmallVector<int64_t, 8> shape;
+        for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) shape.push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i)));
+        Py_DECREF(seq);
+        if (PyErr_Occurred()) throw PythonError{};
+        const Rows rc_ = rows_cols(shape);
+        const int64_t kp = padded32(rc_.cols);
+        const at::Tensor q = bytes_arg(args[0], device, rc_.rows * kp / 2, "dequantize_fp4", "codes");
+        const at::Tensor s = bytes_arg(args[1], device, rc_.rows * kp / (format == SHREWQ_FP4_NV ? 16 : 32), "dequantize_fp4", "scales");
+        const float *gp = args[2] == Py_None ? nullptr : static_cast<const float *>(tensor_scale_arg(args[2], device, "dequantize_fp4"));
+        at::Tensor out = empty(shape, type, device);
+        bind_stream(ctx, device);
+        const uint8_t *qp = static_cast<const uint8_t *>(q.data_ptr()), *sp = static_cast<const uint8_t *>(s.data_ptr());
+        void *op = out.data_ptr();
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = L.dequantize_fp4(ctx, qp, sp, gp, (size_t)rc_.rows, (size_t)rc_.cols, format, ot, op);
+        Py_END_ALLOW_THREADS
+        check(rc, ctx);
+        return wrap(std::move(out));
+    });
+}
+
+// ---- between two blocks ---------------------------------------------------------------------------------------
+// [..., D] as rows of D with one stride between them: the tensor itself where it is that, else a dense copy
+at::Tensor as_rows(const at::Tensor &t, int64_t *ld) {
+    const int64_t D = t.size(-1);
+    if (t.is_contiguous() || t.dim() == 1) {
+        *ld = D;
+        return t.is_contiguous() ? t : t.contiguous();
+    }
+    if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= D) {
+        *ld = t.stride(0);
+        return t;
+    }
+    *ld = D;
+    return t.contiguous();
+}
+
+// a norm's f32 vector of D values on the device, or None
+const float *norm_vector(PyObject *o, int device, int64_t D) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = tensor_arg(o, "residual_norm");
+    if (!on_device(t) || device_index(t) != device || t.scalar_type() != at::kFloat || t.numel() != D || !t.is_contiguous())
+        fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: a norm's weight and bias are " + std::to_string(D) + " float32 values on the device of x");
+    return static_cast<const float *>(t.data_ptr());
+}
+
+// residual_norm(x, branch, gate, pre kind, weight, bias, eps, post kind, weight, bias, eps, residual_scale, branch_scale, out dtype)
+//   -> (residual, normed or None)
+PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        if (n != 14) {
+            PyErr_SetString(PyExc_TypeError, "residual_norm(x, branch, gate, pre, weight, bias, eps, post, weight, bias, eps, residual_scale, branch_scale, out_dtype)");
+            throw PythonError{};
+        }
+        const at::Tensor &x0 = tensor_arg(args[0], "residual_norm");
+        if (!on_device(x0)) fail(SHREWQ_ERR_NO_DEVICE, "residual_norm: x is not on a CUDA device");
+        if (x0.dim() < 1 || x0.size(-1) < 1) fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: x is [..., D], got " + shape_text(x0));
+        const int device = device_index(x0);
+        const int64_t D = x0.size(-1), M = x0.numel() / D;
+        shrewq_residual_norm_args a = {};
+        int64_t ld = 0;
+        const at::Tensor x = as_rows(x0, &ld);
+        a.M = (size_t)M;
+        a.D = (size_t)D;
+        a.ldx = (size_t)ld;
+        a.x_dev = x.data_ptr();
+        a.x_dtype = act_code(x.scalar_type());
+        if (a.x_dtype < 0) fail(SHREWQ_ERR_UNSUPPORTED, "residual_norm: dtype " + dtype_name(x.scalar_type()) + " not supported (f32, bf16)");
+        at::Tensor b, g;
+        if (args[1] != Py_None) {
+            const at::Tensor &b0 = tensor_arg(args[1], "residual_norm");
+            if (!on_device(b0) || device_index(b0) != device || b0.sizes() != x0.sizes())
+                fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: branch has the shape and the device of x");
+            b = as_rows(b0, &ld);
+            a.ldb = (size_t)ld;
+            a.branch_dev = b.data_ptr();
+            a.branch_dtype = act_code(b.scalar_type());
+            if (a.branch_dtype < 0) fail(SHREWQ_ERR_UNSUPPORTED, "residual_norm: branch dtype " + dtype_name(b.scalar_type()) + " not supported (f32, bf16)");
+        }
+        if (args[2] != Py_None) {
+            const at::Tensor &g0 = tensor_arg(args[2], "residual_norm");
+            if (!b.defined()) fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: a gate needs a branch");
+            if (!on_device(g0) || device_index(g0) != device || g0.scalar_type() != b.scalar_type())
+                fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: gate has the dtype and the device of branch");
+            at::DimVector token(x0.sizes().begin(), x0.sizes().end());
+            token.back() = 1;
+            if (g0.sizes() == x0.sizes() && x0.dim() > 1) a.gate_kind = SHREWQ_GATE_FULL;  // (of one dimension: a channel each)
+            else if (g0.dim() == 1 && g0.size(0) == D) a.gate_kind = SHREWQ_GATE_CHANNEL;
+            else if (g0.dim() == x0.dim() && g0.sizes() == at::IntArrayRef(token)) a.gate_kind = SHREWQ_GATE_TOKEN;
+            else fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: gate is [D], [..., 1] or of the shape of x, got " + shape_text(g0));
+            if (a.gate_kind == SHREWQ_GATE_FULL) g = as_rows(g0, &ld);
+            else {
+                g = g0.is_contiguous() ? g0 : g0.contiguous();
+                ld = 1;
+            }
+            a.ldg = (size_t)ld;
+            a.gate_dev = g.data_ptr();
+        }
+        a.pre_norm = (int)int_arg(args[3]);
+        a.pre_weight_dev = norm_vector(args[4], device, D);
+        a.pre_bias_dev = norm_vector(args[5], device, D);
+        a.pre_eps = (float)float_arg(args[6]);
+        a.post_norm = (int)int_arg(args[7]);
+        if (a.post_norm != SHREWQ_NORM_NONE && !b.defined()) fail(SHREWQ_ERR_INVALID_ARG, "residual_norm: a norm after the block needs a branch");
+        a.post_weight_dev = norm_vector(args[8], device, D);
+        a.post_bias_dev = norm_vector(args[9], device, D);
+        a.post_eps = (float)float_arg(args[10]);
+        a.residual_scale = (float)float_arg(args[11]);
+        a.branch_scale = (float)float_arg(args[12]);
+        // without a branch and a scale the residual stream is x as it is
+        const bool same = !b.defined() && a.residual_scale == 1.0f;
+        at::Tensor r, h;
+        if (!same) {
+            r = empty(x0.sizes(), x0.scalar_type(), device);
+            a.residual_dev = r.data_ptr();
+        }
+        if (a.pre_norm != SHREWQ_NORM_NONE) {
+            const at::ScalarType type = dtype_arg(args[13], x0.scalar_type(), "residual_norm: out_dtype");
+            a.normed_dtype = act_code(type);
+            if (a.normed_dtype < 0) fail(SHREWQ_ERR_UNSUPPORTED, "residual_norm: output dtype " + dtype_name(type) + " not supported (f32, bf16)");
+            h = empty(x0.sizes(), type, device);
+            a.normed_dev = h.data_ptr();
+        }
+        if (M > 0 && (a.residual_dev || a.normed_dev)) {
+            shrewq_ctx *ctx = context_of(device);
+            bind_stream(ctx, device);
+            int rc;
+            Py_BEGIN_ALLOW_THREADS
+            rc = L.residual_norm(ctx, &a);
+            Py_END_ALLOW_THREADS
+            check(rc, ctx);
+        }
+        PyObject *ro, *ho = Py_None;
+        if (same) {
+            ro = args[0];
+            Py_INCREF(ro);
+        } else ro = wrap(std::move(r));
+        if (h.defined()) ho = wrap(std::move(h));
+        else Py_INCREF(ho);
+        return Py_BuildValue("NN", ro, ho);
+    });
+}
+
 // bind(addresses by name, error class, device index -> context address)
 PyObject *bind(PyObject *, PyObject *args) {
     PyObject *table, *error, *get;
@@ -459,7 +697,10 @@ PyObject *bind(PyObject *, PyObject *args) {
                    {"shrewq_quantize_f32_batch", reinterpret_cast<void **>(&L.quantize_f32_batch)},
                    {"shrewq_dequantize_ex", reinterpret_cast<void **>(&L.dequantize_ex)},
                    {"shrewq_linear_forward", reinterpret_cast<void **>(&L.linear_forward)},
-                   {"shrewq_linear_forward_gate_up_silu", reinterpret_cast<void **>(&L.gate_up_silu)}};
+                   {"shrewq_linear_forward_gate_up_silu", reinterpret_cast<void **>(&L.gate_up_silu)},
+                   {"shrewq_quantize_fp4", reinterpret_cast<void **>(&L.quantize_fp4)},
+                   {"shrewq_dequantize_fp4", reinterpret_cast<void **>(&L.dequantize_fp4)},
+                   {"shrewq_residual_norm", reinterpret_cast<void **>(&L.residual_norm)}};
     for (auto &e : entries) {
         PyObject *v = PyDict_GetItemString(table, e.name);
         if (!v) {
@@ -483,6 +724,9 @@ PyMethodDef kMethods[] = {
     {"quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(quantize)), METH_FASTCALL, nullptr},
     {"quantize_batch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(quantize_batch)), METH_FASTCALL, nullptr},
     {"dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(dequantize)), METH_FASTCALL, nullptr},
+    {"quantize_fp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(quantize_fp4)), METH_FASTCALL, nullptr},
+    {"dequantize_fp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(dequantize_fp4)), METH_FASTCALL, nullptr},
+    {"residual_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(residual_norm)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

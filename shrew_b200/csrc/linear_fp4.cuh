@@ -1,0 +1,43 @@
+// A layer with 4-bit microscaled weights on the host side: what its handle holds and what a forward is asked for.
+#pragma once
+
+#include "common.cuh"
+#include "fp4_params.cuh"
+
+namespace shrewq {
+
+struct Fp4Weight {
+    const uint8_t *codes = nullptr;   // the caller's, [N][Kp / 2]
+    uint8_t *pieces = nullptr;        // owned: the scales in the order of the block-scaled matrix instructions
+    Fp4Params *params = nullptr;      // owned, on the device
+    bool nv = false;
+    bool round_x = false;             // activations are quantized too
+    float x_scale = 1.0f;             // NV: tensor scale of the activations
+};
+
+struct Fp4Forward {
+    const Fp4Weight *w, *up;          // up null: a plain layer
+    const float *bias, *bias_up;
+    const void *w_tmap, *up_tmap;     // boxes of codes (128 rows, or 64 of a gated pair)
+    const void *x;
+    int x_dtype;
+    void *y;
+    int y_dtype;
+    size_t M, N, K, ldy;
+    int epilogue;
+    bool pdl;                         // weights are older than the previous kernel of the stream
+};
+
+// pieces of 128 rows by 4 blocks along a row, out to whole 256 columns
+inline size_t fp4_pieces(size_t K, bool nv) { return (K + 255) / 256 * (nv ? 4 : 2); }
+
+int launch_fill_f32(shrewq_ctx *ctx, float *p, float v);
+int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows, size_t cols, size_t ld, bool nv, float *g, bool find_g,
+                        void *codes, void *scales);
+int launch_dequantize_fp4(shrewq_ctx *ctx, const void *codes, const void *scales, const float *g, size_t rows, size_t cols, bool nv, int out_dtype, void *out);
+int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, bool nv, uint8_t *out,
+                            Fp4Params *params);
+int launch_gemv_fp4(shrewq_ctx *ctx, const Fp4Forward &a);
+int launch_residual_norm(shrewq_ctx *ctx, const shrewq_residual_norm_args *p);
+
+}  // namespace shrewq
