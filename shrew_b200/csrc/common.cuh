@@ -86,7 +86,7 @@ struct shrewq_linear {
     float *scales_f32 = nullptr;  // owned, out_features entries (per-tensor scale broadcast)
     float *czp = nullptr;         // owned, scale * zero_point per output channel; null = symmetric
     bool int4_packed = false;     // q points at packed INT4 rows (in_features / 2 bytes each)
-    shrewq::Fp4Weight *fp4 = nullptr;  // owned: a layer with 4-bit microscaled weights (q, scales_f32 and czp are null then)
+    shrewq::Fp4Weight *fp4 = nullptr;  // owned: a layer with 4-bit microscaled weights (q and czp are null, scales_f32 the tensor scale then)
     size_t n = 0, k = 0;
     int granularity = 0;
     // TMA descriptors for the INT8 weight matrix (128 B each, opaque CUtensorMap), valid when

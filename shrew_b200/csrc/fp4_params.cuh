@@ -5,6 +5,7 @@ namespace shrewq {
 
 struct Fp4Params {
     float tensor_scale;      // NV; 1 for MX
+    float x_scale;           // tensor scale of quantized activations (NV), else 1
     int max_byte, min_byte;  // MX: range of the scale bytes (NaN apart)
 };
 

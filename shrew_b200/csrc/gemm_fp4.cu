@@ -1,0 +1,74 @@
+// Launchers of the 4-bit by 4-bit forward (device code and its description: gemm_fp4_kernels.cuh): the activations are quantized first, by
+// a launch of the quantizer that writes their scales in pieces.
+#include <cuda_fp16.h>
+
+#include "gemm_tcgen05_launch.cuh"
+#include "fp4_kernels.cuh"
+#include "gemm_fp4_kernels.cuh"
+#include "linear_fp4.cuh"
+
+namespace shrewq {
+namespace {
+
+template <typename T, bool NV>
+cudaError_t quantize_acts(shrewq_ctx *ctx, const Fp4Forward &a, uint32_t *codes, uint8_t *pieces) {
+    const size_t blocks = fp4_pieces(a.K, NV) * 4, threads = blocks * (NV ? 2 : 4);
+    const int vec_ok = (reinterpret_cast<uintptr_t>(a.x) % (8 * sizeof(T))) == 0 && a.K % 8 == 0;
+    return launch_maybe_pdl(fp4_quantize_rows_kernel<T, NV, true>, dim3((unsigned)(a.M < 0x7FFFFFFF ? a.M : 0x7FFFFFFF)),
+                            dim3((unsigned)(threads < kFp4Threads ? threads : kFp4Threads)), 0, ctx->stream, ctx->tuning.pdl != 0, static_cast<const T *>(a.x),
+                            a.M, a.K, a.K, vec_ok, (const float *)&a.w->params->x_scale, (const float *)nullptr, 0, (float *)nullptr, blocks, codes, pieces);
+}
+
+template <int TOK, bool NV, bool GATED, typename YT>
+int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const uint8_t *pieces) {
+    using C = Fp4Cfg<TOK, NV, GATED>;
+    const size_t pitch = (a.K + 31) / 32 * 16;
+    CUtensorMap tx;
+    int rc = encode_2d(ctx, &tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, pitch, a.M, kFp4RowBytes, TOK, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != SHREWQ_OK) return rc;
+    auto kern = gemm_fp4_kernel<TOK, NV, GATED, YT>;
+    static std::atomic<unsigned long long> attr_done{0};
+    if ((rc = set_smem_attr_once(ctx, kern, C::kSmemRequest, attr_done)) != SHREWQ_OK) return rc;
+    const size_t tiles = (a.N + 127) / 128 * ((a.M + TOK - 1) / TOK);
+    if (tiles > 0x7FFFFFFF) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: more than 2^31 tiles");
+    const CUtensorMap &tw = *static_cast<const CUtensorMap *>(a.w_tmap), &tw2 = GATED ? *static_cast<const CUtensorMap *>(a.up_tmap) : tw;
+    const Operands ops{a.alpha, a.bias, a.alpha_up, a.bias_up};
+    SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(kern, dim3((unsigned)tiles), dim3(kFp4GemmThreads), (size_t)C::kSmemRequest, ctx->stream, a.pdl, tw, tw2, tx, (const uint8_t *)a.w->pieces,
+                                          (const uint8_t *)(GATED ? a.up->pieces : a.w->pieces), pieces, ops, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,
+                                          a.epilogue, ctx->dev_status));
+    ctx->launches += 1;
+    SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
+    return SHREWQ_OK;
+}
+
+template <bool NV, typename YT>
+int launch_tokens(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const uint8_t *pieces) {
+    if (a.up) return a.M <= 64 ? launch_one<64, NV, true, YT>(ctx, a, codes, pieces) : launch_one<128, NV, true, YT>(ctx, a, codes, pieces);
+    if (a.M <= 64) return launch_one<64, NV, false, YT>(ctx, a, codes, pieces);
+    if (a.M <= 128) return launch_one<128, NV, false, YT>(ctx, a, codes, pieces);
+    return launch_one<256, NV, false, YT>(ctx, a, codes, pieces);
+}
+
+}  // namespace
+
+int encode_fp4_tmap(shrewq_ctx *ctx, const uint8_t *codes, size_t n, size_t k, int box_rows, int box_bytes, void *tmap_out) {
+    return encode_2d(ctx, static_cast<CUtensorMap *>(tmap_out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, (k + 31) / 32 * 16, n, box_bytes, box_rows,
+                     box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+int launch_gemm_fp4(shrewq_ctx *ctx, const Fp4Forward &a) {
+    const bool nv = a.w->nv;
+    const size_t code_bytes = (a.M * ((a.K + 31) / 32 * 16) + 255) / 256 * 256, piece_bytes = (a.M + 127) / 128 * fp4_pieces(a.K, nv) * 512;
+    int rc = ensure_xsplit(ctx, code_bytes + piece_bytes);
+    if (rc != SHREWQ_OK) return rc;
+    uint32_t *codes = static_cast<uint32_t *>(ctx->xsplit);
+    uint8_t *pieces = static_cast<uint8_t *>(ctx->xsplit) + code_bytes;
+    const bool f32 = a.x_dtype == SHREWQ_F32;
+    SHREWQ_CUDA_TRY(ctx, nv ? (f32 ? quantize_acts<float, true>(ctx, a, codes, pieces) : quantize_acts<__nv_bfloat16, true>(ctx, a, codes, pieces))
+                            : (f32 ? quantize_acts<float, false>(ctx, a, codes, pieces) : quantize_acts<__nv_bfloat16, false>(ctx, a, codes, pieces)));
+    ctx->launches += 1;
+    if (a.y_dtype == SHREWQ_F32) return nv ? launch_tokens<true, float>(ctx, a, codes, pieces) : launch_tokens<false, float>(ctx, a, codes, pieces);
+    return nv ? launch_tokens<true, __nv_bfloat16>(ctx, a, codes, pieces) : launch_tokens<false, __nv_bfloat16>(ctx, a, codes, pieces);
+}
+
+}  // namespace shrewq

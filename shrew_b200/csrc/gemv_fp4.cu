@@ -60,13 +60,13 @@ int launch_gemv_fp4(shrewq_ctx *ctx, const Fp4Forward &a) {
 }
 
 int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, bool nv, uint8_t *out,
-                            Fp4Params *params) {
+                            Fp4Params *params, float x_scale, float *alpha) {
     SHREWQ_CUDA_TRY(ctx, cudaMemsetAsync(&params->max_byte, 0, sizeof(int), ctx->stream));
     SHREWQ_CUDA_TRY(ctx, cudaMemsetAsync(&params->min_byte, 0xFF, sizeof(int), ctx->stream));
     const size_t words = (N + 127) / 128 * 128 * pieces, want = (words + 255) / 256, cap = (size_t)ctx->sm_count * 16;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
-    if (nv) fp4_scale_pieces_kernel<true><<<grid, 256, 0, ctx->stream>>>(scales, g, N, blocks, pieces, out, params);
-    else fp4_scale_pieces_kernel<false><<<grid, 256, 0, ctx->stream>>>(scales, g, N, blocks, pieces, out, params);
+    if (nv) fp4_scale_pieces_kernel<true><<<grid, 256, 0, ctx->stream>>>(scales, g, N, blocks, pieces, out, params, x_scale, alpha);
+    else fp4_scale_pieces_kernel<false><<<grid, 256, 0, ctx->stream>>>(scales, g, N, blocks, pieces, out, params, x_scale, alpha);
     ctx->launches += 1;
     SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
     return SHREWQ_OK;

@@ -343,11 +343,12 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const uint16_t *__restrict__ terms
 
 // ---- a handle's copy of the scales --------------------------------------------------------------------------------------------------
 // scales [N][blocks] -> pieces (128 rows x 4 blocks, 512 bytes, out to whole 256 columns and 128 rows; scale 1 in the padding), the
-// tensor scale, and for MX the range of the bytes (NaN apart): params starts as {tensor scale, max_byte 0, min_byte 255}.
+// tensor scale, and for MX the range of the bytes (NaN apart; params starts with max_byte 0 and min_byte -1).  alpha[n]: what a sum of
+// channel n is multiplied by, the tensor scales of both operands.
 template <bool NV>
 __global__ void __launch_bounds__(256)
 fp4_scale_pieces_kernel(const uint8_t *__restrict__ scales, const float *g, size_t N, size_t blocks, size_t pieces, uint8_t *__restrict__ out,
-                        Fp4Params *params) {
+                        Fp4Params *params, float x_scale, float *__restrict__ alpha) {
     const size_t total = (N + 127) / 128 * 128 * pieces;  // words
     int top = 0, low = 255;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
@@ -379,7 +380,11 @@ fp4_scale_pieces_kernel(const uint8_t *__restrict__ scales, const float *g, size
             atomicMin(reinterpret_cast<unsigned int *>(&params->min_byte), (unsigned int)low);
         }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) params->tensor_scale = NV ? *g : 1.0f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        params->tensor_scale = NV ? *g : 1.0f;
+        params->x_scale = x_scale;
+    }
+    for (size_t n = (size_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (size_t)gridDim.x * 256) alpha[n] = NV ? *g * x_scale : 1.0f;
 }
 
 }  // namespace

@@ -22,35 +22,21 @@ bool sizes_overflow(size_t rows, size_t cols) { return cols > ((size_t)1 << 40) 
 
 }  // namespace
 
-int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &orig, const char **kernel) {
-    Fp4Forward a = orig;
-    if (a.w->round_x) {  // the values that the quantized activations stand for, in f32
-        const size_t values = a.M * a.K, words = a.M * ((a.K + 31) / 32 * 16), blocks = a.M * ((a.K + 31) / 32 * (a.w->nv ? 2 : 1));
-        const size_t off_c = (values * 4 + 255) / 256 * 256, off_s = off_c + (words + 255) / 256 * 256, off_g = off_s + (blocks + 255) / 256 * 256;
-        int rc = ensure_ytmp(ctx, off_g + 4);
-        if (rc != SHREWQ_OK) return rc;
-        char *base = static_cast<char *>(ctx->ytmp);
-        float *g = reinterpret_cast<float *>(base + off_g);
-        if (a.w->nv && (rc = launch_fill_f32(ctx, g, a.w->x_scale)) != SHREWQ_OK) return rc;
-        if ((rc = launch_quantize_fp4(ctx, a.x, a.x_dtype, a.M, a.K, a.K, a.w->nv, g, false, base + off_c, base + off_s)) != SHREWQ_OK) return rc;
-        if ((rc = launch_dequantize_fp4(ctx, base + off_c, base + off_s, g, a.M, a.K, a.w->nv, SHREWQ_F32, base)) != SHREWQ_OK) return rc;
-        a.x = base;
-        a.x_dtype = SHREWQ_F32;
-    }
-    if (a.M > 32) {  // slices of 32 tokens
-        for (size_t m = 0; m < a.M; m += 32) {
-            Fp4Forward s = a;
-            s.M = a.M - m < 32 ? a.M - m : 32;
-            s.x = static_cast<const char *>(a.x) + m * a.K * size_of(a.x_dtype);
-            s.y = static_cast<char *>(a.y) + m * a.ldy * size_of(a.y_dtype);
-            int rc = launch_gemv_fp4(ctx, s);
-            if (rc != SHREWQ_OK) return rc;
-        }
-        *kernel = "mma-fp4";
-        return SHREWQ_OK;
+int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
+    if (a.w->round_x) {
+        *kernel = "tcgen05-fp4";
+        return launch_gemm_fp4(ctx, a);
     }
     *kernel = "mma-fp4";
-    return launch_gemv_fp4(ctx, a);
+    for (size_t m = 0; m < a.M; m += 32) {  // slices of 32 tokens
+        Fp4Forward s = a;
+        s.M = a.M - m < 32 ? a.M - m : 32;
+        s.x = static_cast<const char *>(a.x) + m * a.K * size_of(a.x_dtype);
+        s.y = static_cast<char *>(a.y) + m * a.ldy * size_of(a.y_dtype);
+        int rc = launch_gemv_fp4(ctx, s);
+        if (rc != SHREWQ_OK) return rc;
+    }
+    return SHREWQ_OK;
 }
 
 void destroy_fp4(Fp4Weight *w) {
@@ -137,12 +123,15 @@ int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const ui
     w->round_x = quantize_activations != 0;
     w->x_scale = nv ? activation_scale : 1.0f;
     const size_t pieces = fp4_pieces(in_features, nv), bytes = (out_features + 127) / 128 * pieces * 512;
-    if (cudaMalloc(&w->pieces, bytes) != cudaSuccess || cudaMalloc(&w->params, sizeof(Fp4Params)) != cudaSuccess) {
+    if (cudaMalloc(&w->pieces, bytes) != cudaSuccess || cudaMalloc(&w->params, sizeof(Fp4Params)) != cudaSuccess ||
+        cudaMalloc(&lin->scales_f32, out_features * sizeof(float)) != cudaSuccess) {
         cudaGetLastError();
         shrewq_linear_destroy(lin);
         return set_err(ctx, SHREWQ_ERR_ALLOC, "linear_create_fp4: allocation of %zu bytes for the scales failed", bytes);
     }
-    rc = launch_fp4_scale_pieces(ctx, scales_dev, tensor_scale_dev, out_features, (in_features + 31) / 32 * (nv ? 2 : 1), pieces, nv, w->pieces, w->params);
+    rc = launch_fp4_scale_pieces(ctx, scales_dev, tensor_scale_dev, out_features, (in_features + 31) / 32 * (nv ? 2 : 1), pieces, nv, w->pieces, w->params, w->x_scale,
+                                 lin->scales_f32);
+    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 128, 128, lin->w_tmap);
     if (rc != SHREWQ_OK) {
         shrewq_linear_destroy(lin);
         return rc;

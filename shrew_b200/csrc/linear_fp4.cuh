@@ -18,7 +18,8 @@ struct Fp4Weight {
 struct Fp4Forward {
     const Fp4Weight *w, *up;          // up null: a plain layer
     const float *bias, *bias_up;
-    const void *w_tmap, *up_tmap;     // boxes of codes (128 rows, or 64 of a gated pair)
+    const float *alpha, *alpha_up;    // what the sums of a channel are multiplied by: the tensor scales (tcgen05 kernels)
+    const void *w_tmap, *up_tmap;     // boxes of codes
     const void *x;
     int x_dtype;
     void *y;
@@ -36,7 +37,9 @@ int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows
                         void *codes, void *scales);
 int launch_dequantize_fp4(shrewq_ctx *ctx, const void *codes, const void *scales, const float *g, size_t rows, size_t cols, bool nv, int out_dtype, void *out);
 int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, bool nv, uint8_t *out,
-                            Fp4Params *params);
+                            Fp4Params *params, float x_scale, float *alpha);
+int encode_fp4_tmap(shrewq_ctx *ctx, const uint8_t *codes, size_t n, size_t k, int box_rows, int box_bytes, void *tmap_out);
+int launch_gemm_fp4(shrewq_ctx *ctx, const Fp4Forward &a);
 int launch_gemv_fp4(shrewq_ctx *ctx, const Fp4Forward &a);
 int launch_residual_norm(shrewq_ctx *ctx, const shrewq_residual_norm_args *p);
 

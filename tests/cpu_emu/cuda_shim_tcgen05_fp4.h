@@ -1,0 +1,63 @@
+// Stand-ins for shrew_b200/csrc/ptx_tcgen05_fp4.cuh: tcgen05.cp of block scales and the block-scaled tcgen05.mma on E2M1 operands.
+// Include after cuda_shim_tcgen05.h and cuda_shim_fp4.h.  TEST INFRASTRUCTURE ONLY.
+#pragma once
+
+namespace emu {
+inline uint32_t desc_start(uint64_t d) { return (uint32_t)(d & 0x3FFFu) << 4; }
+inline uint32_t desc_stride(uint64_t d) { return (uint32_t)((d >> 32) & 0x3FFFu) << 4; }
+inline float scale_value(bool nv, uint32_t byte) { return nv ? emu_e4m3_value(byte & 0x7F) : byte == 255 ? NAN : ldexpf(1.0f, (int)byte - 127); }
+// E2M1 value (row, k) of a K-major operand with 128-byte swizzle; rows of 128 bytes, 8-row groups `stride` apart
+inline float fp4_operand(Block *blk, uint64_t desc, uint32_t row, uint32_t k) {
+    const uint32_t addr = (smem_u32(blk->dyn) | desc_start(desc)) + (row >> 3) * desc_stride(desc) + (row & 7) * 128 + (k >> 1);
+    const uint8_t byte = *smem_ptr(swizzle(addr, 128));
+    return emu_e2m1_value(k & 1 ? byte >> 4 : byte & 15);
+}
+inline void cp_scales(Block *blk, uint32_t taddr, uint64_t desc) {
+    const uint32_t col = taddr & 0xFFFF;
+    if ((taddr >> 16) != 0 || col + 4 > 512) { fail("tcgen05.cp outside tensor memory"); return; }
+    EMU_CHECK(((desc >> 61) & 7u) == 0 && ((desc >> 46) & 1u) == 1, "scales: no swizzle, descriptor version 1");
+    for (uint32_t r = 0; r < 32; ++r) {
+        const uint8_t *src = smem_ptr((smem_u32(blk->dyn) | desc_start(desc)) + (r >> 3) * desc_stride(desc) + (r & 7) * 16);
+        for (uint32_t j = 0; j < 4; ++j) {
+            uint32_t w;
+            memcpy(&w, src + 4 * j, 4);
+            for (uint32_t q = 0; q < 4; ++q) blk->tmem[(q * 32 + r) * 512 + col + j] = w;
+        }
+    }
+}
+// rows of A and D: 128 of block `d`; B and its scales as given
+inline void mma_fp4(Block *blk, bool nv, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    const uint32_t N = ((idesc >> 17) & 0x3Fu) << 3, M = ((idesc >> 24) & 0x1Fu) << 4, sa = (idesc >> 29) & 3u, sb = (idesc >> 4) & 3u;
+    EMU_CHECK(M == 128 && ((idesc >> 7) & 7u) == 1 && ((idesc >> 10) & 7u) == 1, "E2M1 operands, 128 rows");
+    EMU_CHECK(((idesc >> 23) & 1u) == (nv ? 0u : 1u), "scale type");
+    EMU_CHECK(nv ? sa == 0 && sb == 0 : (sa & 1) == 0 && (sb & 1) == 0, "scale ids");
+    EMU_CHECK(((a_desc >> 61) & 7u) == 2 && ((b_desc >> 61) & 7u) == 2, "128-byte swizzle");
+    const uint32_t dcol = d_tmem & 0xFFFF, ca = sfa & 0xFFFF, cb = sfb & 0xFFFF;
+    if (dcol + N > 512 || ca + 4 > 512 || cb + (N + 31) / 32 > 512) { fail("block-scaled MMA outside tensor memory"); return; }
+    const uint32_t per = nv ? 16 : 32;
+    auto scale = [&](uint32_t col, uint32_t row, uint32_t group, uint32_t id) {
+        return scale_value(nv, (blk->tmem[(row & 31) * 512 + col + (row >> 5)] >> (8 * (id + group))) & 0xFF);
+    };
+    std::vector<float> a(128 * 64), b(N * 64);
+    for (uint32_t r = 0; r < 128; ++r)
+        for (uint32_t k = 0; k < 64; ++k) a[r * 64 + k] = fp4_operand(blk, a_desc, r, k) * scale(ca, r, k / per, sa);
+    for (uint32_t r = 0; r < N; ++r)
+        for (uint32_t k = 0; k < 64; ++k) b[r * 64 + k] = fp4_operand(blk, b_desc, r, k) * scale(cb, r, k / per, sb);
+    for (uint32_t m = 0; m < 128; ++m)
+        for (uint32_t n = 0; n < N; ++n) {
+            double acc = accumulate ? (double)__uint_as_float(blk->tmem[m * 512 + dcol + n]) : 0.0;
+            for (uint32_t k = 0; k < 64; ++k) acc += (double)a[m * 64 + k] * b[n * 64 + k];
+            blk->tmem[m * 512 + dcol + n] = __float_as_uint((float)acc);
+        }
+}
+}  // namespace emu
+
+static inline void tc_cp_scales(uint32_t taddr, uint64_t desc) {
+    if (emu::tc_deferred()) emu::tc_push([=] { emu::cp_scales(emu::g_block, taddr, desc); });
+    else emu::cp_scales(emu::g_block, taddr, desc);
+}
+template <bool NV>
+static inline void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (emu::tc_deferred()) emu::tc_push([=] { emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate); });
+    else emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate);
+}

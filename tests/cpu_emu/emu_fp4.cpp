@@ -48,11 +48,13 @@ void dequantize(const void *codes, const void *scales, const float *g, size_t ro
 template <bool NV>
 struct Weight {
     std::vector<uint8_t> pieces;
-    Fp4Params params{0.0f, 0, -1};
+    std::vector<float> alpha;
+    Fp4Params params{0.0f, 0.0f, 0, -1};
     Weight(const uint8_t *scales, const float *g, size_t N, size_t K) {
         const size_t n_pieces = (K + 255) / 256 * (NV ? 4 : 2);
+        alpha.assign(N, 0.0f);
         pieces.assign((N + 127) / 128 * n_pieces * 512, 0xEE);
-        emu::launch(3, 256, [&] { fp4_scale_pieces_kernel<NV>(scales, g, N, (K + 31) / 32 * (NV ? 2 : 1), n_pieces, pieces.data(), &params); });
+        emu::launch(3, 256, [&] { fp4_scale_pieces_kernel<NV>(scales, g, N, (K + 31) / 32 * (NV ? 2 : 1), n_pieces, pieces.data(), &params, 1.0f, alpha.data()); });
     }
 };
 

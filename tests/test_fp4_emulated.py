@@ -244,3 +244,36 @@ def test_residual_norm(emu, x_dtype, b_dtype, h_dtype, M, D, V, pre, post, gate_
         rms = np.sqrt(((want_r - (want_r.mean(-1, keepdims=True) if pre == 2 else 0)) ** 2).mean(-1, keepdims=True) + 1e-5)
         spread = np.abs(n[2]) * (scale_r.max(-1, keepdims=True) / rms) * (1 + np.abs(want_r) / rms)
         assert (np.abs(h2.double().numpy() - want_h) <= half[h_dtype] * np.abs(want_h) + 4 * eps * spread).all()
+
+
+@pytest.fixture(scope="module")
+def emu_gemm():
+    L = _build("emu_gemm_fp4")
+    L.emu_gemm_fp4.argtypes = [_vp, _vp, _vp, _vp, _vp, _cf, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _cu]
+    return L
+
+
+@pytest.mark.parametrize("nv", [False, True])
+@pytest.mark.parametrize("M,N,K,tok,gated,seed", [(70, 130, 600, 64, False, 0), (100, 129, 256, 128, False, 3), (300, 40, 330, 256, False, 0), (33, 70, 1300, 64, True, 5),
+                                                  (130, 128, 90, 128, True, 0), (1, 1, 1, 64, False, 0), (200, 20, 2600, 256, False, 7)])
+def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, seed):
+    g = torch.Generator().manual_seed(M + K)
+    x = aligned((M, K), torch.float32)
+    x.copy_(torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g)))
+    ws = [stored(N, K, nv, N + i, spread=6) for i in range(2 if gated else 1)]
+    if nv:
+        for w in ws:   # (moderate scales, so that silu's argument stays ordinary)
+            w[1].copy_(torch.randint(0x20, 0x40, w[1].shape, generator=g).to(torch.uint8))
+            w[2].fill_(2.0 ** -4)
+    biases = [torch.randn(N, generator=g), None][: len(ws)]
+    y = torch.full((M, N + 4), -77.0)
+    table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
+    rc = emu_gemm.emu_gemm_fp4(table([w[0] for w in ws]), table([w[1] for w in ws]), table([w[2] for w in ws]), table(biases), x.data_ptr(), 0.5, M, N, K, tok,
+                               int(nv), int(gated), y.data_ptr(), N + 4, int(not gated and N % 2), seed)
+    assert rc == 0 and (y[:, N:] == -77.0).all()
+    xq = O.quantize(x.double().numpy(), nv, 0.5 if nv else None)[3]
+    wd = [O.dequantize(w[0].numpy(), w[1].numpy(), float(w[2]), K, nv) for w in ws]
+    up = wd[1] if gated else None
+    want = O.product(xq, wd[0], biases[0].numpy(), up=up, relu=not gated and N % 2 == 1)
+    bound = O.product_bound(xq, wd[0], K, up=up, bias=biases[0].numpy())
+    assert (np.abs(y[:, :N].double().numpy() - want) <= bound).all()
