@@ -635,7 +635,7 @@ static int forward_impl(shrewq_linear *lin, shrewq_linear *up, const void *x_dev
         f.w = lin->fp4; f.up = up ? up->fp4 : nullptr;
         f.bias = lin->bias; f.bias_up = up ? up->bias : nullptr;
         f.alpha = lin->scales_f32; f.alpha_up = up ? up->scales_f32 : nullptr;
-        f.w_tmap = lin->w_tmap; f.up_tmap = up ? up->w_tmap : nullptr;
+        f.w_tmap = up ? lin->w_tmap64 : lin->w_tmap; f.up_tmap = up ? up->w_tmap64 : nullptr;
         f.x = x_dev; f.x_dtype = x_dtype; f.y = y_dev; f.y_dtype = y_dtype;
         f.M = M; f.N = lin->n; f.K = lin->k; f.ldy = ldy; f.epilogue = epilogue; f.pdl = a.pdl;
         const char *name = "none";

@@ -27,16 +27,12 @@ int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
         *kernel = "tcgen05-fp4";
         return launch_gemm_fp4(ctx, a);
     }
-    *kernel = "mma-fp4";
-    for (size_t m = 0; m < a.M; m += 32) {  // slices of 32 tokens
-        Fp4Forward s = a;
-        s.M = a.M - m < 32 ? a.M - m : 32;
-        s.x = static_cast<const char *>(a.x) + m * a.K * size_of(a.x_dtype);
-        s.y = static_cast<char *>(a.y) + m * a.ldy * size_of(a.y_dtype);
-        int rc = launch_gemv_fp4(ctx, s);
-        if (rc != SHREWQ_OK) return rc;
+    if (a.M > 32) {
+        *kernel = "tcgen05-w4";
+        return launch_gemm_w4_bf16(ctx, a);
     }
-    return SHREWQ_OK;
+    *kernel = "mma-fp4";
+    return launch_gemv_fp4(ctx, a);
 }
 
 void destroy_fp4(Fp4Weight *w) {
@@ -131,7 +127,9 @@ int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const ui
     }
     rc = launch_fp4_scale_pieces(ctx, scales_dev, tensor_scale_dev, out_features, (in_features + 31) / 32 * (nv ? 2 : 1), pieces, nv, w->pieces, w->params, w->x_scale,
                                  lin->scales_f32);
-    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 128, 128, lin->w_tmap);
+    // boxes of the tensor-core kernels: 128 rows of 256 codes (codes by codes), or of 128 codes with 128 and, gated, 64 rows
+    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 128, w->round_x ? 128 : 64, lin->w_tmap);
+    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, w->round_x ? 128 : 64, w->round_x ? 128 : 64, lin->w_tmap64);
     if (rc != SHREWQ_OK) {
         shrewq_linear_destroy(lin);
         return rc;

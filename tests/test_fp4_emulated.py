@@ -249,14 +249,16 @@ def test_residual_norm(emu, x_dtype, b_dtype, h_dtype, M, D, V, pre, post, gate_
 @pytest.fixture(scope="module")
 def emu_gemm():
     L = _build("emu_gemm_fp4")
-    L.emu_gemm_fp4.argtypes = [_vp, _vp, _vp, _vp, _vp, _cf, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _cu]
+    L.emu_gemm_fp4.argtypes = [_vp, _vp, _vp, _vp, _vp, _cf, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
+    L.emu_gemm_w4_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
     return L
 
 
 @pytest.mark.parametrize("nv", [False, True])
-@pytest.mark.parametrize("M,N,K,tok,gated,seed", [(70, 130, 600, 64, False, 0), (100, 129, 256, 128, False, 3), (300, 40, 330, 256, False, 0), (33, 70, 1300, 64, True, 5),
-                                                  (130, 128, 90, 128, True, 0), (1, 1, 1, 64, False, 0), (200, 20, 2600, 256, False, 7)])
-def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, seed):
+@pytest.mark.parametrize("M,N,K,tok,gated,split,seed", [(70, 130, 600, 64, False, 0, 0), (100, 129, 256, 128, False, 0, 3), (300, 40, 330, 256, False, 1, 0),
+                                                        (33, 70, 1300, 64, True, 1, 5), (130, 128, 90, 128, True, 0, 0), (1, 1, 1, 64, False, 0, 0),
+                                                        (200, 20, 2600, 256, False, 0, 7), (40, 20, 2600, 64, False, 1, 9), (130, 60, 520, 128, True, 1, 2)])
+def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, split, seed):
     g = torch.Generator().manual_seed(M + K)
     x = aligned((M, K), torch.float32)
     x.copy_(torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g)))
@@ -269,7 +271,7 @@ def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, seed):
     y = torch.full((M, N + 4), -77.0)
     table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
     rc = emu_gemm.emu_gemm_fp4(table([w[0] for w in ws]), table([w[1] for w in ws]), table([w[2] for w in ws]), table(biases), x.data_ptr(), 0.5, M, N, K, tok,
-                               int(nv), int(gated), y.data_ptr(), N + 4, int(not gated and N % 2), seed)
+                               int(nv), int(gated), y.data_ptr(), N + 4, int(not gated and N % 2), split, seed)
     assert rc == 0 and (y[:, N:] == -77.0).all()
     xq = O.quantize(x.double().numpy(), nv, 0.5 if nv else None)[3]
     wd = [O.dequantize(w[0].numpy(), w[1].numpy(), float(w[2]), K, nv) for w in ws]
@@ -277,3 +279,30 @@ def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, seed):
     want = O.product(xq, wd[0], biases[0].numpy(), up=up, relu=not gated and N % 2 == 1)
     bound = O.product_bound(xq, wd[0], K, up=up, bias=biases[0].numpy())
     assert (np.abs(y[:, :N].double().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("nv", [False, True])
+@pytest.mark.parametrize("M,N,K,tok,x_dtype,gated,split,seed", [(70, 130, 600, 64, torch.bfloat16, False, 0, 0), (100, 129, 256, 128, torch.bfloat16, False, 1, 3),
+                                                                (300, 40, 336, 256, torch.bfloat16, False, 1, 0), (33, 70, 1300, 64, torch.float32, True, 1, 5),
+                                                                (130, 100, 96, 128, torch.bfloat16, True, 0, 0), (1, 1, 1, 64, torch.float32, False, 0, 0),
+                                                                (200, 150, 1111, 256, torch.bfloat16, True, 1, 7), (65, 20, 900, 64, torch.float32, False, 0, 9)])
+def test_four_bit_weights_on_the_tensor_cores(emu_gemm, nv, M, N, K, tok, x_dtype, gated, split, seed):
+    g = torch.Generator().manual_seed(M + K)
+    x = aligned((M, K), x_dtype)
+    x.copy_(torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g)))
+    ws = [stored(N, K, nv, N + i, spread=6) for i in range(2 if gated else 1)]
+    if nv:
+        for w in ws:
+            w[1].copy_(torch.randint(0x20, 0x40, w[1].shape, generator=g).to(torch.uint8))
+            w[2].fill_(2.0 ** -4)
+    biases = [torch.randn(N, generator=g), None][: len(ws)]
+    y = torch.full((M, N + 4), -77.0)
+    table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
+    rc = emu_gemm.emu_gemm_w4_bf16(table([w[0] for w in ws]), table([w[1] for w in ws]), table([w[2] for w in ws]), table(biases), x.data_ptr(),
+                                   int(x_dtype is torch.float32), M, N, K, tok, int(nv), int(gated), y.data_ptr(), N + 4, int(not gated and N % 2), split, seed)
+    assert rc == 0 and (y[:, N:] == -77.0).all()
+    xd = x.double().numpy()
+    wd = [O.dequantize(w[0].numpy(), w[1].numpy(), float(w[2]), K, nv) for w in ws]
+    up = wd[1] if gated else None
+    want = O.product(xd, wd[0], biases[0].numpy(), up=up, relu=not gated and N % 2 == 1)
+    assert (np.abs(y[:, :N].double().numpy() - want) <= O.product_bound(xd, wd[0], K, up=up, bias=biases[0].numpy())).all()
