@@ -2,61 +2,69 @@
 // description: gemv_fp4_kernels.cuh).
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "gemm_tcgen05_launch.cuh"
 #include "gemv_fp4_kernels.cuh"
 #include "linear_fp4.cuh"
 
 namespace shrewq {
 namespace {
 
-template <int NT, int RT, bool NV, bool GATED, typename YT>
-cudaError_t launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const uint16_t *terms, const int *exps, const int *counts) {
-    const size_t tiles = (a.N + 127) / 128 * (GATED ? 16 : 8);
+template <int NT, bool NV, bool GATED, bool XS, typename T, typename YT>
+int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const Gemv4X<T> &x, size_t staged) {
+    const size_t tiles = (a.N + 127) / 128 * (GATED ? 16 : 8), smem = kGemv4RingBytes + staged;
     const Fp4Operand w0{a.w->codes, a.w->pieces, a.w->params, a.bias};
     const Fp4Operand w1 = GATED ? Fp4Operand{a.up->codes, a.up->pieces, a.up->params, a.bias_up} : w0;
-    return launch_maybe_pdl(gemv_fp4_kernel<NT, RT, NV, GATED, YT>, dim3((unsigned)((tiles + RT - 1) / RT)), dim3(kGemv4Warps * 32), 0, ctx->stream, a.pdl, w0,
-                            w1, terms, exps, counts, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy, a.epilogue);
+    auto kern = gemv_fp4_kernel<NT, NV, GATED, XS, T, YT>;
+    static std::atomic<unsigned long long> attr_done{0};
+    int rc = set_smem_attr_once(ctx, kern, kGemv4RingBytes + (XS ? kGemv4StagedBytes : 0), attr_done);
+    if (rc != SHREWQ_OK) return rc;
+    SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(kern, dim3((unsigned)(tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count)), dim3(kGemv4Threads), smem, ctx->stream,
+                                          a.pdl, w0, w1, x, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy, a.epilogue));
+    ctx->launches += 1;
+    SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
+    return SHREWQ_OK;
 }
 
-template <bool NV, bool GATED, typename YT>
-cudaError_t launch_tokens(shrewq_ctx *ctx, const Fp4Forward &a, const uint16_t *terms, const int *exps, const int *counts) {
-    if (a.M <= 8) return launch_one<1, 1, NV, GATED, YT>(ctx, a, terms, exps, counts);
-    if (a.M <= 16) return launch_one<2, 1, NV, GATED, YT>(ctx, a, terms, exps, counts);
-    return launch_one<4, 1, NV, GATED, YT>(ctx, a, terms, exps, counts);
+template <int NT, bool XS, typename T>
+int launch_weights(shrewq_ctx *ctx, const Fp4Forward &a, const Gemv4X<T> &x, size_t staged) {
+    const bool nv = a.w->nv, f32 = a.y_dtype == SHREWQ_F32;
+#define SHREWQ_GEMV4(NV_, G_)                                                                 \
+    return f32 ? launch_one<NT, NV_, G_, XS, T, float>(ctx, a, x, staged) : launch_one<NT, NV_, G_, XS, T, __nv_bfloat16>(ctx, a, x, staged)
+    if (nv && a.up) SHREWQ_GEMV4(true, true);
+    if (nv) SHREWQ_GEMV4(true, false);
+    if (a.up) SHREWQ_GEMV4(false, true);
+    SHREWQ_GEMV4(false, false);
+#undef SHREWQ_GEMV4
+}
+
+template <typename T>
+int launch_typed(shrewq_ctx *ctx, const Fp4Forward &a) {
+    const size_t steps = (a.K + 127) / 128;
+    Gemv4X<T> x{static_cast<const T *>(a.x), (reinterpret_cast<uintptr_t>(a.x) % (8 * sizeof(T))) == 0 && a.K % 8 == 0, nullptr, nullptr, nullptr};
+    // a few tokens are staged by the CTAs themselves: one launch, no workspace
+    const size_t staged = XTerms<T>::kMost * steps * 256 * a.M;
+    if (a.M <= (size_t)kGemv4MaxStaged && staged <= (size_t)kGemv4StagedBytes) return launch_weights<1, true, T>(ctx, a, x, staged);
+    const int NT = a.M <= 8 ? 1 : a.M <= 16 ? 2 : 4;
+    const size_t plane = (size_t)NT * steps * 2048;
+    int rc = ensure_xsplit(ctx, XTerms<T>::kMost * plane + 2 * a.M * sizeof(int));
+    if (rc != SHREWQ_OK) return rc;
+    char *base = static_cast<char *>(ctx->xsplit);
+    int *exps = reinterpret_cast<int *>(base + XTerms<T>::kMost * plane), *counts = exps + a.M;
+    SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(stage_f16_kernel<T>, dim3((unsigned)(8 * NT)), dim3((unsigned)(steps >= 16 ? 256 : (steps * 16 + 31) / 32 * 32)), 0, ctx->stream,
+                                          ctx->tuning.pdl != 0, x.x, (int)a.M, (int)a.K, x.vec_ok, reinterpret_cast<uint4 *>(base), exps, counts));
+    ctx->launches += 1;
+    x.terms = reinterpret_cast<const uint4 *>(base);
+    x.exps = exps;
+    x.counts = counts;
+    if (NT == 1) return launch_weights<1, false, T>(ctx, a, x, 0);
+    if (NT == 2) return launch_weights<2, false, T>(ctx, a, x, 0);
+    return launch_weights<4, false, T>(ctx, a, x, 0);
 }
 
 }  // namespace
 
 int launch_gemv_fp4(shrewq_ctx *ctx, const Fp4Forward &a) {
-    const size_t Kp = (a.K + 31) / 32 * 32, plane = a.M * Kp * sizeof(uint16_t);
-    int rc = ensure_xsplit(ctx, 3 * plane + 2 * a.M * sizeof(int));
-    if (rc != SHREWQ_OK) return rc;
-    char *base = static_cast<char *>(ctx->xsplit);
-    uint16_t *terms = reinterpret_cast<uint16_t *>(base);
-    int *exps = reinterpret_cast<int *>(base + 3 * plane), *counts = exps + a.M;
-    const bool pdl = ctx->tuning.pdl != 0;
-    const unsigned threads = (unsigned)(Kp / 8 >= 256 ? 256 : (Kp / 8 + 31) / 32 * 32);
-    const size_t esz = a.x_dtype == SHREWQ_F32 ? 4 : 2;
-    const int vec_ok = (reinterpret_cast<uintptr_t>(a.x) % (8 * esz)) == 0 && a.K % 8 == 0;
-    if (a.x_dtype == SHREWQ_F32)
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(stage_f16_kernel<float>, dim3((unsigned)a.M), dim3(threads), 0, ctx->stream, pdl, static_cast<const float *>(a.x),
-                                              (int)a.M, (int)a.K, (int)Kp, vec_ok, terms, exps, counts));
-    else
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(stage_f16_kernel<__nv_bfloat16>, dim3((unsigned)a.M), dim3(threads), 0, ctx->stream, pdl,
-                                              static_cast<const __nv_bfloat16 *>(a.x), (int)a.M, (int)a.K, (int)Kp, vec_ok, terms, exps, counts));
-    cudaError_t e;
-    const bool nv = a.w->nv, gated = a.up != nullptr, f32 = a.y_dtype == SHREWQ_F32;
-#define SHREWQ_GEMV4(NV_, G_)                                                                      \
-    e = f32 ? launch_tokens<NV_, G_, float>(ctx, a, terms, exps, counts) : launch_tokens<NV_, G_, __nv_bfloat16>(ctx, a, terms, exps, counts)
-    if (nv && gated) SHREWQ_GEMV4(true, true);
-    else if (nv) SHREWQ_GEMV4(true, false);
-    else if (gated) SHREWQ_GEMV4(false, true);
-    else SHREWQ_GEMV4(false, false);
-#undef SHREWQ_GEMV4
-    SHREWQ_CUDA_TRY(ctx, e);
-    ctx->launches += 2;
-    SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
-    return SHREWQ_OK;
+    return a.x_dtype == SHREWQ_F32 ? launch_typed<float>(ctx, a) : launch_typed<__nv_bfloat16>(ctx, a);
 }
 
 int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, bool nv, uint8_t *out,

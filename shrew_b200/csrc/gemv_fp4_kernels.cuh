@@ -9,20 +9,24 @@
 //   NV: code * E4M3 scale has 6 significant bits between 2^-10 and 2688;
 //   MX: code * 2^d is exact for d in [-14, 13], so the scales of a tensor are taken in windows of 28 octaves below the largest one; a
 //       tensor whose scales span more (the handle knows their range) takes a pass over its codes for every window.
-// Activations are f16 too: a pass before this kernel (stage_f16_kernel) scales every token by a power of two to [2^14, 2^15) and writes
-// f16 terms: bf16 values down to 2^-32 of their token's largest are exact in the first; where a token has smaller ones a second term
-// holds what the first left, times 2^32.  f32 values take three terms of 11 bits each.  The kernel passes over the codes once for every
-// term that any token needs, and adds the passes' sums with their weights in f32.  Products are exact, sums are f32.
+// Activations are f16 too: staging scales every token by a power of two to [2^14, 2^15) and forms f16 terms: bf16 values down to 2^-32
+// of their token's largest are exact in the first; where a token has smaller ones a second term holds what the first left, times 2^32.
+// f32 values take three terms of 11 bits each.  The kernel passes over the codes once for every term that any token needs, and adds the
+// passes' sums with their weights in f32.  Products are exact, sums are f32.
 //
-// Mapping.  A CTA of 8 warps takes RT tiles of 16 rows (GATED: 8 gate rows and the 8 up rows of the same channels); the warps deal the
-// k range in steps of 128 codes.  mma.sync.m16n8k16 with the weights as the A operand: lane (g = lane / 4, t = lane % 4) loads 16
-// bytes = 32 consecutive codes (one MX block, two NV blocks: the scale is the lane's own) of rows g and g + 8 and the 32 activations
-// of the same k for token g; MMA step i uses the codes 4i .. 4i+3 of that run for A and B alike.  Four steps are requested at a time, the
-// next four before these are used, so that 16 warps keep 64 KB of codes in flight on an SM.  The rows of a tile are 4 neighbours each
-// from the 4 groups of 32 that share 16 bytes of scales in the handle's copy (scale_piece_offset), so that scale sectors are used whole.
-// The warps' sums meet in shared memory in a fixed order.
+// Mapping.  One CTA of 16 warps an SM walks over tiles of 16 rows (GATED: 8 gate rows and the 8 up rows of the same channels); the
+// warps deal the k range in steps of 128 codes.  mma.sync.m16n8k16 with the weights as the A operand: lane (g = lane / 4, t = lane % 4)
+// takes 16 bytes = 32 consecutive codes (one MX block, two NV blocks: the scale is the lane's own) of rows g and g + 8 and the 32
+// activations of the same k for token g; MMA step i uses the codes 4i .. 4i+3 of that run for A and B alike.
+// Codes and scales come by cp.async, every lane its own bytes into its own slots of a ring, several steps ahead and across tiles: no
+// register holds a byte in flight, no barrier guards one, and an SM has some 60 KB on their way.  The rows of a tile are 4 neighbours
+// each from the 4 groups of 32 that share 16 bytes of scales in the handle's copy (scale_piece_offset): scale sectors are used whole.
+// Activations: XS (a few tokens): every CTA stages them in its shared memory while its first codes are on their way: one launch.  Else
+// stage_f16_kernel writes them to global memory in the order of the MMA's B fragments (512 bytes a load, whole lines), from where they
+// come through L1, which keeps them from one tile to the next.
+// The warps' sums of a tile meet in shared memory in a fixed order.
 //
-// Programmatic dependent launch: the first codes and scales are requested before the wait for the previous kernel.
+// Programmatic dependent launch: the ring is filled before the wait for the previous kernel.
 //
 // Device code only (PTX behind ptx_fp4.cuh and ptx_small.cuh): also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once
@@ -36,8 +40,13 @@
 namespace shrewq {
 namespace {
 
-constexpr int kGemv4Warps = 8;
-constexpr int kMxWindow = 28;  // octaves of MX scales that one pass takes
+constexpr int kGemv4Warps = 16, kGemv4Threads = kGemv4Warps * 32;
+constexpr int kGemv4Depth = 4;         // steps of the ring
+constexpr int kGemv4SlotBytes = 40;    // of a lane and step: 16 bytes of codes of two rows, a scale word for each
+constexpr int kGemv4RingBytes = kGemv4Warps * kGemv4Depth * 32 * kGemv4SlotBytes;
+constexpr int kGemv4MaxStaged = 4;     // tokens that a CTA stages itself (XS) ...
+constexpr int kGemv4StagedBytes = 96 * 1024;  // ... in at most this much shared memory
+constexpr int kMxWindow = 28;          // octaves of MX scales that one pass takes
 
 // What the kernels need of one weight matrix (device pointers; params and pieces belong to the handle)
 struct Fp4Operand {
@@ -48,83 +57,101 @@ struct Fp4Operand {
 };
 
 // ---- activations -> f16 terms -----------------------------------------------------------------------------------------------
-// A CTA a token.  terms: [3][M][Kp] f16 (Kp = K to whole 32s, zeros beyond K); exps[m]: the power of two that the token was divided
-// by; counts[m]: terms in use.  Infinities and NaNs stay what they are in the first term and are 0 in the others.
+// Terms of f32 and bf16 activations, and the power of two between them
 template <typename T>
-__global__ void __launch_bounds__(256)
-stage_f16_kernel(const T *__restrict__ x, int M, int K, int Kp, int vec_ok, uint16_t *__restrict__ terms, int *__restrict__ exps,
-                 int *__restrict__ counts) {
-    pdl_launch_dependents();
-    __shared__ unsigned int s_max[8], s_more[8];
-    pdl_wait();
-    const int m = blockIdx.x, threads = (int)blockDim.x, warps = threads >> 5;
-    const T *row = x + (size_t)m * K;
-    const int groups = Kp >> 3;
-    unsigned int top = 0;  // largest exponent field of a finite value
-    for (int i = threadIdx.x; i < groups; i += threads) {
-        float v[8];
-        if (vec_ok && i * 8 + 8 <= K) load_vec8<T>(row + i * 8, v);
-        else load_guarded8<T>(row + i * 8, i * 8 < K ? (size_t)(K - i * 8) : 0, v);
+struct XTerms {
+    static constexpr int kMost = sizeof(T) == 4 ? 3 : 2;
+    static constexpr int kOctaves = sizeof(T) == 4 ? 11 : 32;
+};
+template <typename T>
+__device__ __forceinline__ void load_token8(const T *row, int i, int K, int vec_ok, float *v) {
+    if (vec_ok && i * 8 + 8 <= K) load_vec8<T>(row + i * 8, v);
+    else load_guarded8<T>(row + i * 8, i * 8 < K ? (size_t)(K - i * 8) : 0, v);
+}
+// largest exponent field of finite values among v[8] and top
+__device__ __forceinline__ unsigned int top_exponent(const float *v, unsigned int top) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned int e = (__float_as_uint(v[j]) >> 23) & 0xFFu;
-            top = e < 255u && e > top ? e : top;
+    for (int j = 0; j < 8; ++j) {
+        const unsigned int e = (__float_as_uint(v[j]) >> 23) & 0xFFu;
+        top = e < 255u && e > top ? e : top;
+    }
+    return top;
+}
+__device__ __forceinline__ unsigned int warp_max(unsigned int v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned int other = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        v = other > v ? other : v;
+    }
+    return v;
+}
+// v[8] -> terms of 8 f16; returns whether the first term left anything.  Infinities and NaNs stay what they are in the first term and
+// are 0 in the others.  top: the token's largest exponent field: x is multiplied by 2^(141 - top), as two factors that are ordinary numbers
+template <typename T>
+__device__ __forceinline__ bool f16_terms(float *v, unsigned int top, uint4 *out) {
+    const int up = 141 - (int)top;  // -113 .. 141
+    const float f0 = __uint_as_float((uint32_t)(127 + (up > 100 ? 100 : up)) << 23), f1 = __uint_as_float((uint32_t)(127 + (up > 100 ? up - 100 : 0)) << 23);
+    const float next = sizeof(T) == 4 ? 2048.0f : 4294967296.0f;
+    bool more = false;
+    uint32_t w[XTerms<T>::kMost][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a = v[2 * j] * f0 * f1, b = v[2 * j + 1] * f0 * f1;
+#pragma unroll
+        for (int t = 0; t < XTerms<T>::kMost; ++t) {
+            w[t][j] = pack_f16x2_rn(b, a);
+            float ha, hb;
+            f32x2_of_f16x2(w[t][j], ha, hb);
+            a = ha - ha == 0.0f ? (a - ha) * next : 0.0f;
+            b = hb - hb == 0.0f ? (b - hb) * next : 0.0f;
+            if (t == 0) more = more || a != 0.0f || b != 0.0f;
         }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned int other = __shfl_xor_sync(0xFFFFFFFFu, top, o);
-        top = other > top ? other : top;
+    for (int t = 0; t < XTerms<T>::kMost; ++t) out[t] = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
+    return more;
+}
+
+// A CTA a token of the padded batch (8 tokens a group; beyond M zeros).  terms: [kMost][token groups][steps][4][32 lanes][8] f16 in the order
+// of the B fragments: piece q of lane 4 g + t holds k = 128 step + 32 t + 8 q .. + 7 of token g.  exps[m]: the power of two that the token
+// was divided by; counts[m]: terms in use.
+template <typename T>
+__global__ void __launch_bounds__(256)
+stage_f16_kernel(const T *__restrict__ x, int M, int K, int vec_ok, uint4 *__restrict__ terms, int *__restrict__ exps, int *__restrict__ counts) {
+    pdl_launch_dependents();
+    __shared__ unsigned int s_max[8], s_more[8];
+    const int m = blockIdx.x, threads = (int)blockDim.x, warps = threads >> 5, steps = (K + 127) >> 7, groups = steps << 4;
+    const size_t plane = (size_t)(gridDim.x >> 3) * steps * 128;  // 16-byte pieces of a term
+    pdl_wait();
+    const T *row = x + (size_t)m * K;
+    unsigned int top = 0, more = 0;
+    if (m < M) {
+        for (int i = threadIdx.x; i < groups; i += threads) {
+            float v[8];
+            load_token8<T>(row, i, K, vec_ok, v);
+            top = top_exponent(v, top);
+        }
     }
+    top = warp_max(top);
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
     __syncthreads();
     for (int w = 0; w < warps; ++w) top = s_max[w] > top ? s_max[w] : top;
-    // x * 2^(14 - (top - 127)), in two factors that are both ordinary numbers
-    const int up = 141 - (int)top;                       // -113 .. 141
-    const float f0 = __uint_as_float((uint32_t)(127 + (up > 100 ? 100 : up)) << 23), f1 = __uint_as_float((uint32_t)(127 + (up > 100 ? up - 100 : 0)) << 23);
-    constexpr bool kWide = sizeof(T) == 4;               // f32: three terms, 11 octaves apart; bf16: two, 32 apart
-    const float next = kWide ? 2048.0f : 4294967296.0f;
-    const size_t plane = (size_t)M * Kp;
-    unsigned int more = 0;
     for (int i = threadIdx.x; i < groups; i += threads) {
         float v[8];
-        if (vec_ok && i * 8 + 8 <= K) load_vec8<T>(row + i * 8, v);
-        else load_guarded8<T>(row + i * 8, i * 8 < K ? (size_t)(K - i * 8) : 0, v);
-        uint32_t t0[4], t1[4], t2[4];
+        load_token8<T>(row, i, m < M ? K : 0, vec_ok, v);
+        uint4 out[XTerms<T>::kMost];
+        more |= f16_terms<T>(v, top, out) ? 1u : 0u;
+        const size_t at = ((size_t)((m >> 3) * steps + (i >> 4)) * 4 + (i & 3)) * 32 + (m & 7) * 4 + ((i >> 2) & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float a = v[2 * j] * f0 * f1, b = v[2 * j + 1] * f0 * f1, ha, hb;
-            const auto rest = [&](float &r, float h) {  // what a term left, for the next one
-                r = (h - h == 0.0f) ? (r - h) * next : 0.0f;
-            };
-            t0[j] = pack_f16x2_rn(b, a);
-            f32x2_of_f16x2(t0[j], ha, hb);
-            rest(a, ha);
-            rest(b, hb);
-            more |= (a != 0.0f || b != 0.0f) ? 1u : 0u;
-            t1[j] = pack_f16x2_rn(b, a);
-            if constexpr (kWide) {
-                f32x2_of_f16x2(t1[j], ha, hb);
-                rest(a, ha);
-                rest(b, hb);
-                t2[j] = pack_f16x2_rn(b, a);
-            } else {
-                t2[j] = 0;
-            }
-        }
-        uint16_t *dst = terms + (size_t)m * Kp + i * 8;
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
-        *reinterpret_cast<uint4 *>(dst + plane) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
-        if constexpr (kWide) *reinterpret_cast<uint4 *>(dst + 2 * plane) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+        for (int t = 0; t < XTerms<T>::kMost; ++t) terms[t * plane + at] = out[t];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) more |= __shfl_xor_sync(0xFFFFFFFFu, more, o);
+    more = warp_max(more);
     if ((threadIdx.x & 31) == 0) s_more[threadIdx.x >> 5] = more;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && m < M) {
         for (int w = 0; w < warps; ++w) more |= s_more[w];
-        exps[m] = -up;
-        counts[m] = more ? (kWide ? 3 : 2) : 1;
+        exps[m] = (int)top - 141;
+        counts[m] = more ? XTerms<T>::kMost : 1;
     }
 }
 
@@ -154,56 +181,115 @@ __device__ __forceinline__ int gemv4_row(int tile, int i) {
     return (tile / kTiles) * 128 + (tile % kTiles) * (1 << kShift) + (i & ((1 << kShift) - 1)) + 32 * (i >> kShift);
 }
 
-// NT: token groups of 8 (M <= 8 * NT); RT: tiles of 16 rows a CTA
-template <int NT, int RT, bool NV, bool GATED, typename YT>
-__global__ void __launch_bounds__(kGemv4Warps * 32, 2)
-gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const uint16_t *__restrict__ terms, const int *__restrict__ exps, const int *__restrict__ counts,
-                YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
-    constexpr int SB = RT == 1 && NT == 1 ? 4 : 2;  // steps requested together (registers)
-    constexpr int kRows = GATED ? 8 : 16;
-    __shared__ float s_red[kGemv4Warps][RT][NT][4][32];
+// Where the activations are: staged by stage_f16_kernel (terms, exps, counts), or, XS, still [M][K] of T
+template <typename T>
+struct Gemv4X {
+    const T *x;
+    int vec_ok;
+    const uint4 *terms;
+    const int *exps, *counts;
+};
+
+// NT: token groups of 8 (M <= 8 * NT; XS: M <= kGemv4MaxStaged)
+template <int NT, bool NV, bool GATED, bool XS, typename T, typename YT>
+__global__ void __launch_bounds__(kGemv4Threads, 1)
+gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
+    static_assert(!XS || NT == 1, "a few tokens");
+    constexpr int kRows = GATED ? 8 : 16, kBufs = NT >= 4 ? 1 : 2;  // (48 KB of static shared memory)
+    SHREWQ_DYNAMIC_SMEM(uint8_t, smem);  // ring, then the staged activations (XS)
+    __shared__ float s_red[kBufs][kGemv4Warps][NT][4][32];
+    __shared__ unsigned int s_max[kGemv4MaxStaged][kGemv4Warps], s_more[kGemv4Warps];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int Kp = (K + 31) & ~31, pitch = Kp >> 1;
     const int steps = (Kp + 127) >> 7;
     const size_t pieces = (size_t)((K + 255) >> 8) * (NV ? 4 : 2);
-    const uint8_t *code_ptr[RT][2], *scale_ptr[RT][2];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
+    const int tiles = ((N + 127) >> 7) * (GATED ? 16 : 8);
+    const int mine = (steps - warp + kGemv4Warps - 1) / kGemv4Warps;  // this warp's steps of a tile (not negative: warp < 16)
+
+    // ---- the ring: item i of this warp is its step i % mine of the CTA's tile i / mine ----
+    const uint32_t ring = smem_offset(smem) + (uint32_t)((warp * kGemv4Depth * 32 + lane) * 16);
+    constexpr uint32_t kRowH = kGemv4Warps * kGemv4Depth * 32 * 16;   // codes of rows g, codes of rows g + 8, scale words of both
+    const uint32_t ring_scales = smem_offset(smem) + 2 * kRowH + (uint32_t)((warp * kGemv4Depth * 32 + lane) * 8);
+    const uint8_t *code_ptr[2], *scale_ptr[2];
+    int next_tile = (int)blockIdx.x, next_step = warp, slot_in = 0;
+    auto aim = [&](int tile) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const Fp4Operand &w = GATED && h ? w1 : w0;
-            const int row = gemv4_row<GATED>((int)blockIdx.x * RT + r, GATED ? g : g + 8 * h);
+            const int row = gemv4_row<GATED>(tile, GATED ? g : g + 8 * h);
             const int safe = row < N ? row : N - 1;  // rows past the end are computed from another row and dropped
-            code_ptr[r][h] = w.codes + (size_t)safe * pitch + 16 * t;
-            scale_ptr[r][h] = w.pieces + scale_piece_offset((size_t)safe, NV ? 4 * (t >> 1) : 0, pieces);
-        }
-
-    uint4 code[2][SB][RT][2];
-    uint32_t scale[2][SB][RT][2];
-    auto request = [&](uint4 (&c)[SB][RT][2], uint32_t (&s)[SB][RT][2], int first) {
-#pragma unroll
-        for (int b = 0; b < SB; ++b) {
-            const int step = first + b * kGemv4Warps;
-            const bool in = step < steps, whole = in && step * 64 + 16 * t < pitch;
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    c[b][r][h] = whole ? ld_stream_16(code_ptr[r][h] + (size_t)step * 64) : make_uint4(0, 0, 0, 0);
-                    s[b][r][h] = in ? __ldg(reinterpret_cast<const uint32_t *>(scale_ptr[r][h] + (size_t)step * (NV ? 1024 : 512))) : 0u;
-                }
+            code_ptr[h] = w.codes + (size_t)safe * pitch + 16 * t;
+            scale_ptr[h] = w.pieces + scale_piece_offset((size_t)safe, NV ? 4 * (t >> 1) : 0, pieces);
         }
     };
-    request(code[0], scale[0], warp);
+    // requests the next item, or nothing behind the last one; every call closes a group of copies
+    auto request = [&]() {
+        if (next_step < steps && next_tile < tiles) {
+            const bool in = next_step * 64 + 16 * t < pitch;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                copy_async_16(ring + h * kRowH + slot_in * 512, code_ptr[h] + (in ? (size_t)next_step * 64 : 0), in);
+                copy_async_4(ring_scales + slot_in * 256 + h * 4, scale_ptr[h] + (size_t)next_step * (NV ? 1024 : 512), true);
+            }
+            slot_in = slot_in + 1 == kGemv4Depth ? 0 : slot_in + 1;
+            next_step += kGemv4Warps;
+            if (next_step >= steps) {
+                next_step = warp;
+                next_tile += (int)gridDim.x;
+                if (next_tile < tiles) aim(next_tile);
+            }
+        }
+        copy_async_commit();
+    };
+    // passes over a tile's codes: a ring that is read more than once would have to be filled again, so the passes are outermost
+    aim(next_tile);
+#pragma unroll
+    for (int i = 0; i < kGemv4Depth - 1; ++i) request();
     pdl_wait();  // activations may be the previous kernel's output, which may also still read y
 
+    // ---- activations ----
     int n_terms = 1;
-    for (int m = lane; m < M; m += 32) n_terms = counts[m];
+    const uint4 *sx = reinterpret_cast<const uint4 *>(smem + kGemv4RingBytes);  // XS: [terms][steps][4][4 t][M]
+    unsigned int tops[kGemv4MaxStaged];
+    if constexpr (XS) {
+        const int groups = steps << 4;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const int other = __shfl_xor_sync(0xFFFFFFFFu, n_terms, o);
-        n_terms = other > n_terms ? other : n_terms;
+        for (int m = 0; m < kGemv4MaxStaged; ++m) {
+            tops[m] = 0;
+            if (m < M)
+                for (int i = threadIdx.x; i < groups; i += kGemv4Threads) {
+                    float v[8];
+                    load_token8<T>(xs.x + (size_t)m * K, i, K, xs.vec_ok, v);
+                    tops[m] = top_exponent(v, tops[m]);
+                }
+            tops[m] = warp_max(tops[m]);
+            if (lane == 0) s_max[m][warp] = tops[m];
+        }
+        __syncthreads();
+        unsigned int more = 0;
+        uint4 *dst = reinterpret_cast<uint4 *>(smem + kGemv4RingBytes);
+#pragma unroll
+        for (int m = 0; m < kGemv4MaxStaged; ++m) {
+            for (int w = 0; w < kGemv4Warps; ++w) tops[m] = s_max[m][w] > tops[m] ? s_max[m][w] : tops[m];
+            if (m < M)
+                for (int i = threadIdx.x; i < groups; i += kGemv4Threads) {
+                    float v[8];
+                    load_token8<T>(xs.x + (size_t)m * K, i, K, xs.vec_ok, v);
+                    uint4 out[XTerms<T>::kMost];
+                    more |= f16_terms<T>(v, tops[m], out) ? 1u : 0u;
+#pragma unroll
+                    for (int e = 0; e < XTerms<T>::kMost; ++e)
+                        dst[(size_t)(((e * steps + (i >> 4)) * 4 + (i & 3)) * 4 + ((i >> 2) & 3)) * M + m] = out[e];
+                }
+        }
+        more = warp_max(more);
+        if (lane == 0) s_more[warp] = more;
+        __syncthreads();
+        for (int w = 0; w < kGemv4Warps; ++w) n_terms = s_more[w] ? XTerms<T>::kMost : n_terms;
+    } else {
+        for (int m = lane; m < M; m += 32) n_terms = xs.counts[m];
+        n_terms = (int)warp_max((unsigned int)n_terms);
     }
     int top = 0, windows = 1;
     if constexpr (!NV) {
@@ -215,130 +301,121 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const uint16_t *__restrict__ terms
         }
         windows = top >= low ? (top - low) / kMxWindow + 1 : 1;
     }
+    const int passes = n_terms * windows;
+    const size_t x_plane = (size_t)NT * steps * 128;
 
-    float total[RT][NT][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
+    // One step: codes (two rows), scale words, activations -> acc
+    auto multiply = [&](float (&acc)[NT][4], uint4 ca, uint4 cb, uint32_t sa, uint32_t sb, int step, int term, int first) {
+        uint4 xv[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) total[r][n][i] = 0.0f;
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (XS) xv[n][q] = g < M ? sx[(size_t)(((term * steps + step) * 4 + q) * 4 + t) * M + g] : make_uint4(0, 0, 0, 0);
+                else xv[n][q] = __ldg(xs.terms + term * x_plane + ((size_t)(n * steps + step) * 4 + q) * 32 + lane);
+            }
+        uint32_t f[2][2];
+        if constexpr (NV) {  // blocks 2t and 2t + 1 of the step's 8: half t % 2 of word t / 2, which this lane loaded
+            const uint32_t a2 = cvt_f16x2_e4m3(sa >> (16 * (t & 1))), b2 = cvt_f16x2_e4m3(sb >> (16 * (t & 1)));
+            f[0][0] = dup_lo(a2);
+            f[0][1] = dup_hi(a2);
+            f[1][0] = dup_lo(b2);
+            f[1][1] = dup_hi(b2);
+        } else {
+            f[0][0] = f[0][1] = mx_scale_f16x2(sa, t, first);
+            f[1][0] = f[1][1] = mx_scale_f16x2(sb, t, first);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // words of 8 codes
+            uint32_t ha[4], hb[4];
+            cvt_f16x8_e2m1(q == 0 ? ca.x : q == 1 ? ca.y : q == 2 ? ca.z : ca.w, ha);
+            cvt_f16x8_e2m1(q == 0 ? cb.x : q == 1 ? cb.y : q == 2 ? cb.z : cb.w, hb);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                ha[p] = mul_f16x2(ha[p], f[0][q >> 1]);
+                hb[p] = mul_f16x2(hb[p], f[1][q >> 1]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma_f16_16816(acc[n], ha[0], hb[0], ha[1], hb[1], xv[n][q].x, xv[n][q].y);
+                mma_f16_16816(acc[n], ha[2], hb[2], ha[3], hb[3], xv[n][q].z, xv[n][q].w);
+            }
+        }
+    };
 
-    const int passes = n_terms * windows;
-    for (int pass = 0; pass < passes; ++pass) {
-        const int term = pass / windows, window = pass % windows;
-        const int first = top - (kMxWindow - 1) - kMxWindow * window;  // MX: the byte of 2^-14 in this window
-        const uint16_t *xrow[NT];
+    const float alpha0 = NV ? w0.params->tensor_scale : 1.0f, alpha1 = GATED && NV ? w1.params->tensor_scale : 1.0f;
+    int slot = 0, turn = 0;
+    for (int tile = (int)blockIdx.x; tile < tiles; tile += (int)gridDim.x, turn ^= kBufs - 1) {
+        float total[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) xrow[n] = 8 * n + g < M ? terms + ((size_t)term * M + 8 * n + g) * Kp + 32 * t : nullptr;
-        float acc[RT][NT][4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+            for (int i = 0; i < 4; ++i) total[n][i] = 0.0f;
+        for (int s = 0; s < mine; ++s) {
+            request();
+            copy_async_wait<kGemv4Depth - 1>();
+            const uint8_t *at = smem + (size_t)(warp * kGemv4Depth * 32 + slot * 32 + lane) * 16;
+            const uint4 ca = *reinterpret_cast<const uint4 *>(at), cb = *reinterpret_cast<const uint4 *>(at + kRowH);
+            const uint2 sc = *reinterpret_cast<const uint2 *>(smem + 2 * kRowH + (size_t)(warp * kGemv4Depth * 32 + slot * 32 + lane) * 8);
+            slot = slot + 1 == kGemv4Depth ? 0 : slot + 1;
+            const int step = warp + s * kGemv4Warps;
+            if (passes == 1) {
+                multiply(total, ca, cb, sc.x, sc.y, step, 0, top - (kMxWindow - 1));
+            } else {
+                for (int pass = 0; pass < passes; ++pass) {
+                    const int term = pass / windows, window = pass % windows;
+                    float acc[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
-        auto multiply = [&](uint4 (&c)[SB][RT][2], uint32_t (&s)[SB][RT][2], int first_step) {
+                        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+                    multiply(acc, ca, cb, sc.x, sc.y, step, term, top - (kMxWindow - 1) - kMxWindow * window);
+                    // weight of this pass's sums: 2^-11 or 2^-32 for each term, 2^-28 for each window
+                    const float weight = ldexpf(1.0f, -XTerms<T>::kOctaves * term - kMxWindow * window);
 #pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                const int step = first_step + b * kGemv4Warps;
-                if (step >= steps) break;
-                const int k = step * 128 + 32 * t;
-                uint4 xv[NT][4];
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        xv[n][q] = xrow[n] && k < Kp ? __ldg(reinterpret_cast<const uint4 *>(xrow[n] + step * 128) + q) : make_uint4(0, 0, 0, 0);
-                uint32_t f[RT][2][2];
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (NV) {  // blocks 2t and 2t + 1 of the step's 8: half t % 2 of word t / 2, which this lane loaded
-                            const uint32_t two = cvt_f16x2_e4m3(s[b][r][h] >> (16 * (t & 1)));
-                            f[r][h][0] = dup_lo(two);
-                            f[r][h][1] = dup_hi(two);
-                        } else {
-                            f[r][h][0] = f[r][h][1] = mx_scale_f16x2(s[b][r][h], t, first);
-                        }
-                    }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {  // words of 8 codes
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        const uint4 &ca = c[b][r][0], &cb = c[b][r][1];
-                        const uint32_t wa = q == 0 ? ca.x : q == 1 ? ca.y : q == 2 ? ca.z : ca.w, wb = q == 0 ? cb.x : q == 1 ? cb.y : q == 2 ? cb.z : cb.w;
-                        uint32_t ha[4], hb[4];
-                        cvt_f16x8_e2m1(wa, ha);
-                        cvt_f16x8_e2m1(wb, hb);
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            ha[p] = mul_f16x2(ha[p], f[r][0][q >> 1]);
-                            hb[p] = mul_f16x2(hb[p], f[r][1][q >> 1]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma_f16_16816(acc[r][n], ha[0], hb[0], ha[1], hb[1], xv[n][q].x, xv[n][q].y);
-                            mma_f16_16816(acc[r][n], ha[2], hb[2], ha[3], hb[3], xv[n][q].z, xv[n][q].w);
-                        }
-                    }
+                        for (int i = 0; i < 4; ++i) total[n][i] = __fmaf_rn(acc[n][i], weight, total[n][i]);
                 }
             }
-        };
-        for (int step = warp; step < steps; step += 2 * SB * kGemv4Warps) {
-            const int second = step + SB * kGemv4Warps;
-            request(code[1], scale[1], second);
-            multiply(code[0], scale[0], step);
-            // (behind the last steps: the first ones again, for a pass that may follow)
-            const int third = second + SB * kGemv4Warps;
-            if (third < steps || pass + 1 < passes) request(code[0], scale[0], third < steps ? third : warp);
-            multiply(code[1], scale[1], second);
         }
-        // weight of this pass's sums: 2^-11 or 2^-32 for each term, 2^-28 for each window
-        const float weight = pass == 0 ? 1.0f : ldexpf(1.0f, -(n_terms == 3 ? 11 : 32) * term - kMxWindow * window);
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) total[r][n][i] = __fmaf_rn(acc[r][n][i], weight, total[r][n][i]);
-    }
-
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
+        if (kBufs == 1 && tile != (int)blockIdx.x) __syncthreads();  // the tile before has been read
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s_red[warp][r][n][i][lane] = total[r][n][i];
-    __syncthreads();
+            for (int i = 0; i < 4; ++i) s_red[turn][warp][n][i][lane] = total[n][i];
+        __syncthreads();  // (with two buffers a warp writes this one again only behind the next barrier)
 
-    // accumulator (lane, i) of token group n: row (lane / 4) + (i >= 2 ? 8 : 0), token 8 n + 2 (lane % 4) + (i & 1)
-    const float a0 = NV ? w0.params->tensor_scale : 1.0f, a1 = GATED && NV ? w1.params->tensor_scale : 1.0f;
-    for (int o = threadIdx.x; o < kRows * RT * 8 * NT; o += kGemv4Warps * 32) {
-        const int i = o % kRows, r = o / kRows % RT, m = o / (kRows * RT);
-        const int n = gemv4_row<GATED>((int)blockIdx.x * RT + r, i);
-        if (n >= N || m >= M) continue;
-        const int ln = (i & 7) * 4 + ((m & 7) >> 1), lo = (m & 1) + ((i & 8) ? 2 : 0);
-        float s0 = 0.0f, s1 = 0.0f;
+        // accumulator (lane, i) of token group n: row (lane / 4) + (i >= 2 ? 8 : 0), token 8 n + 2 (lane % 4) + (i & 1)
+        for (int o = threadIdx.x; o < kRows * 8 * NT; o += kGemv4Threads) {
+            const int i = o % kRows, m = o / kRows;
+            const int n = gemv4_row<GATED>(tile, i);
+            if (n >= N || m >= M) continue;
+            const int ln = (i & 7) * 4 + ((m & 7) >> 1), lo = (m & 1) + ((i & 8) ? 2 : 0);
+            float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kGemv4Warps; ++w) {
-            s0 += s_red[w][r][m >> 3][lo][ln];
-            if constexpr (GATED) s1 += s_red[w][r][m >> 3][2 + (m & 1)][ln];
+            for (int w = 0; w < kGemv4Warps; ++w) {
+                s0 += s_red[turn][w][m >> 3][lo][ln];
+                if constexpr (GATED) s1 += s_red[turn][w][m >> 3][2 + (m & 1)][ln];
+            }
+            int exponent;
+            if constexpr (XS) exponent = (int)(m == 0 ? tops[0] : m == 1 ? tops[1] : m == 2 ? tops[2] : tops[3]) - 141;
+            else exponent = xs.exps[m];
+            // back from the token's power of two and, for MX, from the window's: the first window has its largest scale, 2^(top - 127), at 2^13
+            const int back = exponent + (NV ? 0 : top - 127 - 13);
+            float v = ldexpf(s0, back) * alpha0;
+            if (w0.bias) v += w0.bias[n];
+            if constexpr (GATED) {
+                float u = ldexpf(s1, back) * alpha1;
+                if (w1.bias) u += w1.bias[n];
+                v = v / (1.0f + __expf(-v)) * u;
+            } else if (epilogue == SHREWQ_EPILOGUE_RELU) {
+                v = fmaxf(v, 0.0f);
+            }
+            store_out<YT>(y + (size_t)m * ldy + n, v);
         }
-        // back from the token's power of two and, for MX, from the window's: the first window has its largest scale, 2^(top - 127), at 2^13
-        const int back = exps[m] + (NV ? 0 : top - 127 - 13);
-        float v = ldexpf(s0, back) * a0;
-        if (w0.bias) v += w0.bias[n];
-        if constexpr (GATED) {
-            float u = ldexpf(s1, back) * a1;
-            if (w1.bias) u += w1.bias[n];
-            v = v / (1.0f + __expf(-v)) * u;
-        } else if (epilogue == SHREWQ_EPILOGUE_RELU) {
-            v = fmaxf(v, 0.0f);
-        }
-        store_out<YT>(y + (size_t)m * ldy + n, v);
     }
+    copy_async_wait<0>();
 }
 
 // ---- a handle's copy of the scales --------------------------------------------------------------------------------------------------

@@ -92,6 +92,21 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     return d;
 }
 
+__device__ __forceinline__ uint32_t smem_offset(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// asynchronous copies global -> shared memory of this thread's own bytes (16, past L1; 4); `valid` false: zeros, nothing is read
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest N groups of this thread have landed, visible to this thread
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 }  // namespace
 }  // namespace shrewq
 #endif  // SHREWQ_CPU_EMU

@@ -3,6 +3,14 @@
 #pragma once
 #include "cuda_shim.h"
 
+namespace emu {
+// address of a shared-memory offset that smem_u32 (cuda_shim_tcgen05.h, or below) made from a pointer into the block's dynamic memory
+inline void *smem_ptr_of(uint32_t addr) {
+    return reinterpret_cast<void *>((reinterpret_cast<uintptr_t>(g_block->dyn) & ~uintptr_t(0xFFFFFFFFu)) | addr);
+}
+}  // namespace emu
+static inline uint32_t smem_offset(const void *p) { return (uint32_t)reinterpret_cast<uintptr_t>(p); }
+
 static inline float __fdiv_rn(float a, float b) { return a / b; }
 static inline float __frcp_rn(float a) { return 1.0f / a; }
 static inline float rsqrtf(float a) { return (float)(1.0 / sqrt((double)a)); }
@@ -66,4 +74,30 @@ static inline uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 static inline uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     return pack_bf16x2_rn(emu_f32_of_bf16(a >> 16) * emu_f32_of_bf16(b >> 16), emu_f32_of_bf16(a & 0xFFFF) * emu_f32_of_bf16(b & 0xFFFF));
+}
+
+// cp.async: performed when it is waited for, so that a read without a wait finds old bytes
+namespace emu {
+struct AsyncCopy { void *dst; uint8_t data[16]; int bytes; int group; };
+inline thread_local std::vector<AsyncCopy> g_copies;
+inline thread_local int g_copy_group = 0;
+inline void copy_async(uint32_t dst, const void *src, int bytes, bool valid) {
+    AsyncCopy c{smem_ptr_of(dst), {0}, bytes, g_copy_group};
+    if (valid) memcpy(c.data, src, bytes);
+    EMU_CHECK(!valid || (reinterpret_cast<uintptr_t>(src) % bytes) == 0, "cp.async off its boundary");
+    g_copies.push_back(c);
+}
+}  // namespace emu
+static inline void copy_async_16(uint32_t dst, const void *src, bool valid) { emu::copy_async(dst, src, 16, valid); }
+static inline void copy_async_4(uint32_t dst, const void *src, bool valid) { emu::copy_async(dst, src, 4, valid); }
+static inline void copy_async_commit() { ++emu::g_copy_group; }
+template <int N>
+static inline void copy_async_wait() {
+    auto &v = emu::g_copies;
+    size_t kept = 0;
+    for (auto &c : v) {
+        if (c.group < emu::g_copy_group - N) memcpy(c.dst, c.data, c.bytes);
+        else v[kept++] = c;
+    }
+    v.resize(kept);
 }

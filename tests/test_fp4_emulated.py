@@ -18,7 +18,7 @@ def emu():
     L = _build("emu_fp4")
     L.emu_fp4_quantize.argtypes = [_vp, _ci, _sz, _sz, _sz, _ci, _vp, _ci, _ci, _cu, _vp, _vp]
     L.emu_fp4_dequantize.argtypes = [_vp, _vp, _vp, _sz, _sz, _ci, _ci, _ci, _vp]
-    L.emu_fp4_forward.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci]
+    L.emu_fp4_forward.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _cu, _ci]
     L.emu_residual_norm.argtypes = [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _ci, _ci, _ci, _ci, _cf, _cf, _cf, _ci, _ci, _ci, _ci,
                                     _ci, _cu]
     return L
@@ -130,14 +130,19 @@ def test_dequantize_rounds_once(emu, dtype, nv, cols, route):
     assert torch.equal(out.nan_to_num(77.0), want.nan_to_num(77.0)) and torch.equal(out.isnan(), want.isnan())
 
 
-def forward(emu, x, weights, biases, K, nv, relu=False, pad=0):
+def forward(emu, x, weights, biases, K, nv, relu=False, pad=0, ctas=5):
     M, N = x.shape[0], weights[0][0].shape[0]
     y = torch.full((M, N + pad), -77.0)
     table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
     rc = emu.emu_fp4_forward(table([w[0] for w in weights]), table([w[1] for w in weights]), table([w[2] for w in weights]), table(biases), x.data_ptr(),
-                             int(x.dtype is torch.float32), M, N, K, int(nv), int(len(weights) == 2), y.data_ptr(), N + pad, int(relu))
+                             int(x.dtype is torch.float32), M, N, K, int(nv), int(len(weights) == 2), y.data_ptr(), N + pad, int(relu), ctas, 0)
     assert rc == 0
     assert (y[:, N:] == -77.0).all()
+    if M <= 4:   # staged by the CTAs themselves: the same sums
+        y2 = torch.full((M, N + pad), -77.0)
+        rc = emu.emu_fp4_forward(table([w[0] for w in weights]), table([w[1] for w in weights]), table([w[2] for w in weights]), table(biases), x.data_ptr(),
+                                 int(x.dtype is torch.float32), M, N, K, int(nv), int(len(weights) == 2), y2.data_ptr(), N + pad, int(relu), ctas + 2, 1)
+        assert rc == 0 and torch.equal(y.nan_to_num(5.0), y2.nan_to_num(5.0))
     return y[:, :N].double().numpy()
 
 
