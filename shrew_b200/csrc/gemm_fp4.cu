@@ -33,7 +33,7 @@ int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const ui
     const CUtensorMap &tw = *static_cast<const CUtensorMap *>(a.w_tmap), &tw2 = GATED ? *static_cast<const CUtensorMap *>(a.up_tmap) : tw;
     const Operands ops{a.alpha, a.bias, a.alpha_up, a.bias_up};
     int per_cta;
-    const int S = split_over_cluster(tiles, (int)((a.K + kFp4StageK - 1) / kFp4StageK), TOK, ctx->sm_count, 2, &per_cta);
+    const int S = split_over_cluster(tiles, (int)((a.K + kFp4StageK - 1) / kFp4StageK), ctx->sm_count, 2, &per_cta);
     if (tiles * S > 0x7FFFFFFF) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: more than 2^31 tiles");
     SHREWQ_CUDA_TRY(ctx, launch_cluster(kern, (unsigned)(tiles * S), kFp4GemmThreads, (size_t)C::kSmemRequest, ctx->stream, a.pdl, S, tw, tw2, tx, (const uint8_t *)a.w->pieces,
                                           (const uint8_t *)(GATED ? a.up->pieces : a.w->pieces), pieces, ops, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,

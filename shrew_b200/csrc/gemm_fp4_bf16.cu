@@ -22,7 +22,7 @@ int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const void *x_rows, size_t 
     constexpr size_t kChan = GATED ? 64 : 128;
     const size_t tiles = (a.N + kChan - 1) / kChan * ((a.M + TOK - 1) / TOK);
     int per_cta;
-    const int S = split_over_cluster(tiles, (int)((a.K + kW4StageK - 1) / kW4StageK), TOK, ctx->sm_count, 4, &per_cta);
+    const int S = split_over_cluster(tiles, (int)((a.K + kW4StageK - 1) / kW4StageK), ctx->sm_count, 4, &per_cta);
     if (tiles * S > 0x7FFFFFFF) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: more than 2^31 tiles");
     const CUtensorMap &tw = *static_cast<const CUtensorMap *>(a.w_tmap), &tw2 = GATED ? *static_cast<const CUtensorMap *>(a.up_tmap) : tw;
     const Operands ops{a.alpha, a.bias, a.alpha_up, a.bias_up};

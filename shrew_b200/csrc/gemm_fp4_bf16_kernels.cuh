@@ -149,7 +149,6 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 
     if (threadIdx.x == 0) {
         ctl->abort_flag = 0;
-        ctl->tmem_base = 0;
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(bars + kFullBar + s * 8, 1);
             mbar_init(bars + kAreadyBar + s * 8, 4);

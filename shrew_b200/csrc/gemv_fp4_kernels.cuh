@@ -1,4 +1,4 @@
-// Forward of a layer with 4-bit microscaled weights for up to 32 tokens, sm_100a: warp-level MMA on f16 operands.
+// Forward of a layer with 4-bit microscaled weights for up to 4 tokens, sm_100a: warp-level MMA on f16 operands.
 //
 //   y[m,n] = alpha * sum_k w[n,k] x[m,k] + bias[n],   w = code * block scale  (alpha: the tensor scale of NV, 1 for MX)
 //
@@ -21,9 +21,8 @@
 // Codes and scales come by cp.async, every lane its own bytes into its own slots of a ring, several steps ahead and across tiles: no
 // register holds a byte in flight, no barrier guards one, and an SM has some 60 KB on their way.  The rows of a tile are 4 neighbours
 // each from the 4 groups of 32 that share 16 bytes of scales in the handle's copy (scale_piece_offset): scale sectors are used whole.
-// Activations: XS (a few tokens): every CTA stages them in its shared memory while its first codes are on their way: one launch.  Else
-// stage_f16_kernel writes them to global memory in the order of the MMA's B fragments (512 bytes a load, whole lines), from where they
-// come through L1, which keeps them from one tile to the next.
+// Activations: every CTA stages them in its shared memory while its first codes are on their way: one launch, no workspace.  (From 5 tokens
+// on gemm_fp4_f16_kernels.cuh: an m16n8k16 of mma.sync holds its tensor pipe for 32 cycles, which one group of 8 tokens just allows.)
 // The warps' sums of a tile meet in shared memory in a fixed order.
 //
 // Programmatic dependent launch: the ring is filled before the wait for the previous kernel.
@@ -44,7 +43,7 @@ constexpr int kGemv4Warps = 16, kGemv4Threads = kGemv4Warps * 32;
 constexpr int kGemv4Depth = 4;         // steps of the ring
 constexpr int kGemv4SlotBytes = 40;    // of a lane and step: 16 bytes of codes of two rows, a scale word for each
 constexpr int kGemv4RingBytes = kGemv4Warps * kGemv4Depth * 32 * kGemv4SlotBytes;
-constexpr int kGemv4MaxStaged = 4;     // tokens that a CTA stages itself (XS) ...
+constexpr int kGemv4MaxStaged = 4;     // tokens that a CTA stages ...
 constexpr int kGemv4StagedBytes = 96 * 1024;  // ... in at most this much shared memory
 constexpr int kMxWindow = 28;          // octaves of MX scales that one pass takes
 
@@ -112,25 +111,22 @@ __device__ __forceinline__ bool f16_terms(float *v, unsigned int top, uint4 *out
     return more;
 }
 
-// A CTA a token of the padded batch (8 tokens a group; beyond M zeros).  terms: [kMost][token groups][steps][4][32 lanes][8] f16 in the order
-// of the B fragments: piece q of lane 4 g + t holds k = 128 step + 32 t + 8 q .. + 7 of token g.  exps[m]: the power of two that the token
-// was divided by; counts[m]: terms in use.
+// For gemm_fp4_f16_kernels.cuh: a CTA a token.  terms: [kMost][M][Kp] f16 (Kp = K to whole 32s, zeros beyond K); exps[m]: the power of two that
+// the token was divided by; counts[m]: terms in use.
 template <typename T>
 __global__ void __launch_bounds__(256)
-stage_f16_kernel(const T *__restrict__ x, int M, int K, int vec_ok, uint4 *__restrict__ terms, int *__restrict__ exps, int *__restrict__ counts) {
+stage_f16_kernel(const T *__restrict__ x, int M, int K, int Kp, int vec_ok, uint4 *__restrict__ terms, int *__restrict__ exps, int *__restrict__ counts) {
     pdl_launch_dependents();
     __shared__ unsigned int s_max[8], s_more[8];
-    const int m = blockIdx.x, threads = (int)blockDim.x, warps = threads >> 5, steps = (K + 127) >> 7, groups = steps << 4;
-    const size_t plane = (size_t)(gridDim.x >> 3) * steps * 128;  // 16-byte pieces of a term
+    const int m = blockIdx.x, threads = (int)blockDim.x, warps = threads >> 5, groups = Kp >> 3;
+    const size_t plane = (size_t)M * groups;
     pdl_wait();
     const T *row = x + (size_t)m * K;
     unsigned int top = 0, more = 0;
-    if (m < M) {
-        for (int i = threadIdx.x; i < groups; i += threads) {
-            float v[8];
-            load_token8<T>(row, i, K, vec_ok, v);
-            top = top_exponent(v, top);
-        }
+    for (int i = threadIdx.x; i < groups; i += threads) {
+        float v[8];
+        load_token8<T>(row, i, K, vec_ok, v);
+        top = top_exponent(v, top);
     }
     top = warp_max(top);
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
@@ -138,17 +134,16 @@ stage_f16_kernel(const T *__restrict__ x, int M, int K, int vec_ok, uint4 *__res
     for (int w = 0; w < warps; ++w) top = s_max[w] > top ? s_max[w] : top;
     for (int i = threadIdx.x; i < groups; i += threads) {
         float v[8];
-        load_token8<T>(row, i, m < M ? K : 0, vec_ok, v);
+        load_token8<T>(row, i, K, vec_ok, v);
         uint4 out[XTerms<T>::kMost];
         more |= f16_terms<T>(v, top, out) ? 1u : 0u;
-        const size_t at = ((size_t)((m >> 3) * steps + (i >> 4)) * 4 + (i & 3)) * 32 + (m & 7) * 4 + ((i >> 2) & 3);
 #pragma unroll
-        for (int t = 0; t < XTerms<T>::kMost; ++t) terms[t * plane + at] = out[t];
+        for (int t = 0; t < XTerms<T>::kMost; ++t) terms[t * plane + (size_t)m * groups + i] = out[t];
     }
     more = warp_max(more);
     if ((threadIdx.x & 31) == 0) s_more[threadIdx.x >> 5] = more;
     __syncthreads();
-    if (threadIdx.x == 0 && m < M) {
+    if (threadIdx.x == 0) {
         for (int w = 0; w < warps; ++w) more |= s_more[w];
         exps[m] = (int)top - 141;
         counts[m] = more ? XTerms<T>::kMost : 1;
@@ -181,23 +176,13 @@ __device__ __forceinline__ int gemv4_row(int tile, int i) {
     return (tile / kTiles) * 128 + (tile % kTiles) * (1 << kShift) + (i & ((1 << kShift) - 1)) + 32 * (i >> kShift);
 }
 
-// Where the activations are: staged by stage_f16_kernel (terms, exps, counts), or, XS, still [M][K] of T
-template <typename T>
-struct Gemv4X {
-    const T *x;
-    int vec_ok;
-    const uint4 *terms;
-    const int *exps, *counts;
-};
-
-// NT: token groups of 8 (M <= 8 * NT; XS: M <= kGemv4MaxStaged)
-template <int NT, bool NV, bool GATED, bool XS, typename T, typename YT>
+// M <= kGemv4MaxStaged
+template <bool NV, bool GATED, typename T, typename YT>
 __global__ void __launch_bounds__(kGemv4Threads, 1)
-gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
-    static_assert(!XS || NT == 1, "a few tokens");
-    constexpr int kRows = GATED ? 8 : 16, kBufs = NT >= 4 ? 1 : 2;  // (48 KB of static shared memory)
-    SHREWQ_DYNAMIC_SMEM(uint8_t, smem);  // ring, then the staged activations (XS)
-    __shared__ float s_red[kBufs][kGemv4Warps][NT][4][32];
+gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const T *__restrict__ x, int vec_ok, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
+    constexpr int kRows = GATED ? 8 : 16;
+    SHREWQ_DYNAMIC_SMEM(uint8_t, smem);  // ring, then the staged activations
+    __shared__ float s_red[2][kGemv4Warps][4][32];
     __shared__ unsigned int s_max[kGemv4MaxStaged][kGemv4Warps], s_more[kGemv4Warps];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -250,9 +235,9 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
 
     // ---- activations ----
     int n_terms = 1;
-    const uint4 *sx = reinterpret_cast<const uint4 *>(smem + kGemv4RingBytes);  // XS: [terms][steps][4][4 t][M]
+    const uint4 *sx = reinterpret_cast<const uint4 *>(smem + kGemv4RingBytes);  // [terms][steps][4][4 t][M]
     unsigned int tops[kGemv4MaxStaged];
-    if constexpr (XS) {
+    {
         const int groups = steps << 4;
 #pragma unroll
         for (int m = 0; m < kGemv4MaxStaged; ++m) {
@@ -260,7 +245,7 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
             if (m < M)
                 for (int i = threadIdx.x; i < groups; i += kGemv4Threads) {
                     float v[8];
-                    load_token8<T>(xs.x + (size_t)m * K, i, K, xs.vec_ok, v);
+                    load_token8<T>(x + (size_t)m * K, i, K, vec_ok, v);
                     tops[m] = top_exponent(v, tops[m]);
                 }
             tops[m] = warp_max(tops[m]);
@@ -275,7 +260,7 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
             if (m < M)
                 for (int i = threadIdx.x; i < groups; i += kGemv4Threads) {
                     float v[8];
-                    load_token8<T>(xs.x + (size_t)m * K, i, K, xs.vec_ok, v);
+                    load_token8<T>(x + (size_t)m * K, i, K, vec_ok, v);
                     uint4 out[XTerms<T>::kMost];
                     more |= f16_terms<T>(v, tops[m], out) ? 1u : 0u;
 #pragma unroll
@@ -287,9 +272,6 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
         if (lane == 0) s_more[warp] = more;
         __syncthreads();
         for (int w = 0; w < kGemv4Warps; ++w) n_terms = s_more[w] ? XTerms<T>::kMost : n_terms;
-    } else {
-        for (int m = lane; m < M; m += 32) n_terms = xs.counts[m];
-        n_terms = (int)warp_max((unsigned int)n_terms);
     }
     int top = 0, windows = 1;
     if constexpr (!NV) {
@@ -302,18 +284,12 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
         windows = top >= low ? (top - low) / kMxWindow + 1 : 1;
     }
     const int passes = n_terms * windows;
-    const size_t x_plane = (size_t)NT * steps * 128;
 
     // One step: codes (two rows), scale words, activations -> acc
-    auto multiply = [&](float (&acc)[NT][4], uint4 ca, uint4 cb, uint32_t sa, uint32_t sb, int step, int term, int first) {
-        uint4 xv[NT][4];
+    auto multiply = [&](float (&acc)[4], uint4 ca, uint4 cb, uint32_t sa, uint32_t sb, int step, int term, int first) {
+        uint4 xv[4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if constexpr (XS) xv[n][q] = g < M ? sx[(size_t)(((term * steps + step) * 4 + q) * 4 + t) * M + g] : make_uint4(0, 0, 0, 0);
-                else xv[n][q] = __ldg(xs.terms + term * x_plane + ((size_t)(n * steps + step) * 4 + q) * 32 + lane);
-            }
+        for (int q = 0; q < 4; ++q) xv[q] = g < M ? sx[(size_t)(((term * steps + step) * 4 + q) * 4 + t) * M + g] : make_uint4(0, 0, 0, 0);
         uint32_t f[2][2];
         if constexpr (NV) {  // blocks 2t and 2t + 1 of the step's 8: half t % 2 of word t / 2, which this lane loaded
             const uint32_t a2 = cvt_f16x2_e4m3(sa >> (16 * (t & 1))), b2 = cvt_f16x2_e4m3(sb >> (16 * (t & 1)));
@@ -335,22 +311,15 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
                 ha[p] = mul_f16x2(ha[p], f[0][q >> 1]);
                 hb[p] = mul_f16x2(hb[p], f[1][q >> 1]);
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_f16_16816(acc[n], ha[0], hb[0], ha[1], hb[1], xv[n][q].x, xv[n][q].y);
-                mma_f16_16816(acc[n], ha[2], hb[2], ha[3], hb[3], xv[n][q].z, xv[n][q].w);
-            }
+            mma_f16_16816(acc, ha[0], hb[0], ha[1], hb[1], xv[q].x, xv[q].y);
+            mma_f16_16816(acc, ha[2], hb[2], ha[3], hb[3], xv[q].z, xv[q].w);
         }
     };
 
     const float alpha0 = NV ? w0.params->tensor_scale : 1.0f, alpha1 = GATED && NV ? w1.params->tensor_scale : 1.0f;
     int slot = 0, turn = 0;
-    for (int tile = (int)blockIdx.x; tile < tiles; tile += (int)gridDim.x, turn ^= kBufs - 1) {
-        float total[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) total[n][i] = 0.0f;
+    for (int tile = (int)blockIdx.x; tile < tiles; tile += (int)gridDim.x, turn ^= 1) {
+        float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = 0; s < mine; ++s) {
             request();
             copy_async_wait<kGemv4Depth - 1>();
@@ -364,43 +333,32 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, Gemv4X<T> xs, YT *__restrict__ y, 
             } else {
                 for (int pass = 0; pass < passes; ++pass) {
                     const int term = pass / windows, window = pass % windows;
-                    float acc[NT][4];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     multiply(acc, ca, cb, sc.x, sc.y, step, term, top - (kMxWindow - 1) - kMxWindow * window);
                     // weight of this pass's sums: 2^-11 or 2^-32 for each term, 2^-28 for each window
                     const float weight = ldexpf(1.0f, -XTerms<T>::kOctaves * term - kMxWindow * window);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) total[n][i] = __fmaf_rn(acc[n][i], weight, total[n][i]);
+                    for (int i = 0; i < 4; ++i) total[i] = __fmaf_rn(acc[i], weight, total[i]);
                 }
             }
         }
-        if (kBufs == 1 && tile != (int)blockIdx.x) __syncthreads();  // the tile before has been read
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s_red[turn][warp][n][i][lane] = total[n][i];
+        for (int i = 0; i < 4; ++i) s_red[turn][warp][i][lane] = total[i];
         __syncthreads();  // (with two buffers a warp writes this one again only behind the next barrier)
 
-        // accumulator (lane, i) of token group n: row (lane / 4) + (i >= 2 ? 8 : 0), token 8 n + 2 (lane % 4) + (i & 1)
-        for (int o = threadIdx.x; o < kRows * 8 * NT; o += kGemv4Threads) {
+        // accumulator (lane, i): row (lane / 4) + (i >= 2 ? 8 : 0), token 2 (lane % 4) + (i & 1)
+        for (int o = threadIdx.x; o < kRows * M; o += kGemv4Threads) {
             const int i = o % kRows, m = o / kRows;
             const int n = gemv4_row<GATED>(tile, i);
-            if (n >= N || m >= M) continue;
-            const int ln = (i & 7) * 4 + ((m & 7) >> 1), lo = (m & 1) + ((i & 8) ? 2 : 0);
+            if (n >= N) continue;
+            const int ln = (i & 7) * 4 + (m >> 1), lo = (m & 1) + ((i & 8) ? 2 : 0);
             float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
             for (int w = 0; w < kGemv4Warps; ++w) {
-                s0 += s_red[turn][w][m >> 3][lo][ln];
-                if constexpr (GATED) s1 += s_red[turn][w][m >> 3][2 + (m & 1)][ln];
+                s0 += s_red[turn][w][lo][ln];
+                if constexpr (GATED) s1 += s_red[turn][w][2 + (m & 1)][ln];
             }
-            int exponent;
-            if constexpr (XS) exponent = (int)(m == 0 ? tops[0] : m == 1 ? tops[1] : m == 2 ? tops[2] : tops[3]) - 141;
-            else exponent = xs.exps[m];
+            const int exponent = (int)(m == 0 ? tops[0] : m == 1 ? tops[1] : m == 2 ? tops[2] : tops[3]) - 141;
             // back from the token's power of two and, for MX, from the window's: the first window has its largest scale, 2^(top - 127), at 2^13
             const int back = exponent + (NV ? 0 : top - 127 - 13);
             float v = ldexpf(s0, back) * alpha0;

@@ -31,8 +31,12 @@ int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
         *kernel = "tcgen05-w4";
         return launch_gemm_w4_bf16(ctx, a);
     }
-    *kernel = "mma-fp4";
-    return launch_gemv_fp4(ctx, a);
+    if (gemv_fp4_supported(a)) {
+        *kernel = "mma-fp4";
+        return launch_gemv_fp4(ctx, a);
+    }
+    *kernel = "tcgen05-w4-f16";
+    return launch_gemm_w4_f16(ctx, a);
 }
 
 void destroy_fp4(Fp4Weight *w) {

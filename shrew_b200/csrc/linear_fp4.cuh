@@ -55,11 +55,11 @@ inline cudaError_t launch_cluster(Kern kern, unsigned grid, unsigned block, size
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// How many CTAs (1, 2, 4 or 8) share the k range of a tile: as many as the SMs can hold of all tiles at once, each with at least
-// min_rounds stages and none without one, and 16 tokens at least for each to finish.
-inline int split_over_cluster(size_t tiles, int rounds, int tok, int sm_count, int min_rounds, int *rounds_per_cta) {
+// How many CTAs (1, 2, 4 or 8) share the k range of a tile: as many as `room` holds of all tiles at once, each with at least
+// min_rounds stages and none without one.
+inline int split_over_cluster(size_t tiles, int rounds, int room, int min_rounds, int *rounds_per_cta) {
     int S = 1;
-    while (S < 8 && tiles * (size_t)(2 * S) <= (size_t)sm_count && rounds >= 2 * S * min_rounds && tok >= 2 * S * 16) S *= 2;
+    while (S < 8 && tiles * (size_t)(2 * S) <= (size_t)room && rounds >= 2 * S * min_rounds) S *= 2;
     while (S > 1 && (S - 1) * ((rounds + S - 1) / S) >= rounds) S /= 2;
     *rounds_per_cta = (rounds + S - 1) / S;
     return S;
@@ -77,6 +77,8 @@ int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float 
 int encode_fp4_tmap(shrewq_ctx *ctx, const uint8_t *codes, size_t n, size_t k, int box_rows, int box_bytes, void *tmap_out);
 int launch_gemm_w4_bf16(shrewq_ctx *ctx, const Fp4Forward &a);
 int launch_gemm_fp4(shrewq_ctx *ctx, const Fp4Forward &a);
+bool gemv_fp4_supported(const Fp4Forward &a);
+int launch_gemm_w4_f16(shrewq_ctx *ctx, const Fp4Forward &a);
 int launch_gemv_fp4(shrewq_ctx *ctx, const Fp4Forward &a);
 int launch_residual_norm(shrewq_ctx *ctx, const shrewq_residual_norm_args *p);
 

@@ -1,5 +1,5 @@
-// The PTX instructions of the block-scaled tensor-core kernels (tcgen05.mma kind::mxf4 / kind::mxf4nvf4, tcgen05.cp of their scales),
-// each behind a small function; the rest comes from ptx_tcgen05.cuh.  The CPU tests (tests/cpu_emu/) provide stand-ins.
+// The PTX instructions of the block-scaled tensor-core kernels (tcgen05.mma kind::mxf4 / kind::mxf4nvf4, tcgen05.cp of their scales) and of
+// kernels that take half of an SM's tensor memory, each behind a small function; the rest comes from ptx_tcgen05.cuh.  The CPU tests (tests/cpu_emu/) provide stand-ins.
 #pragma once
 
 #include "ptx_tcgen05.cuh"
@@ -31,6 +31,25 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uin
             "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
             ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
             : "memory");
+}
+
+// tc_mma_ts with f16 operands (the instruction descriptor names the types)
+__device__ __forceinline__ void tc_mma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    tc_mma_ts(d_tmem, a_tmem, b_desc, idesc, accumulate);
+}
+// 256 columns of tensor memory (two CTAs an SM); the base address is written to shared memory at result_smem
+__device__ __forceinline__ void tc_alloc_256(uint32_t result_smem) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(result_smem) : "memory");
+}
+__device__ __forceinline__ void tc_dealloc_256(uint32_t tmem_base) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem_base) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 
 }  // namespace

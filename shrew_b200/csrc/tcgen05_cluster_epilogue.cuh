@@ -2,8 +2,9 @@
 // k range optionally split over the CTAs of a cluster.
 //
 // Where the output tiles alone leave most SMs idle, a tile is computed by a cluster of S CTAs (2, 4 or 8), each over its part of k.  Their
-// sums meet in shared memory: every CTA finishes 1/S of the tile's tokens and receives the other CTAs' raw sums of those tokens by plain
-// stores into its pipeline stages, which are idle by then; the parts are added in rank order, so the result does not depend on timing.
+// sums meet in shared memory: every CTA (of a narrow tile the first few: 16 tokens are the least) finishes its share of the tile's tokens
+// and receives the other CTAs' raw sums of those tokens by plain stores into its pipeline stages, which are idle by then; the parts are
+// added in rank order, so the result does not depend on timing.
 // Against partial sums in global memory that costs no workspace (two streams, a captured graph) and no second trip through L2.
 //
 // A thread holds one channel (tensor-memory lane) and walks over 16 tokens at a time; values go through a [16 tokens][channels] staging
@@ -26,20 +27,24 @@ constexpr int kEpiStageBytes = kEpiChunk * 128 * 4;        // a group's staging 
 template <int NCOLS, int MODE>
 struct ClusterEpi {
     static constexpr int kAccs = MODE == kEpiColumns ? 2 : 1;
-    // received sums: [source][accumulator][NCOLS / S tokens][128 lanes] f32 from `slots` on; all sources together stay below this
-    static constexpr int kSlotBytes = kAccs * NCOLS * 128 * 4;
+    // received sums: [source][accumulator][tokens of a finisher][128 lanes] f32 from `slots` on; this is the most (8 CTAs)
+    static constexpr int kSlotBytes = kAccs * (NCOLS >= 128 ? NCOLS : 7 * kEpiChunk) * 128 * 4;
 };
+// CTAs of a cluster of S that finish tokens of a tile of NCOLS
+template <int NCOLS>
+__device__ __forceinline__ int cluster_finishers(int S) { return S < NCOLS / kEpiChunk ? S : NCOLS / kEpiChunk; }
 
 // Sends this CTA's raw sums of the other CTAs' tokens to them.  One call per epilogue thread; the receivers' stages must be idle (a
 // cluster barrier before), the sums are there after the next cluster barrier.
 template <int NCOLS, int G, int MODE>
 __device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_local, int S, uint32_t rank, int group, int quad, int lane) {
-    const int tokens = NCOLS / S, row = quad * 32 + lane;
+    const int F = cluster_finishers<NCOLS>(S), tokens = NCOLS / F, row = quad * 32 + lane;
     const uint32_t taddr = tmem_d + ((uint32_t)(quad * 32) << 16);
     const int chunks = tokens / kEpiChunk, per_dest = ClusterEpi<NCOLS, MODE>::kAccs * chunks;
-    for (int i = group; i < (S - 1) * per_dest; i += G) {
+    const int dests = (int)rank < F ? F - 1 : F;
+    for (int i = group; i < dests * per_dest; i += G) {
         const int step = i / per_dest, acc = i % per_dest / chunks, c = i % chunks;
-        const uint32_t dest = (rank + 1 + step) % S;       // everybody starts with another receiver
+        const uint32_t dest = (rank + 1 + step) % F;       // everybody starts with another receiver (a finisher never meets itself)
         const uint32_t source = rank < dest ? rank : rank - 1;
         uint32_t r[kEpiChunk];
         tc_ld16(taddr + acc * NCOLS + dest * tokens + c * kEpiChunk, r);
@@ -51,13 +56,15 @@ __device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_loc
     }
 }
 
-// Finishes this CTA's NCOLS / S tokens, m0 the tile's first token.  One call per epilogue thread (G groups of 128).
-template <int NCOLS, int G, int MODE, typename YT>
+// Finishes this CTA's share of the tokens, m0 the tile's first token.  One call per epilogue thread (G groups of 128).
+// TOKENS: the sums of token m are first multiplied by 2^(exps[m] + back).
+template <int NCOLS, int G, int MODE, typename YT, bool TOKENS = false>
 __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_base, const float *slots, int S, uint32_t rank, int group, int quad, int lane, bool ok,
-                                               const Operands &ops, YT *__restrict__ y, int M, int N, size_t ldy, int epilogue, int n0, int m0) {
+                                               const Operands &ops, YT *__restrict__ y, int M, int N, size_t ldy, int epilogue, int n0, int m0,
+                                               const int *__restrict__ exps = nullptr, int back = 0) {
     constexpr int CW = kEpiChunk, CH = MODE == kEpiLanesPaired ? 64 : 128, RB = CH * (int)sizeof(YT), EPV = 16 / (int)sizeof(YT), PPR = RB / 16, PIECES = CW * PPR;
     constexpr int ACCS = ClusterEpi<NCOLS, MODE>::kAccs;
-    const int tokens = NCOLS / S, row = quad * 32 + lane;
+    const int F = cluster_finishers<NCOLS>(S), tokens = NCOLS / F, row = quad * 32 + lane;
     const uint32_t taddr = tmem_d + ((uint32_t)(quad * 32) << 16);
     const bool is_up = MODE == kEpiLanesPaired && (row & 1);
     const int ch = MODE == kEpiLanesPaired ? row >> 1 : row, n = n0 + ch;
@@ -73,7 +80,7 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
     uint8_t *stage = stage_base + group * kEpiStageBytes;
     YT *out_st = reinterpret_cast<YT *>(stage);
     const bool vec_ok = ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * sizeof(YT))) & 15) == 0;
-    const int chunks = tokens / CW, first_col = (int)rank * tokens;
+    const int chunks = (int)rank < F ? tokens / CW : 0, first_col = (int)rank * tokens;
 #pragma unroll 1
     for (int c = group; c < chunks; c += G) {
         if (ok) {
@@ -86,7 +93,7 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
 #pragma unroll
                 for (int a = 0; a < ACCS; ++a)
 #pragma unroll
-                    for (int i = 0; i < CW; ++i) v[a][i] = __uint_as_float(raw[a][i]) * sc[a] + bs[a];
+                    for (int i = 0; i < CW; ++i) v[a][i] = __uint_as_float(raw[a][i]);
             } else {
 #pragma unroll
                 for (int a = 0; a < ACCS; ++a)
@@ -106,10 +113,17 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
                             for (int i = 0; i < CW; ++i) v[a][i] += p[((size_t)a * tokens + i) * 128];
                     }
                 }
+            }
 #pragma unroll
-                for (int a = 0; a < ACCS; ++a)
+            for (int i = 0; i < CW; ++i) {
+                if constexpr (TOKENS) {
+                    const int m = m0 + first_col + c * CW + i;
+                    const int e = m < M ? exps[m] + back : 0;
 #pragma unroll
-                    for (int i = 0; i < CW; ++i) v[a][i] = v[a][i] * sc[a] + bs[a];
+                    for (int a = 0; a < ACCS; ++a) v[a][i] = ldexpf(v[a][i], e);
+                }
+#pragma unroll
+                for (int a = 0; a < ACCS; ++a) v[a][i] = v[a][i] * sc[a] + bs[a];
             }
             if constexpr (MODE == kEpiColumns) {
 #pragma unroll

@@ -61,3 +61,43 @@ static inline void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc
     if (emu::tc_deferred()) emu::tc_push([=] { emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate); });
     else emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate);
 }
+
+// tcgen05.mma kind::f16 with f16 operands: A from tensor memory, B K-major in shared memory with the 128-byte swizzle
+namespace emu {
+inline void mma_ts_f16(Block *blk, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    const uint32_t N = ((idesc >> 17) & 0x3Fu) << 3, M = ((idesc >> 24) & 0x1Fu) << 4, dcol = d_tmem & 0xFFFF, acol = a_tmem & 0xFFFF;
+    EMU_CHECK(M == 128 && N % 16 == 0 && N >= 16 && N <= 256 && ((idesc >> 4) & 3u) == 1 && ((idesc >> 7) & 7u) == 0 && ((idesc >> 10) & 7u) == 0, "D f32, A and B f16");
+    EMU_CHECK(((b_desc >> 61) & 7u) == 2 && ((b_desc >> 46) & 1u) == 1, "128-byte swizzle, descriptor version 1");
+    if (dcol + N > 512 || acol + 8 > 512) { fail("tcgen05.mma operands outside tensor memory"); return; }
+    std::vector<float> b((size_t)N * 16);
+    for (uint32_t n = 0; n < N; ++n)
+        for (uint32_t k = 0; k < 16; ++k) {
+            uint16_t h;
+            memcpy(&h, smem_ptr(swizzle((smem_u32(blk->dyn) | desc_start(b_desc)) + (n >> 3) * desc_stride(b_desc) + (n & 7) * 128 + k * 2, 128)), 2);
+            b[n * 16 + k] = (float)emu_f16_of(h);
+        }
+    for (uint32_t m = 0; m < 128; ++m)
+        for (uint32_t n = 0; n < N; ++n) {
+            double acc = accumulate ? (double)__uint_as_float(blk->tmem[m * 512 + dcol + n]) : 0.0;
+            for (uint32_t k = 0; k < 16; ++k) {
+                const uint32_t w = blk->tmem[m * 512 + acol + (k >> 1)];
+                acc += (double)emu_f16_of(k & 1 ? w >> 16 : w & 0xFFFF) * (double)b[n * 16 + k];
+            }
+            blk->tmem[m * 512 + dcol + n] = __float_as_uint((float)acc);
+        }
+}
+}  // namespace emu
+static inline void tc_mma_ts_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if (emu::tc_deferred()) emu::tc_push([=] { emu::mma_ts_f16(emu::g_block, d, a, b, idesc, accumulate); });
+    else emu::mma_ts_f16(emu::g_block, d, a, b, idesc, accumulate);
+}
+
+// half of tensor memory: the model's allocation is the whole of it
+static inline void tc_alloc_256(uint32_t result_smem) { tc_alloc_512(result_smem); }
+static inline void tc_dealloc_256(uint32_t) {}
+static inline void tc_st16(uint32_t taddr, const uint32_t *r) {
+    const uint32_t lane = (taddr >> 16) + (threadIdx.x & 31), col = taddr & 0xFFFF;
+    if (!(lane < 128 && col + 16 <= 512)) { emu::fail("tcgen05.st outside tensor memory"); return; }
+    EMU_CHECK((taddr >> 16) == 32 * ((threadIdx.x >> 5) & 3), "a warp may only touch the lane quadrant warp % 4");
+    for (int i = 0; i < 16; ++i) emu::g_block->tmem[lane * 512 + col + i] = r[i];
+}

@@ -58,30 +58,17 @@ struct Weight {
     }
 };
 
-template <int NT, bool NV, bool GATED, bool XS, typename T>
+template <bool NV, bool GATED, typename T>
 void forward(const uint8_t *const *codes, const uint8_t *const *scales, const float *const *g, const float *const *bias, const void *x, int M, int N, int K, float *y,
              size_t ldy, int epilogue, unsigned ctas) {
-    const size_t steps = (K + 127) / 128, plane = NT * steps * 2048;
-    std::vector<uint8_t> raw(XTerms<T>::kMost * plane + 64, 0x7E);  // (f16 NaN where nothing is written)
-    uint4 *terms = reinterpret_cast<uint4 *>((reinterpret_cast<uintptr_t>(raw.data()) + 63) & ~uintptr_t(63));
-    std::vector<int> exps(M), counts(M);
-    Gemv4X<T> xs{static_cast<const T *>(x), (reinterpret_cast<uintptr_t>(x) % (8 * sizeof(T))) == 0 && K % 8 == 0, terms, exps.data(), counts.data()};
-    if (!XS) emu::launch(8 * NT, (unsigned)(steps >= 16 ? 256 : (steps * 16 + 31) / 32 * 32), [&] { stage_f16_kernel<T>(xs.x, M, K, xs.vec_ok, terms, exps.data(), counts.data()); });
+    const size_t steps = (K + 127) / 128;
     Weight<NV> w0(scales[0], g[0], N, K);
     Weight<NV> w1(scales[GATED ? 1 : 0], g[GATED ? 1 : 0], N, K);
     const Fp4Operand a{codes[0], w0.pieces.data(), &w0.params, bias[0]}, b{codes[GATED ? 1 : 0], w1.pieces.data(), &w1.params, bias[GATED ? 1 : 0]};
     const unsigned tiles = (unsigned)((N + 127) / 128 * (GATED ? 16 : 8));
-    emu::launch(tiles < ctas ? tiles : ctas, kGemv4Threads, kGemv4RingBytes + (XS ? XTerms<T>::kMost * steps * 256 * M : 0),
-                [&] { gemv_fp4_kernel<NT, NV, GATED, XS, T, float>(a, b, xs, y, M, N, K, ldy, epilogue); });
-}
-
-template <bool NV, bool GATED, typename T>
-void forward_tokens(const uint8_t *const *codes, const uint8_t *const *scales, const float *const *g, const float *const *bias, const void *x, int M, int N, int K, float *y,
-                    size_t ldy, int epilogue, unsigned ctas, int self_staged) {
-    if (self_staged) forward<1, NV, GATED, true, T>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas);
-    else if (M <= 8) forward<1, NV, GATED, false, T>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas);
-    else if (M <= 16) forward<2, NV, GATED, false, T>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas);
-    else forward<4, NV, GATED, false, T>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas);
+    const int vec_ok = (reinterpret_cast<uintptr_t>(x) % (8 * sizeof(T))) == 0 && K % 8 == 0;
+    emu::launch(tiles < ctas ? tiles : ctas, kGemv4Threads, kGemv4RingBytes + XTerms<T>::kMost * steps * 256 * M,
+                [&] { gemv_fp4_kernel<NV, GATED, T, float>(a, b, static_cast<const T *>(x), vec_ok, y, M, N, K, ldy, epilogue); });
 }
 
 template <typename TX, typename TB, typename TY>
@@ -115,10 +102,10 @@ extern "C" int emu_fp4_dequantize(const void *codes, const void *scales, const f
 }
 
 extern "C" int emu_fp4_forward(const uint8_t *const *codes, const uint8_t *const *scales, const float *const *g, const float *const *bias, const void *x, int x_f32,
-                               int M, int N, int K, int nv, int gated, float *y, size_t ldy, int epilogue, unsigned ctas, int self_staged) {
-#define CALL(NV, G)                                                                                                           \
-    (x_f32 ? forward_tokens<NV, G, float>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas, self_staged)            \
-           : forward_tokens<NV, G, __nv_bfloat16>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas, self_staged))
+                               int M, int N, int K, int nv, int gated, float *y, size_t ldy, int epilogue, unsigned ctas) {
+#define CALL(NV, G)                                                                                              \
+    (x_f32 ? forward<NV, G, float>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas)                   \
+           : forward<NV, G, __nv_bfloat16>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, ctas))
     if (nv) gated ? CALL(true, true) : CALL(true, false);
     else gated ? CALL(false, true) : CALL(false, false);
 #undef CALL

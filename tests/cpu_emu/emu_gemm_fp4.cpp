@@ -8,6 +8,7 @@
 #include "../../shrew_b200/csrc/gemv_fp4_kernels.cuh"
 #include "../../shrew_b200/csrc/gemm_fp4_kernels.cuh"
 #include "../../shrew_b200/csrc/gemm_fp4_bf16_kernels.cuh"
+#include "../../shrew_b200/csrc/gemm_fp4_f16_kernels.cuh"
 
 using namespace shrewq;
 
@@ -96,6 +97,41 @@ int run_w4(const uint8_t *const *codes, const uint8_t *const *scales, const floa
     return outcome(status);
 }
 
+// up to 32 tokens, activations staged as f16 terms
+template <int TOK, bool NV, bool GATED, typename T>
+int run_h4(const uint8_t *const *codes, const uint8_t *const *scales, const float *const *g, const float *const *bias, const void *x, int M, int N, int K, float *y,
+           size_t ldy, int epilogue, int split) {
+    using C = H4Cfg<TOK, NV, GATED>;
+    const size_t pitch = (K + 31) / 32 * 16, pieces = (size_t)(K + 255) / 256 * (NV ? 4 : 2), Kp = pitch * 2;
+    std::vector<uint8_t> raw[3];
+    std::vector<float> alpha[2];
+    uint8_t *wp[2];
+    Fp4Params params[2];
+    for (int i = 0; i < C::kMats; ++i) {
+        wp[i] = aligned(raw[i], (N + 127) / 128 * pieces * 512, 0xEE);
+        alpha[i].assign(N, 0.0f);
+        params[i] = Fp4Params{0.0f, 0.0f, 0, -1};
+        emu::launch(2, 256, [&] { fp4_scale_pieces_kernel<NV>(scales[i], g[i], N, (K + 31) / 32 * (NV ? 2 : 1), pieces, wp[i], &params[i], 1.0f, alpha[i].data()); });
+    }
+    uint8_t *terms = aligned(raw[2], XTerms<T>::kMost * M * Kp * 2, 0x7E);
+    std::vector<int> exps(M), counts(M);
+    emu::launch(M, (unsigned)(Kp / 8 >= 256 ? 256 : (Kp / 8 + 31) / 32 * 32), [&] {
+        stage_f16_kernel<T>(static_cast<const T *>(x), M, K, (int)Kp, (reinterpret_cast<uintptr_t>(x) & 31) == 0 && K % 8 == 0, reinterpret_cast<uint4 *>(terms),
+                            exps.data(), counts.data());
+    });
+    const int box = GATED ? 64 : 128;
+    const CUtensorMap tw = map2d(codes[0], pitch, N, 64, box, 1, 64), tw2 = map2d(codes[GATED ? 1 : 0], pitch, N, 64, box, 1, 64);
+    const CUtensorMap tx = map2d(terms, Kp, XTerms<T>::kMost * M, 64, TOK, 2);
+    const Fp4Operand w0{codes[0], wp[0], &params[0], bias[0]}, w1{codes[GATED ? 1 : 0], wp[GATED ? 1 : 0], &params[GATED ? 1 : 0], bias[GATED ? 1 : 0]};
+    DeviceStatus status{0, 0, 0, 0};
+    const int rounds = (K + kH4StageK - 1) / kH4StageK, per_cta = split ? (rounds + 1) / 2 : rounds;
+    launch_tiles((size_t)(N + box - 1) / box, split, kH4Threads, C::kSmemBytes, [&] {
+        gemm_w4_f16_kernel<TOK, NV, GATED, float>(tw, tw2, tx, w0, w1, alpha[0].data(), alpha[GATED ? 1 : 0].data(), exps.data(), counts.data(), XTerms<T>::kOctaves, y, M,
+                                                  N, K, ldy, epilogue, split ? 2 : 1, per_cta, &status);
+    });
+    return outcome(status);
+}
+
 }  // namespace
 
 // async_seed: 0 = copies and tensor-core work complete at issue, else deferred in an adversarial order
@@ -121,6 +157,17 @@ extern "C" int emu_gemm_w4_bf16(const uint8_t *const *codes, const uint8_t *cons
                                 int M, int N, int K, int tok, int nv, int gated, float *y, size_t ldy, int epilogue, int split, unsigned async_seed) {
     emu::g_tma_async_seed = async_seed;
     int rc = -3;
+    if (tok <= 32) {
+#define CALL(T, X) rc = nv ? (gated ? run_h4<T, true, true, X>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split)      \
+                                    : run_h4<T, true, false, X>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split))    \
+                           : (gated ? run_h4<T, false, true, X>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split)     \
+                                    : run_h4<T, false, false, X>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split))
+        if (tok == 16) { if (x_f32) CALL(16, float); else CALL(16, __nv_bfloat16); }
+        if (tok == 32) { if (x_f32) CALL(32, float); else CALL(32, __nv_bfloat16); }
+#undef CALL
+        emu::g_tma_async_seed = 0;
+        return rc;
+    }
 #define CALL(T, XT) rc = nv ? (gated ? run_w4<T, XT, true, true>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split)      \
                                      : run_w4<T, XT, true, false>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split))    \
                             : (gated ? run_w4<T, XT, false, true>(codes, scales, g, bias, x, M, N, K, y, ldy, epilogue, split)     \

@@ -18,7 +18,7 @@ def emu():
     L = _build("emu_fp4")
     L.emu_fp4_quantize.argtypes = [_vp, _ci, _sz, _sz, _sz, _ci, _vp, _ci, _ci, _cu, _vp, _vp]
     L.emu_fp4_dequantize.argtypes = [_vp, _vp, _vp, _sz, _sz, _ci, _ci, _ci, _vp]
-    L.emu_fp4_forward.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _cu, _ci]
+    L.emu_fp4_forward.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _cu]
     L.emu_residual_norm.argtypes = [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _ci, _ci, _ci, _ci, _cf, _cf, _cf, _ci, _ci, _ci, _ci,
                                     _ci, _cu]
     return L
@@ -130,54 +130,64 @@ def test_dequantize_rounds_once(emu, dtype, nv, cols, route):
     assert torch.equal(out.nan_to_num(77.0), want.nan_to_num(77.0)) and torch.equal(out.isnan(), want.isnan())
 
 
-def forward(emu, x, weights, biases, K, nv, relu=False, pad=0, ctas=5):
+def forward(emu, emu_gemm, x, weights, biases, K, nv, relu=False, pad=0):
+    """The kernel that takes so many tokens: a few by warp MMA, more on the tensor cores (there also with k split over a cluster of two)."""
     M, N = x.shape[0], weights[0][0].shape[0]
-    y = torch.full((M, N + pad), -77.0)
     table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
-    rc = emu.emu_fp4_forward(table([w[0] for w in weights]), table([w[1] for w in weights]), table([w[2] for w in weights]), table(biases), x.data_ptr(),
-                             int(x.dtype is torch.float32), M, N, K, int(nv), int(len(weights) == 2), y.data_ptr(), N + pad, int(relu), ctas, 0)
-    assert rc == 0
+    args = (table([w[0] for w in weights]), table([w[1] for w in weights]), table([w[2] for w in weights]), table(biases), x.data_ptr(),
+            int(x.dtype is torch.float32), M, N, K)
+    y = torch.full((M, N + pad), -77.0)
+    if M <= 4:
+        assert emu.emu_fp4_forward(*args, int(nv), int(len(weights) == 2), y.data_ptr(), N + pad, int(relu), 5) == 0
+    else:
+        split = int(K > 128 and N % 2)
+        assert emu_gemm.emu_gemm_w4_bf16(*args, 16 if M <= 16 else 32, int(nv), int(len(weights) == 2), y.data_ptr(), N + pad, int(relu), split, M % 3) == 0
     assert (y[:, N:] == -77.0).all()
-    if M <= 4:   # staged by the CTAs themselves: the same sums
-        y2 = torch.full((M, N + pad), -77.0)
-        rc = emu.emu_fp4_forward(table([w[0] for w in weights]), table([w[1] for w in weights]), table([w[2] for w in weights]), table(biases), x.data_ptr(),
-                                 int(x.dtype is torch.float32), M, N, K, int(nv), int(len(weights) == 2), y2.data_ptr(), N + pad, int(relu), ctas + 2, 1)
-        assert rc == 0 and torch.equal(y.nan_to_num(5.0), y2.nan_to_num(5.0))
     return y[:, :N].double().numpy()
+
+
+@pytest.fixture(scope="module")
+def emu_gemm():
+    L = _build("emu_gemm_fp4")
+    L.emu_gemm_fp4.argtypes = [_vp, _vp, _vp, _vp, _vp, _cf, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
+    L.emu_gemm_w4_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
+    return L
 
 
 @pytest.mark.parametrize("nv", [False, True])
 @pytest.mark.parametrize("M,N,K,x_dtype", [(1, 130, 256, torch.bfloat16), (3, 40, 1100, torch.bfloat16), (9, 129, 96, torch.float32), (20, 17, 33, torch.bfloat16),
                                            (32, 5, 2100, torch.bfloat16), (2, 1, 1, torch.float32)])
-def test_forward(emu, nv, M, N, K, x_dtype):
+def test_forward(emu, emu_gemm, nv, M, N, K, x_dtype):
     g = torch.Generator().manual_seed(M * N + K)
     x = aligned((M, K), x_dtype)
     x.copy_(torch.randn(M, K, generator=g) * torch.exp(3 * torch.randn(M, 1, generator=g)))
     w, bias = stored(N, K, nv, N, spread=9), torch.randn(N, generator=g)
-    y = forward(emu, x, [w], [bias], K, nv, relu=N % 2 == 1, pad=3)
+    y = forward(emu, emu_gemm, x, [w], [bias], K, nv, relu=N % 2 == 1, pad=3)
     xd, wd = x.double().numpy(), O.dequantize(w[0].numpy(), w[1].numpy(), 0.5, K, nv)
     want, bound = O.product(xd, wd, bias.numpy(), relu=N % 2 == 1), O.product_bound(xd, wd, K, bias=bias.numpy())
     assert (np.abs(y - want) <= bound).all()
 
 
 @pytest.mark.parametrize("nv", [False, True])
-def test_gated_forward(emu, nv):
-    M, N, K = 5, 70, 300
+@pytest.mark.parametrize("M", [3, 5, 30])
+def test_gated_forward(emu, emu_gemm, nv, M):
+    N, K = 70, 300
     g = torch.Generator().manual_seed(8)
     x = aligned((M, K), torch.bfloat16)
     x.copy_(torch.randn(M, K, generator=g))
     ws, biases = [stored(N, K, nv, s, spread=5 + 20 * s) for s in (0, 1)], [torch.randn(N, generator=g), None]
     for w in ws:
         w[2].fill_(2.0 ** -9 if nv else 1.0)
-    y = forward(emu, x, ws, biases, K, nv)
+    y = forward(emu, emu_gemm, x, ws, biases, K, nv)
     xd = x.double().numpy()
     wd = [O.dequantize(w[0].numpy(), w[1].numpy(), 2.0 ** -9, K, nv) for w in ws]
     assert (np.abs(y - O.product(xd, wd[0], biases[0].numpy(), up=wd[1])) <= O.product_bound(xd, wd[0], K, up=wd[1], bias=biases[0].numpy())).all()
 
 
-def test_scales_wider_than_a_window_and_activations_wider_than_a_term(emu):
+@pytest.mark.parametrize("M,N", [(3, 24), (7, 24), (20, 25)])
+def test_scales_wider_than_a_window_and_activations_wider_than_a_term(emu, emu_gemm, M, N):
     """Block scales over 90 octaves and activations over 60: every product still counts, whatever large things stand beside it."""
-    M, N, K = 3, 24, 320
+    K = 320
     c, s, g1 = stored(N, K, False, 4, spread=90)
     x = aligned((M, K), torch.bfloat16)
     gen = torch.Generator().manual_seed(2)
@@ -188,20 +198,21 @@ def test_scales_wider_than_a_window_and_activations_wider_than_a_term(emu):
     x[2, 40:] = 0.0
     x[2, 32] = 2.0 ** 20
     c[:, 16] = 0x00   # codes of columns 32, 33: the large activation of token 2 meets zeros
-    y = forward(emu, x, [(c, s, g1)], [None], K, False)
+    y = forward(emu, emu_gemm, x, [(c, s, g1)], [None], K, False)
     xd, wd = x.double().numpy(), O.dequantize(c.numpy(), s.numpy(), 1.0, K, False)
     assert (np.abs(y - O.product(xd, wd)) <= O.product_bound(xd, wd, K)).all()
 
 
-def test_infinities_and_nan_reach_their_outputs_only(emu):
-    M, N, K = 4, 20, 64
+@pytest.mark.parametrize("M", [4, 9])
+def test_infinities_and_nan_reach_their_outputs_only(emu, emu_gemm, M):
+    N, K = 20, 64
     w = stored(N, K, False, 4, spread=3)
     w[1][7, 1] = 255                       # a NaN block of row 7
     x = aligned((M, K), torch.bfloat16)
     x.copy_(torch.randn(M, K, generator=torch.Generator().manual_seed(1)))
     x[2, 5] = float("inf")
     x[3, 9] = float("nan")
-    y = forward(emu, x, [w], [None], K, False)
+    y = forward(emu, emu_gemm, x, [w], [None], K, False)
     wd = O.dequantize(w[0].numpy(), w[1].numpy(), 1.0, K, False)
     want = O.product(x.double().numpy(), wd)
     np.testing.assert_array_equal(np.isnan(y), np.isnan(want))
@@ -249,14 +260,6 @@ def test_residual_norm(emu, x_dtype, b_dtype, h_dtype, M, D, V, pre, post, gate_
         rms = np.sqrt(((want_r - (want_r.mean(-1, keepdims=True) if pre == 2 else 0)) ** 2).mean(-1, keepdims=True) + 1e-5)
         spread = np.abs(n[2]) * (scale_r.max(-1, keepdims=True) / rms) * (1 + np.abs(want_r) / rms)
         assert (np.abs(h2.double().numpy() - want_h) <= half[h_dtype] * np.abs(want_h) + 4 * eps * spread).all()
-
-
-@pytest.fixture(scope="module")
-def emu_gemm():
-    L = _build("emu_gemm_fp4")
-    L.emu_gemm_fp4.argtypes = [_vp, _vp, _vp, _vp, _vp, _cf, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
-    L.emu_gemm_w4_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
-    return L
 
 
 @pytest.mark.parametrize("nv", [False, True])
