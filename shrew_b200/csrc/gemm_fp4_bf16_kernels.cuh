@@ -164,7 +164,7 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
     bool ok = true;
 
     if (warp == 0) {
@@ -194,7 +194,7 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             for (int i = 0; i < pre; ++i) load_x(i, i);
             uint32_t s = 0, ph = 0;
             for (int i = pre; i < rounds; ++i) {
-                if (!mbar_wait_c<kTimeoutW4>(bars + kEmptyBar + s * 8, ph, ctl, status, 0, s)) break;
+                if (!mbar_wait_close<kTimeoutW4>(bars + kEmptyBar + s * 8, ph, ctl, status, 0, s)) break;
                 load_w(i, s);
                 load_x(i, s);
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
@@ -207,8 +207,8 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t s = 0, ph = 0;
             bool good = true;
             for (int i = 0; i < rounds; ++i) {
-                good = mbar_wait_c<kTimeoutW4>(bars + kAreadyBar + s * 8, ph, ctl, status, 2, s) &&
-                       mbar_wait_c<kTimeoutW4>(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
+                // (the converters have waited for the stage: its activations are there too)
+                good = mbar_wait_close<kTimeoutW4>(bars + kAreadyBar + s * 8, ph, ctl, status, 2, s);
                 if (!good) break;
                 tc_fence_after();
                 const uint64_t bdesc = make_b_desc(smem_base + s * C::kStageBytes + C::kXOff);
@@ -236,11 +236,10 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const int prow = GATED ? (n0 & 64) + (row >> 1) : row;
         const int scale_at = C::kScaleOff + (GATED ? (row & 1) * C::kPieces * 512 : 0) + (prow & 31) * 16 + (prow >> 5) * 4;
         pdl_wait();  // a stage is full only with its activations; outputs may be in use by the previous kernel
-        for (int i = 0; i < rounds && ok; ++i) {
+        for (int i = 0; i < rounds; ++i) {
             const int s = i % C::kStages;
             if (s % kW4Groups != group) continue;
-            ok = mbar_wait_warp_c<kTimeoutW4>(bars + kFullBar + s * 8, (i / C::kStages) & 1, ctl, status, 3, s);
-            if (!ok) break;
+            mbar_wait_all<kTimeoutW4>(bars + kFullBar + s * 8, (i / C::kStages) & 1, ctl, status, 3, s);
             tc_fence_after();
             const uint8_t *stage = smem + s * C::kStageBytes;
             uint32_t f[kW4StageK / 32][2];  // factors of the row's blocks
@@ -269,8 +268,9 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + kAreadyBar + s * 8);
         }
-        if (ok) ok = mbar_wait_warp_c<kTimeoutW4>(bars + kAccBar, 0, ctl, status, 4, 0);
-        if (ok) tc_fence_after();
+        mbar_wait_all<kTimeoutW4>(bars + kAccBar, 0, ctl, status, 4, 0);
+        ok = warp_ok(ctl);
+        tc_fence_after();
         if (S == 1)
             cluster_finish<TOK, kW4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0);
     }

@@ -32,7 +32,7 @@
 namespace shrewq {
 namespace {
 
-constexpr int kH4StageK = 128, kH4Groups = 2, kH4Threads = 64 + 128 * kH4Groups;
+constexpr int kH4StageK = 128, kH4Groups = 3, kH4Threads = 64 + 128 * kH4Groups;
 constexpr uint32_t kTimeoutH4 = 7;  // DeviceStatus::timeout_flag of this kernel
 
 template <int TOK, bool NV, bool GATED>
@@ -47,7 +47,7 @@ struct H4Cfg {
     static constexpr int kStages = 6, kSlots = kH4Groups;                  // (kStages a multiple of the groups, see the converters)
     static constexpr int kACols = kH4StageK / 2, kABase = 64;              // tensor memory: sums, totals of several passes, widened codes
     static constexpr int kSmemBytes = kStages * kStageBytes + 2048;
-    static constexpr int kSlotOff = kH4Groups * kEpiStageBytes;
+    static constexpr int kSlotOff = 2 * kEpiStageBytes;                    // (at most two chunks of 16 tokens: two groups have staging tiles)
     static_assert(kABase >= 2 * TOK && kABase + kSlots * kACols <= 256 && kStages % kH4Groups == 0, "tensor memory of half an SM");
     // What is asked for is half an SM's shared memory, and enough that a kernel which takes all of tensor memory (they ask for 120 KB) never
     // shares an SM with this one: of two such neighbours in a stream, started early, one could hold the memory that the other waits for.
@@ -110,7 +110,7 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
     // the next kernel of the stream may start, now that this one has its tensor memory: it will wait for this one to end, with whatever it
     // has allocated on this SM
     pdl_launch_dependents();
@@ -161,7 +161,7 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             int pass = pre == rounds ? 1 : 0, r = pre == rounds ? 0 : pre;
             for (int i = pre; i < items; ++i) {
                 // a stage of the first round through the ring is free: the wait for the phase before it returns at once
-                if (!mbar_wait_c<kTimeoutH4>(bars + kEmptyBar + s * 8, ph, ctl, status, 0, s)) break;
+                if (!mbar_wait_close<kTimeoutH4>(bars + kEmptyBar + s * 8, ph, ctl, status, 0, s)) break;
                 load_w(r, (int)s);
                 load_x(r, pass / windows, (int)s);
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
@@ -169,17 +169,17 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             }
         }
     } else if (warp == 1) {
+        // D=f32, A=f16 (tensor memory), B=f16 (K-major), M=128, N=TOK
+        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        uint32_t s = 0, slot = 0, slot_ph = 0;
+        bool good = true;
         if (elect_one()) {
-            // D=f32, A=f16 (tensor memory), B=f16 (K-major), M=128, N=TOK
-            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-            uint32_t s = 0, ph = 0, slot = 0, slot_ph = 0;
-            bool good = true;
             for (int pass = 0; pass < passes && good; ++pass) {
                 // the sums of the pass before have been taken out
-                if (pass > 0) good = mbar_wait_c<kTimeoutH4>(bars + kTakenBar, (uint32_t)(pass - 1) & 1u, ctl, status, 5, 0);
+                if (pass > 0) good = mbar_wait_close<kTimeoutH4>(bars + kTakenBar, (uint32_t)(pass - 1) & 1u, ctl, status, 5, 0);
                 for (int i = 0; i < rounds && good; ++i) {
-                    good = mbar_wait_c<kTimeoutH4>(bars + kAreadyBar + slot * 8, slot_ph, ctl, status, 2, slot) &&
-                           mbar_wait_c<kTimeoutH4>(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
+                    // (the converters have waited for the stage: its activations are there too)
+                    good = mbar_wait_close<kTimeoutH4>(bars + kAreadyBar + slot * 8, slot_ph, ctl, status, 2, slot);
                     if (!good) break;
                     tc_fence_after();
                     const uint64_t bdesc = make_b_desc(smem_base + s * C::kStageBytes + C::kXOff);
@@ -189,9 +189,9 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
                             tc_mma_ts_f16(tmem, a + j * 32 + q * 8, bdesc + (uint64_t)((j * C::kXBox + q * 32) >> 4), idesc, (i > 0 || j > 0 || q > 0) ? 1u : 0u);
-                    tc_commit(bars + kEmptyBar + s * 8);     // frees the stage ...
-                    tc_commit(bars + kAfreeBar + slot * 8);  // ... and the place of its widened codes
-                    if (++s == C::kStages) { s = 0; ph ^= 1; }
+                    tc_commit(bars + kAfreeBar + slot * 8);  // frees the place of its widened codes ...
+                    tc_commit(bars + kEmptyBar + s * 8);     // ... and the stage
+                    if (++s == C::kStages) s = 0;
                     if (++slot == C::kSlots) { slot = 0; slot_ph ^= 1; }
                 }
                 if (good) tc_commit(bars + kAccBar);
@@ -205,58 +205,47 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         const int prow = GATED ? (n0 & 64) + (row >> 1) : row;
         const int scale_at = C::kScaleOff + (GATED ? (row & 1) * C::kPieces * 512 : 0) + (prow & 31) * 16 + (prow >> 5) * 4;
         int item = 0;
-        for (int pass = 0; pass < passes && ok; ++pass) {
+        for (int pass = 0; pass < passes; ++pass) {
             const int first = top - (kMxWindow - 1) - kMxWindow * (pass % windows);  // MX: the byte of 2^-14 in this window
-            for (int i = 0; i < rounds && ok; ++i, ++item) {
-                // group g takes the items i % 2 == g, and with an even ring the stages and places of that parity: it passes through every
-                // phase of the barriers that it polls, so that a wait for a parity cannot take one phase for another
+            for (int i = 0; i < rounds; ++i, ++item) {
+                // group g takes the items i % 3 == g, and so, the ring being a multiple, always the same stages and place: it passes through
+                // every phase of the barriers that it polls, so that a wait for a parity cannot take one phase for another
                 const int slot = item % C::kSlots, s = item % C::kStages;
                 if (slot != group) continue;
-                ok = mbar_wait_warp_c<kTimeoutH4>(bars + kFullBar + s * 8, (uint32_t)(item / C::kStages) & 1u, ctl, status, 3, s);
-                if (!ok) break;
+                mbar_wait_all<kTimeoutH4>(bars + kFullBar + s * 8, (uint32_t)(item / C::kStages) & 1u, ctl, status, 3, s);
                 const uint8_t *stage = smem + s * C::kStageBytes;
-                uint32_t f[4][2];
-                if constexpr (NV) {
+                uint32_t scales[2];
+                scales[0] = *reinterpret_cast<const uint32_t *>(stage + scale_at);
+                if constexpr (NV) scales[1] = *reinterpret_cast<const uint32_t *>(stage + scale_at + 512);
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t *>(stage + scale_at + p * 512);
-                        const uint32_t a = cvt_f16x2_e4m3(w), b = cvt_f16x2_e4m3(w >> 16);
-                        f[2 * p][0] = dup_lo(a);
-                        f[2 * p][1] = dup_hi(a);
-                        f[2 * p + 1][0] = dup_lo(b);
-                        f[2 * p + 1][1] = dup_hi(b);
+                for (int b = 0; b < 4; ++b) {  // 32 codes
+                    uint32_t f0, f1, packed[16];
+                    if constexpr (NV) {
+                        const uint32_t two = cvt_f16x2_e4m3(scales[b >> 1] >> (16 * (b & 1)));
+                        f0 = dup_lo(two);
+                        f1 = dup_hi(two);
+                    } else {
+                        f0 = f1 = mx_scale_f16x2(scales[0], b, first);
                     }
-                } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t *>(stage + scale_at);
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) f[b][0] = f[b][1] = mx_scale_f16x2(w, b, first);
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t packed[32];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-                        widen32_f16(*reinterpret_cast<const uint4 *>(stage + srow * (kH4StageK / 2) + (((2 * j + b) ^ swz) << 4)), f[2 * j + b][0], f[2 * j + b][1],
-                                    packed + 16 * b);
-                    if (j == 0) {  // the MMAs of this group's item before have read their codes
+                    widen32_f16(*reinterpret_cast<const uint4 *>(stage + srow * (kH4StageK / 2) + ((b ^ swz) << 4)), f0, f1, packed);
+                    if (b == 0) {  // the MMAs of this group's item before have read their codes
                         if (item >= C::kSlots)
-                            ok = mbar_wait_warp_c<kTimeoutH4>(bars + kAfreeBar + slot * 8, (uint32_t)(item / C::kSlots - 1) & 1u, ctl, status, 6, slot);
-                        if (!ok) break;
+                            mbar_wait_all<kTimeoutH4>(bars + kAfreeBar + slot * 8, (uint32_t)(item / C::kSlots - 1) & 1u, ctl, status, 6, slot);
                         tc_fence_after();
                     }
-                    tc_st32(tmem + lanes + C::kABase + slot * C::kACols + j * 32, packed);
+                    tc_st16(tmem + lanes + C::kABase + slot * C::kACols + b * 16, packed);
                 }
-                if (!ok) break;
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bars + kAreadyBar + slot * 8);
             }
-            if (ok) ok = mbar_wait_warp_c<kTimeoutH4>(bars + kAccBar, (uint32_t)pass & 1u, ctl, status, 4, 0);
-            if (ok) tc_fence_after();
+            mbar_wait_all<kTimeoutH4>(bars + kAccBar, (uint32_t)pass & 1u, ctl, status, 4, 0);
+            ok = warp_ok(ctl);
+            tc_fence_after();
             if (passes > 1) {
                 // the first group adds the pass's sums to the totals, which take the sums' place in the end
-                if (ok && group == 0) {
+                if (group == 0) {
                     const float weight = ldexpf(1.0f, -octaves * (pass / windows) - kMxWindow * (pass % windows));
                     const bool last = pass + 1 == passes;
 #pragma unroll 1

@@ -64,7 +64,7 @@ struct Fp4Cfg {
 };
 
 __device__ __forceinline__ bool fp4_wait(uint32_t bar, uint32_t parity, Ctl *ctl, DeviceStatus *st, uint32_t role, uint32_t stage) {
-    return mbar_wait_c<kTimeoutFp4>(bar, parity, ctl, st, role, stage);
+    return mbar_wait_close<kTimeoutFp4>(bar, parity, ctl, st, role, stage);
 }
 
 // Shared-memory descriptor of a scale piece: no swizzle, rows of 16 bytes, 8-row groups 128 bytes apart
@@ -125,7 +125,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
     bool ok = true;
 
     if (warp == 0) {
@@ -207,8 +207,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     } else {
         const int group = (warp - 2) >> 2, quad = warp & 3;
         pdl_wait();  // y may be in use by the previous kernel of the stream
-        ok = mbar_wait_warp_c<kTimeoutFp4>(bars + kAccBar, 0, ctl, status, 4, 0);
-        if (ok) tc_fence_after();
+        mbar_wait_all<kTimeoutFp4>(bars + kAccBar, 0, ctl, status, 4, 0);
+        ok = warp_ok(ctl);
+        tc_fence_after();
         if (S == 1)
             cluster_finish<TOK, kFp4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0);
     }

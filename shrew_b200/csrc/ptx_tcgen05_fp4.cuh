@@ -8,6 +8,19 @@
 namespace shrewq {
 namespace {
 
+// whether the phase of this parity has completed: never suspends the thread, as mbarrier.try_wait may
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // 32 rows of 16 bytes in shared memory (rows 16 bytes apart) -> four columns of tensor memory, the same in all four lane quadrants
 __device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");

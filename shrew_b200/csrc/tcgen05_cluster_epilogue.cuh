@@ -15,10 +15,31 @@
 #pragma once
 
 #include "ptx_cluster.cuh"
+#include "ptx_tcgen05_fp4.cuh"
+#include "tcgen05_common.cuh"
 #include "tcgen05_epilogue.cuh"
 
 namespace shrewq {
 namespace {
+
+// Bounded waits of the kernels whose stages take a few hundred cycles.  One thread: polls back to back for a while (mbarrier.try_wait
+// suspends a thread that comes too early, and it was woken some 500 cycles after the phase completed), then as the other kernels do.
+constexpr uint32_t kSpinClose = SHREWQ_SPIN_FAST_LIMIT;
+template <uint32_t CODE>
+__device__ __forceinline__ bool mbar_wait_close(uint32_t bar, uint32_t parity, Ctl *ctl, DeviceStatus *st, uint32_t role, uint32_t stage) {
+    for (uint32_t i = 0; i < kSpinClose; ++i)
+        if (mbar_test(bar, parity)) return true;
+    return mbar_wait_slow(bar, parity, ctl, st, role, stage, CODE);
+}
+// A whole warp: every lane looks (67 cycles where the phase is complete; one lane and a shuffle take 110, one lane, a shuffle and a second
+// look by all, as mbar_wait_warp_c has it, 270).  A wait that runs out raises the abort flag and the warp goes on, so that its lanes stay
+// together: what it computes then is not stored.  warp_ok() says afterwards whether anything gave up.
+template <uint32_t CODE>
+__device__ __forceinline__ void mbar_wait_all(uint32_t bar, uint32_t parity, Ctl *ctl, DeviceStatus *st, uint32_t role, uint32_t stage) {
+    mbar_wait_close<CODE>(bar, parity, ctl, st, role, stage);
+    __syncwarp();
+}
+__device__ __forceinline__ bool warp_ok(Ctl *ctl) { return __all_sync(0xFFFFFFFFu, ctl->abort_flag == 0) != 0; }
 
 enum { kEpiPlain = 0, kEpiLanesPaired = 1, kEpiColumns = 2 };
 constexpr int kEpiChunk = 16;                              // tokens a step

@@ -52,6 +52,7 @@ inline void mma_fp4(Block *blk, bool nv, uint32_t d_tmem, uint64_t a_desc, uint6
 }
 }  // namespace emu
 
+static inline bool mbar_test(uint32_t bar, uint32_t parity) { return mbar_try(bar, parity); }
 static inline void tc_cp_scales(uint32_t taddr, uint64_t desc) {
     if (emu::tc_deferred()) emu::tc_push([=] { emu::cp_scales(emu::g_block, taddr, desc); });
     else emu::cp_scales(emu::g_block, taddr, desc);
