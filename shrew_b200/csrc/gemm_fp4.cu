@@ -5,6 +5,7 @@
 #include "gemm_tcgen05_launch.cuh"
 #include "fp4_kernels.cuh"
 #include "gemm_fp4_kernels.cuh"
+#include "gemm_fp4_pair_kernels.cuh"
 #include "linear_fp4.cuh"
 
 namespace shrewq {
@@ -19,23 +20,22 @@ cudaError_t quantize_acts(shrewq_ctx *ctx, const Fp4Forward &a, uint32_t *codes,
                             a.M, a.K, a.K, vec_ok, (const float *)&a.w->params->x_scale, (const float *)nullptr, 0, (float *)nullptr, blocks, codes, pieces);
 }
 
+size_t pair_tiles(const Fp4Forward &a) { return (a.N + (a.up ? 127 : 255)) / (a.up ? 128 : 256) * ((a.M + kPairTok - 1) / kPairTok); }
+
 template <int TOK, bool NV, bool GATED, typename YT>
 int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const uint8_t *pieces) {
     using C = Fp4Cfg<TOK, NV, GATED>;
-    const size_t pitch = (a.K + 31) / 32 * 16;
-    CUtensorMap tx;
-    int rc = encode_2d(ctx, &tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, pitch, a.M, kFp4RowBytes, TOK, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != SHREWQ_OK) return rc;
     auto kern = gemm_fp4_kernel<TOK, NV, GATED, YT>;
     static std::atomic<unsigned long long> attr_done{0};
+    int rc;
     if ((rc = set_smem_attr_once(ctx, kern, C::kSmemRequest, attr_done)) != SHREWQ_OK) return rc;
     const size_t tiles = (a.N + 127) / 128 * ((a.M + TOK - 1) / TOK);
-    const CUtensorMap &tw = *static_cast<const CUtensorMap *>(a.w_tmap), &tw2 = GATED ? *static_cast<const CUtensorMap *>(a.up_tmap) : tw;
     const Operands ops{a.alpha, a.bias, a.alpha_up, a.bias_up};
     int per_cta;
     const int S = split_over_cluster(tiles, (int)((a.K + kFp4StageK - 1) / kFp4StageK), ctx->sm_count, 2, &per_cta);
     if (tiles * S > 0x7FFFFFFF) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: more than 2^31 tiles");
-    SHREWQ_CUDA_TRY(ctx, launch_cluster(kern, (unsigned)(tiles * S), kFp4GemmThreads, (size_t)C::kSmemRequest, ctx->stream, a.pdl, S, tw, tw2, tx, (const uint8_t *)a.w->pieces,
+    SHREWQ_CUDA_TRY(ctx, launch_cluster(kern, (unsigned)(tiles * S), kFp4GemmThreads, (size_t)C::kSmemRequest, ctx->stream, a.pdl, S, a.w->codes,
+                                        GATED ? a.up->codes : a.w->codes, static_cast<const uint8_t *>(codes), (const uint8_t *)a.w->pieces,
                                           (const uint8_t *)(GATED ? a.up->pieces : a.w->pieces), pieces, ops, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,
                                           a.epilogue, S, per_cta, ctx->dev_status));
     ctx->launches += 1;
@@ -43,8 +43,31 @@ int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const ui
     return SHREWQ_OK;
 }
 
+template <bool NV, bool GATED, typename YT>
+int launch_pair(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const uint8_t *pieces) {
+    using C = Fp4PairCfg<NV, GATED, YT>;
+    auto kern = gemm_fp4_pair_kernel<NV, GATED, YT>;
+    static std::atomic<unsigned long long> attr_done{0};
+    int rc = set_smem_attr_once(ctx, kern, C::kSmemBytes, attr_done);
+    if (rc != SHREWQ_OK) return rc;
+    const size_t tiles = pair_tiles(a);
+    const int pairs = (int)(tiles < (size_t)ctx->sm_count / 2 ? tiles : (size_t)ctx->sm_count / 2);
+    if (tiles > 0x3FFFFFFF) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: more than 2^31 tiles");
+    const Operands ops{a.alpha, a.bias, a.alpha_up, a.bias_up};
+    SHREWQ_CUDA_TRY(ctx, launch_cluster(kern, (unsigned)(2 * pairs), kPairThreads, (size_t)C::kSmemBytes, ctx->stream, a.pdl, 2, a.w->codes,
+                                        GATED ? a.up->codes : a.w->codes, static_cast<const uint8_t *>(codes), (const uint8_t *)a.w->pieces,
+                                        (const uint8_t *)(GATED ? a.up->pieces : a.w->pieces), pieces, ops, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,
+                                        a.epilogue, (int)tiles, pairs, ctx->dev_status));
+    ctx->launches += 1;
+    SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
+    return SHREWQ_OK;
+}
+
 template <bool NV, typename YT>
 int launch_tokens(shrewq_ctx *ctx, const Fp4Forward &a, const void *codes, const uint8_t *pieces) {
+    // pairs of CTAs where their tiles of 256 tokens fill most of the machine
+    if (a.M > 128 && pair_tiles(a) * 4 >= (size_t)ctx->sm_count)
+        return a.up ? launch_pair<NV, true, YT>(ctx, a, codes, pieces) : launch_pair<NV, false, YT>(ctx, a, codes, pieces);
     if (a.up) return a.M <= 64 ? launch_one<64, NV, true, YT>(ctx, a, codes, pieces) : launch_one<128, NV, true, YT>(ctx, a, codes, pieces);
     if (a.M <= 64) return launch_one<64, NV, false, YT>(ctx, a, codes, pieces);
     if (a.M <= 128) return launch_one<128, NV, false, YT>(ctx, a, codes, pieces);

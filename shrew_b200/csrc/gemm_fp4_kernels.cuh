@@ -4,18 +4,24 @@
 //   y[m,n] = epi( alpha[n] * sum_k (w code * w scale)[n,k] (x code * x scale)[m,k] + bias[n] ),  f32 sums
 //
 // Mapping.  D[128 x TOK] += A[128 x 64] * B[TOK x 64]^T for each instruction: A = 128 weight rows, B = a tile of tokens, both packed codes in
-// shared memory (TMA, 128-byte swizzle, K-major: one row of a stage is 256 codes = 128 bytes), D = f32 accumulators in tensor memory
-// (lane = output channel, column = token).  The scales of a stage come as the 512-byte pieces that the quantizer and the handle lay out
-// (scale_piece_offset), by 1-D bulk copies, and go to tensor memory with tcgen05.cp just ahead of the MMAs that use them; every stage
-// of the ring has its own columns for them, so the release of the stage covers them too.
+// shared memory (128-byte swizzle, K-major: one row of a stage is 256 codes = 128 bytes), D = f32 accumulators in tensor memory
+// (lane = output channel, column = token).  The scales of a stage are the 512-byte pieces that the quantizer and the handle lay out
+// (scale_piece_offset); they go on to tensor memory with tcgen05.cp just ahead of the MMAs that use them, every stage of the ring into
+// columns of its own, so that the release of the stage covers them too.
+//
+// What bounds a tile of 256 tokens is getting 51 KB a stage into the SM: at the matrix rate a stage lasts 512 cycles.  TMA moves a row of a box in
+// some 4 cycles whatever its length (measured: 16 / 29 / 47 bytes a cycle and SM with rows of 64 / 128 / 256 bytes, and the swizzle allows
+// 128), cp.async 64 to 67; 384 rows by TMA were 1470 cycles.  So the eight epilogue warps, idle until the end, bring the stages with cp.async,
+// 16 bytes a lane, swizzled as they land: each warp waits for its own copies of a stage two stages later, makes them visible to the
+// tensor core (fence.proxy.async) and arrives.
 //
 // GATED: two MMAs into two accumulators: gate rows and up rows of the same 128 channels against the same token tile; a lane then
 // holds both values of its channel and the epilogue writes silu(gate) * up without an exchange.
 //
 // The k range of a tile may be split over a cluster (tcgen05_cluster_epilogue.cuh).
 //
-// Warp roles: warp 0 = TMA producer, warp 1 = tensor-memory allocation and MMA issue, then 8 epilogue warps.  full[s] (bytes landed) ->
-// MMA -> empty[s] (tcgen05.commit) -> producer; every wait is bounded as in the other tcgen05 kernels.
+// Warp roles: warp 0 = tensor-memory allocation and MMA issue, then 8 warps that copy and, at the end, run the epilogue.  full[s] (8
+// arrivals) -> MMA -> empty[s] (tcgen05.commit) -> copies; every wait is bounded as in the other tcgen05 kernels.
 // Programmatic dependent launch: weights of the first stages are requested before the wait for the previous kernel, the activations'
 // codes (the quantizer's output) after it.
 //
@@ -24,6 +30,7 @@
 
 #include "../../include/shrewq.h"
 #include "dests.cuh"
+#include "ptx_fp4.cuh"
 #include "ptx_small.cuh"
 #include "ptx_tcgen05.cuh"
 #include "ptx_tcgen05_fp4.cuh"
@@ -35,8 +42,8 @@ namespace {
 
 constexpr int kFp4StageK = 256;       // codes of k a stage: rows of 128 bytes
 constexpr int kFp4RowBytes = 128;
-constexpr int kFp4Groups = 2;         // epilogue groups of 4 warps
-constexpr int kFp4GemmThreads = 64 + 128 * kFp4Groups;
+constexpr int kFp4Groups = 2;         // groups of 4 warps that copy and run the epilogue
+constexpr int kFp4Copiers = 4 * kFp4Groups, kFp4GemmThreads = 32 + 32 * kFp4Copiers;
 constexpr uint32_t kTimeoutFp4 = 5;   // DeviceStatus::timeout_flag of this kernel
 
 template <int TOK, bool NV, bool GATED>
@@ -83,11 +90,34 @@ __device__ __forceinline__ constexpr uint32_t fp4_idesc(bool nv, int m, int n, u
     return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (nv ? 0u : 1u << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 4) | (sf << 29);
 }
 
+// `rows` rows of 128 bytes of a K-major operand into a swizzled tile: 4 rows an instruction, the warp's share of them.  src: the lane's first
+// row and 16-byte piece; rows past `last` repeat it (what they give is not stored).
+template <int ROWS>
+struct CopyRows {
+    static constexpr int kInstr = ROWS / 4 / kFp4Copiers;  // of a warp
+    const uint8_t *src[kInstr];
+    __device__ __forceinline__ CopyRows(const uint8_t *base, size_t pitch, int row0, int last, int copier, int lane) {
+#pragma unroll
+        for (int j = 0; j < kInstr; ++j) {
+            const int r = row0 + (copier * kInstr + j) * 4 + (lane >> 3);
+            src[j] = base + (size_t)(r < last ? r : last) * pitch + (lane & 7) * 16;
+        }
+    }
+    // `in`: false = zeros
+    __device__ __forceinline__ void copy(uint32_t tile, size_t byte, int copier, int lane, bool in) const {
+#pragma unroll
+        for (int j = 0; j < kInstr; ++j) {
+            const int r = (copier * kInstr + j) * 4 + (lane >> 3);
+            copy_async_16(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4), in ? src[j] + byte : src[j], in);
+        }
+    }
+};
+
 template <int TOK, bool NV, bool GATED, typename YT>
 __global__ void __launch_bounds__(kFp4GemmThreads, 1)
-gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2, const __grid_constant__ CUtensorMap tmap_x,
-                const uint8_t *__restrict__ w_pieces, const uint8_t *__restrict__ w2_pieces, const uint8_t *__restrict__ x_pieces, Operands ops,
-                YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue, int S, int rounds_per_cta, DeviceStatus *status) {
+gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__ w2_codes, const uint8_t *__restrict__ x_codes, const uint8_t *__restrict__ w_pieces,
+                const uint8_t *__restrict__ w2_pieces, const uint8_t *__restrict__ x_pieces, Operands ops, YT *__restrict__ y, int M, int N, int K, size_t ldy,
+                int epilogue, int S, int rounds_per_cta, DeviceStatus *status) {
     using C = Fp4Cfg<TOK, NV, GATED>;
     pdl_launch_dependents();
     SHREWQ_DYNAMIC_SMEM(uint8_t, smem_raw);
@@ -98,8 +128,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     // token tiles fastest: the CTAs that share a weight tile start together, so it comes from DRAM once
     const int m_tiles = (M + TOK - 1) / TOK;
     constexpr int kMode = GATED ? kEpiColumns : kEpiPlain;
-    // (the rank from the block's index: a value that the compiler knows to be the same in all lanes, as the operands of TMA and
-    // tcgen05 instructions are that derive from it)
+    // (the rank from the block's index: a value that the compiler knows to be the same in all lanes, as the operands of tcgen05
+    // instructions are that derive from it)
     const uint32_t rank = blockIdx.x % (unsigned)S;
     const int tile = (int)(blockIdx.x / (unsigned)S);
     const int m0 = tile % m_tiles * TOK, n0 = tile / m_tiles * 128;
@@ -112,13 +142,14 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (threadIdx.x == 0) {
         ctl->abort_flag = 0;
         for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(bars + kFullBar + s * 8, 1);
+            mbar_init(bars + kFullBar + s * 8, 32 * kFp4Copiers);
             mbar_init(bars + kEmptyBar + s * 8, 1);
         }
         mbar_init(bars + kAccBar, 1);
         mbar_fence_init();
     }
-    if (warp == 1) {
+    if (warp == 0) {
+        __syncwarp();
         tc_alloc_512(smem_u32(&ctl->tmem_base));
         tc_relinquish();
     }
@@ -127,45 +158,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
     bool ok = true;
+    const int copier = warp - 1, group = copier >> 2, quad = warp & 3;
 
     if (warp == 0) {
-        if (elect_one()) {
-            auto load_w = [&](int i, int s) {
-                const uint32_t dst = smem_base + s * C::kStageBytes, fb = bars + kFullBar + s * 8;
-                mbar_expect_tx(fb, C::kStageBytes);
-                const int r = r_begin + i;
-                const size_t at = ((size_t)(n0 >> 7) * pieces + (size_t)r * C::kPieces) * 512;
-                tma_load_2d(dst, &tmap_w, r * kFp4RowBytes, n0, fb);
-                bulk_load_1d(dst + C::kSfaOff, w_pieces + at, C::kSfaBytes, fb);
-                if constexpr (GATED) {
-                    tma_load_2d(dst + C::kABytes, &tmap_w2, r * kFp4RowBytes, n0, fb);
-                    bulk_load_1d(dst + C::kSfaOff + C::kSfaBytes, w2_pieces + at, C::kSfaBytes, fb);
-                }
-            };
-            // the token tiles of the pieces beyond the last one are read from it again: their columns are not stored
-            const int last_tile = (M - 1) >> 7;
-            auto load_x = [&](int i, int s) {
-                const uint32_t dst = smem_base + s * C::kStageBytes, fb = bars + kFullBar + s * 8;
-                tma_load_2d(dst + C::kBOff, &tmap_x, (r_begin + i) * kFp4RowBytes, m0, fb);
-#pragma unroll
-                for (int j = 0; j < C::kTokTiles; ++j) {
-                    const int xt = (m0 >> 7) + j < last_tile ? (m0 >> 7) + j : last_tile;
-                    bulk_load_1d(dst + C::kSfbOff + j * C::kPieces * 512, x_pieces + ((size_t)xt * pieces + (size_t)(r_begin + i) * C::kPieces) * 512, C::kPieces * 512, fb);
-                }
-            };
-            const int pre = rounds < C::kStages ? rounds : C::kStages;
-            for (int i = 0; i < pre; ++i) load_w(i, i);
-            pdl_wait();
-            for (int i = 0; i < pre; ++i) load_x(i, i);
-            uint32_t s = 0, ph = 0;
-            for (int i = pre; i < rounds; ++i) {
-                if (!fp4_wait(bars + kEmptyBar + s * 8, ph, ctl, status, 0, s)) break;
-                load_w(i, s);
-                load_x(i, s);
-                if (++s == C::kStages) { s = 0; ph ^= 1; }
-            }
-        }
-    } else if (warp == 1) {
         if (elect_one()) {
             pdl_wait();  // a stage is full only with its activations: the time limit of the waits starts when they exist
             uint32_t s = 0, ph = 0;
@@ -173,11 +168,12 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             for (int i = 0; i < rounds; ++i) {
                 good = fp4_wait(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
                 if (!good) break;
+                fence_proxy_async_smem();
                 tc_fence_after();
                 const uint32_t base = smem_base + s * C::kStageBytes;
                 const uint32_t sf = tmem + C::kAccCols + s * C::kSfCols;             // A pieces (gate, up), then B pieces
                 constexpr int kSfbCol = C::kMats * C::kPieces * 4, kBStep = 4 * C::kTokTiles;
-// descriptors of this stage: every other one is a constant away (16-byte units; the address field does not overflow)
+                // descriptors of this stage: every other one is a constant away (16-byte units; the address field does not overflow)
                 const uint64_t adesc = make_b_desc(base), bdesc = make_b_desc(base + C::kBOff), sdesc = make_scale_desc(base + C::kSfaOff);
                 const uint32_t tok_col = TOK < 128 ? (uint32_t)((m0 & 127) >> 5) : 0u;  // a token tile of half a piece
 #pragma unroll
@@ -205,8 +201,47 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         }
         __syncwarp();
     } else {
-        const int group = (warp - 2) >> 2, quad = warp & 3;
-        pdl_wait();  // y may be in use by the previous kernel of the stream
+        // ---------------- copies, then the epilogue ----------------
+        const size_t pitch = (size_t)((K + 31) >> 5) * 16;
+        const int t = (int)threadIdx.x - 32;  // 0 .. 255
+        const CopyRows<128> gate_rows(w_codes, pitch, n0, N - 1, copier, lane), up_rows(w2_codes, pitch, n0, N - 1, copier, lane);
+        const CopyRows<TOK> token_rows(x_codes, pitch, m0, M - 1, copier, lane);
+        auto copy_w = [&](int i, int s) {
+            const uint32_t dst = smem_base + s * C::kStageBytes;
+            const size_t byte = (size_t)(r_begin + i) * kFp4RowBytes;
+            const bool in = byte + (lane & 7) * 16 < pitch;  // (codes past the end of a row: zeros)
+            gate_rows.copy(dst, byte, copier, lane, in);
+            if constexpr (GATED) up_rows.copy(dst + C::kABytes, byte, copier, lane, in);
+            const size_t at = ((size_t)(n0 >> 7) * pieces + (size_t)(r_begin + i) * C::kPieces) * 512;
+            if (t < C::kMats * C::kSfaBytes / 16) {
+                const int mat = GATED ? t / (C::kSfaBytes / 16) : 0, c = t % (C::kSfaBytes / 16);
+                copy_async_16(dst + C::kSfaOff + t * 16, (mat ? w2_pieces : w_pieces) + at + c * 16, true);
+            }
+        };
+        // the token tiles of the pieces beyond the last one are read from it again: their columns are not stored
+        const int last_tile = (M - 1) >> 7;
+        auto copy_x = [&](int i, int s) {
+            const uint32_t dst = smem_base + s * C::kStageBytes;
+            const size_t byte = (size_t)(r_begin + i) * kFp4RowBytes;
+            token_rows.copy(dst + C::kBOff, byte, copier, lane, byte + (lane & 7) * 16 < pitch);
+            if (t < C::kSfbBytes / 16) {
+                const int j = t / (C::kPieces * 32), c = t % (C::kPieces * 32);
+                const int xt = (m0 >> 7) + j < last_tile ? (m0 >> 7) + j : last_tile;
+                copy_async_16(dst + C::kSfbOff + t * 16, x_pieces + ((size_t)xt * pieces + (size_t)(r_begin + i) * C::kPieces) * 512 + c * 16, true);
+            }
+        };
+        const int pre = rounds < C::kStages ? rounds : C::kStages;
+        for (int i = 0; i < pre; ++i) copy_w(i, i);
+        pdl_wait();  // (and y may be in use by the previous kernel of the stream)
+        for (int i = 0; i < rounds; ++i) {
+            const int s = i % C::kStages;
+            if (i >= C::kStages) {
+                mbar_wait_all<kTimeoutFp4>(bars + kEmptyBar + s * 8, (uint32_t)(i / C::kStages - 1) & 1u, ctl, status, 0, s);
+                copy_w(i, s);
+            }
+            copy_x(i, s);
+            copy_async_arrive(bars + kFullBar + s * 8);
+        }
         mbar_wait_all<kTimeoutFp4>(bars + kAccBar, 0, ctl, status, 4, 0);
         ok = warp_ok(ctl);
         tc_fence_after();
@@ -214,26 +249,25 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             cluster_finish<TOK, kFp4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0);
     }
     if (S > 1) {
-        const int group = (warp - 2) >> 2, quad = warp & 3;
         tc_fence_before();
         __syncwarp();
         cluster_arrive();  // every CTA of the tile has its sums: the stages are idle everywhere
         cluster_wait();
         tc_fence_after();
-        if (warp >= 2 && ok) cluster_send<TOK, kFp4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane);
+        if (warp >= 1 && ok) cluster_send<TOK, kFp4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane);
         __syncwarp();
         cluster_arrive();  // and has received the others'
         cluster_wait();
-        if (warp >= 2)
+        if (warp >= 1)
             cluster_finish<TOK, kFp4Groups, kMode, YT>(tmem, smem, reinterpret_cast<const float *>(smem + C::kSlotOff), S, rank, group, quad, lane, ok, ops, y, M, N,
                                                        ldy, epilogue, n0, m0);
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 0) {
         if (ctl->abort_flag) {
-            for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies and MMAs in flight get a bounded moment to land
+            for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // MMAs in flight get a bounded moment to land
         }
         tc_fence_after();
         __syncwarp();

@@ -100,6 +100,8 @@ __device__ __forceinline__ void copy_async_16(uint32_t dst, const void *src, boo
 __device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
+// this thread arrives on the barrier (of a count that includes it) when all of its copies so far have landed
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all but the newest N groups of this thread have landed, visible to this thread
 template <int N>

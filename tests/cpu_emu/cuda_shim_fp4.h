@@ -101,3 +101,9 @@ static inline void copy_async_wait() {
     }
     v.resize(kept);
 }
+static inline void mbar_arrive(uint32_t bar);
+static inline void copy_async_arrive(uint32_t bar) {
+    for (auto &c : emu::g_copies) memcpy(c.dst, c.data, c.bytes);
+    emu::g_copies.clear();
+    mbar_arrive(bar);
+}

@@ -25,7 +25,31 @@ inline void cp_scales(Block *blk, uint32_t taddr, uint64_t desc) {
         }
     }
 }
-// rows of A and D: 128 of block `d`; B and its scales as given
+// rows 128 r .. of A, its scales and D in block r of the pair (or the one block), rows 128 r .. of B there too, B's scales in every block
+inline void mma_fp4_pair(Block *leader, bool nv, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    const uint32_t N = ((idesc >> 17) & 0x3Fu) << 3, M = ((idesc >> 24) & 0x1Fu) << 4, sa = (idesc >> 29) & 3u, sb = (idesc >> 4) & 3u;
+    EMU_CHECK(leader->rank == 0 && M == 256 && N == 256 && ((idesc >> 7) & 7u) == 1 && ((idesc >> 10) & 7u) == 1, "E2M1 operands, 256 x 256, issued by the leader");
+    EMU_CHECK(((idesc >> 23) & 1u) == (nv ? 0u : 1u) && (nv ? sa == 0 && sb == 0 : (sa & 1) == 0 && (sb & 1) == 0), "scale type and ids");
+    const uint32_t dcol = d_tmem & 0xFFFF, ca = sfa & 0xFFFF, cb = sfb & 0xFFFF, per = nv ? 16 : 32;
+    if (dcol + N > 512 || ca + 4 > 512 || cb + 8 > 512) { fail("block-scaled MMA outside tensor memory"); return; }
+    for (uint32_t r = 0; r < 2; ++r) {
+        Block *blk = leader->cluster[r];
+        auto scale = [&](uint32_t col, uint32_t row, uint32_t group, uint32_t id) {
+            return scale_value(nv, (blk->tmem[(row & 31) * 512 + col + (row >> 5)] >> (8 * (id + group))) & 0xFF);
+        };
+        std::vector<float> a(128 * 64), b(N * 64);
+        for (uint32_t i = 0; i < 128; ++i)
+            for (uint32_t k = 0; k < 64; ++k) a[i * 64 + k] = fp4_operand(blk, a_desc, i, k) * scale(ca, i, k / per, sa);
+        for (uint32_t i = 0; i < N; ++i)
+            for (uint32_t k = 0; k < 64; ++k) b[i * 64 + k] = fp4_operand(leader->cluster[i >> 7], b_desc, i & 127, k) * scale(cb, i, k / per, sb);
+        for (uint32_t m = 0; m < 128; ++m)
+            for (uint32_t n = 0; n < N; ++n) {
+                double acc = accumulate ? (double)__uint_as_float(blk->tmem[m * 512 + dcol + n]) : 0.0;
+                for (uint32_t k = 0; k < 64; ++k) acc += (double)a[m * 64 + k] * b[n * 64 + k];
+                blk->tmem[m * 512 + dcol + n] = __float_as_uint((float)acc);
+            }
+    }
+}
 inline void mma_fp4(Block *blk, bool nv, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     const uint32_t N = ((idesc >> 17) & 0x3Fu) << 3, M = ((idesc >> 24) & 0x1Fu) << 4, sa = (idesc >> 29) & 3u, sb = (idesc >> 4) & 3u;
     EMU_CHECK(M == 128 && ((idesc >> 7) & 7u) == 1 && ((idesc >> 10) & 7u) == 1, "E2M1 operands, 128 rows");
@@ -61,6 +85,17 @@ template <bool NV>
 static inline void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     if (emu::tc_deferred()) emu::tc_push([=] { emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate); });
     else emu::mma_fp4(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate);
+}
+
+static inline void tc_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+    auto both = [=] { for (int r = 0; r < 2; ++r) emu::cp_scales(emu::g_block->cluster[r], taddr, desc); };
+    if (emu::tc_deferred()) emu::tc_push(both);
+    else both();
+}
+template <bool NV>
+static inline void tc_mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (emu::tc_deferred()) emu::tc_push([=] { emu::mma_fp4_pair(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate); });
+    else emu::mma_fp4_pair(emu::g_block, NV, d, a, b, idesc, sfa, sfb, accumulate);
 }
 
 // tcgen05.mma kind::f16 with f16 operands: A from tensor memory, B K-major in shared memory with the 128-byte swizzle

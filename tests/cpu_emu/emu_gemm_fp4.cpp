@@ -7,6 +7,7 @@
 #include "cuda_shim_tcgen05_fp4.h"
 #include "../../shrew_b200/csrc/gemv_fp4_kernels.cuh"
 #include "../../shrew_b200/csrc/gemm_fp4_kernels.cuh"
+#include "../../shrew_b200/csrc/gemm_fp4_pair_kernels.cuh"
 #include "../../shrew_b200/csrc/gemm_fp4_bf16_kernels.cuh"
 #include "../../shrew_b200/csrc/gemm_fp4_f16_kernels.cuh"
 
@@ -52,12 +53,18 @@ int run(const uint8_t *const *codes, const uint8_t *const *scales, const float *
     emu::launch(M, (unsigned)threads, [&] {
         fp4_quantize_rows_kernel<float, NV, true>(x, M, K, K, 0, &params[0].x_scale, nullptr, 0, nullptr, blocks, reinterpret_cast<uint32_t *>(xc), xp);
     });
-    const CUtensorMap tw = map2d(codes[0], pitch, N, 128, 128), tw2 = map2d(codes[GATED ? 1 : 0], pitch, N, 128, 128), tx = map2d(xc, pitch, M, 128, TOK);
     const Operands ops{alpha[0].data(), bias[0], alpha[GATED ? 1 : 0].data(), bias[GATED ? 1 : 0]};
     DeviceStatus status{0, 0, 0, 0};
+    if (split == 2) {  // CTA pairs
+        const int per = GATED ? 128 : 256, tiles = (N + per - 1) / per * ((M + 255) / 256), pairs = tiles < 2 ? tiles : 2;
+        emu::launch_cluster2((unsigned)(2 * pairs), 1, 1, kPairThreads, Fp4PairCfg<NV, GATED, float>::kSmemBytes, [&] {
+            gemm_fp4_pair_kernel<NV, GATED, float>(codes[0], codes[GATED ? 1 : 0], xc, wp[0], wp[GATED ? 1 : 0], xp, ops, y, M, N, K, ldy, epilogue, tiles, pairs, &status);
+        });
+        return outcome(status);
+    }
     const int rounds = (K + kFp4StageK - 1) / kFp4StageK, per_cta = split ? (rounds + 1) / 2 : rounds;
     launch_tiles((size_t)(N + 127) / 128 * ((M + TOK - 1) / TOK), split, kFp4GemmThreads, C::kSmemRequest, [&] {
-        gemm_fp4_kernel<TOK, NV, GATED, float>(tw, tw2, tx, wp[0], wp[GATED ? 1 : 0], xp, ops, y, M, N, K, ldy, epilogue, split ? 2 : 1, per_cta, &status);
+        gemm_fp4_kernel<TOK, NV, GATED, float>(codes[0], codes[GATED ? 1 : 0], xc, wp[0], wp[GATED ? 1 : 0], xp, ops, y, M, N, K, ldy, epilogue, split ? 2 : 1, per_cta, &status);
     });
     return outcome(status);
 }
@@ -134,7 +141,7 @@ int run_h4(const uint8_t *const *codes, const uint8_t *const *scales, const floa
 
 }  // namespace
 
-// async_seed: 0 = copies and tensor-core work complete at issue, else deferred in an adversarial order
+// split: 1 = the k range of a tile over a cluster of two, 2 = CTA pairs (tok is 256 there, 128 in the list of gated ones).  async_seed: 0 = copies and tensor-core work complete at issue, else deferred in an adversarial order
 extern "C" int emu_gemm_fp4(const uint8_t *const *codes, const uint8_t *const *scales, const float *const *g, const float *const *bias, const float *x, float x_scale,
                             int M, int N, int K, int tok, int nv, int gated, float *y, size_t ldy, int epilogue, int split, unsigned async_seed) {
     emu::g_tma_async_seed = async_seed;

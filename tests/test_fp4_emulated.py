@@ -265,7 +265,9 @@ def test_residual_norm(emu, x_dtype, b_dtype, h_dtype, M, D, V, pre, post, gate_
 @pytest.mark.parametrize("nv", [False, True])
 @pytest.mark.parametrize("M,N,K,tok,gated,split,seed", [(70, 130, 600, 64, False, 0, 0), (100, 129, 256, 128, False, 0, 3), (300, 40, 330, 256, False, 1, 0),
                                                         (33, 70, 1300, 64, True, 1, 5), (130, 128, 90, 128, True, 0, 0), (1, 1, 1, 64, False, 0, 0),
-                                                        (200, 20, 2600, 256, False, 0, 7), (40, 20, 2600, 64, False, 1, 9), (130, 60, 520, 128, True, 1, 2)])
+                                                        (200, 20, 2600, 256, False, 0, 7), (40, 20, 2600, 64, False, 1, 9), (130, 60, 520, 128, True, 1, 2),
+                                                        (140, 270, 600, 256, False, 2, 0), (300, 100, 1700, 256, False, 2, 4), (200, 150, 300, 128, True, 2, 0),
+                                                        (290, 30, 1600, 128, True, 2, 8)])
 def test_four_bits_by_four_bits(emu_gemm, nv, M, N, K, tok, gated, split, seed):
     g = torch.Generator().manual_seed(M + K)
     x = aligned((M, K), torch.float32)

@@ -168,6 +168,20 @@ def test_gated_pair(fmt, rounded, x_dtype, m, n, k):
     near(h, O.product(xd, wg, bg, up=wu, bias_up=bu), O.product_bound(xd, wg, k, up=wu, bias=bg, bias_up=bu))
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(129, 9473, 33), (140, 9600, 320), (300, 4900, 600), (513, 3400, 2080), (1100, 2000, 1600)])
+def test_wide_products_of_quantized_activations(fmt, gated, m, n, k):
+    """Outputs that fill the machine, in both directions."""
+    lin, w, b = layer(n, k, fmt, m + n, quantize_activations=True, activation_scale=0.5)
+    up, wu, bu = layer(n, k, fmt, 2, bias=False, quantize_activations=True, activation_scale=0.5)
+    x = acts(m, k, BF16) / (8 * k ** 0.5)
+    xq = O.quantize(x.double().cpu().numpy(), fmt is Fp4Format.Nv, 0.5)[3]
+    y = lin.forward_gate_up_silu(up, x) if gated else lin.forward(x, out_dtype=F32)
+    pair = dict(up=wu, bias_up=bu) if gated else {}
+    near(y, O.product(xq, w, b, **pair), O.product_bound(xq, w, k, bias=b, **pair))
+
+
 @pytest.mark.parametrize("rounded", [False, True])
 @pytest.mark.parametrize("m", [3, 40, 150])
 def test_column_slice_of_a_wider_buffer(rounded, m):
