@@ -43,7 +43,7 @@ namespace {
 constexpr int kFp4StageK = 256;       // codes of k a stage: rows of 128 bytes
 constexpr int kFp4RowBytes = 128;
 constexpr int kFp4Groups = 2;         // groups of 4 warps that copy and run the epilogue
-constexpr int kFp4Copiers = 4 * kFp4Groups, kFp4GemmThreads = 32 + 32 * kFp4Copiers;
+constexpr int kFp4Copiers = 4 * kFp4Groups, kFp4GemmThreads = 32 + 32 * kFp4Copiers + 32;
 constexpr uint32_t kTimeoutFp4 = 5;   // DeviceStatus::timeout_flag of this kernel
 
 template <int TOK, bool NV, bool GATED>
@@ -136,13 +136,14 @@ gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__
     const int rounds_total = (K + kFp4StageK - 1) / kFp4StageK, r_begin = (int)rank * rounds_per_cta;
     const int rounds = min(rounds_total - r_begin, rounds_per_cta);  // >= 1 by construction of the grid
     const size_t pieces = (size_t)rounds_total * C::kPieces;  // along a row
-    constexpr uint32_t kFullBar = 0, kEmptyBar = C::kStages * 8, kAccBar = 2 * C::kStages * 8;
+    constexpr uint32_t kFullBar = 0, kEmptyBar = C::kStages * 8, kReadyBar = 2 * C::kStages * 8, kAccBar = 3 * C::kStages * 8;
     const uint32_t bars = smem_u32(bar_area), smem_base = smem_u32(smem);
 
     if (threadIdx.x == 0) {
         ctl->abort_flag = 0;
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(bars + kFullBar + s * 8, 32 * kFp4Copiers);
+            mbar_init(bars + kReadyBar + s * 8, 1);
             mbar_init(bars + kEmptyBar + s * 8, 1);
         }
         mbar_init(bars + kAccBar, 1);
@@ -159,17 +160,20 @@ gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
     bool ok = true;
     const int copier = warp - 1, group = copier >> 2, quad = warp & 3;
+    const bool epi = warp >= 1 && warp <= kFp4Copiers;
 
     if (warp == 0) {
         if (elect_one()) {
             pdl_wait();  // a stage is full only with its activations: the time limit of the waits starts when they exist
             uint32_t s = 0, ph = 0;
-            bool good = true;
+            bool good = true, ready = false;
             for (int i = 0; i < rounds; ++i) {
-                good = fp4_wait(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
+                good = ready || fp4_wait(bars + kReadyBar + s * 8, ph, ctl, status, 1, s);
                 if (!good) break;
-                fence_proxy_async_smem();
                 tc_fence_after();
+                // (a look takes 150 to 300 cycles here: the next stage's is under way while this one's MMAs are issued)
+                const uint32_t next = s + 1 == C::kStages ? 0 : s + 1, next_ph = s + 1 == C::kStages ? ph ^ 1u : ph;
+                ready = mbar_test(bars + kReadyBar + next * 8, next_ph);
                 const uint32_t base = smem_base + s * C::kStageBytes;
                 const uint32_t sf = tmem + C::kAccCols + s * C::kSfCols;             // A pieces (gate, up), then B pieces
                 constexpr int kSfbCol = C::kMats * C::kPieces * 4, kBStep = 4 * C::kTokTiles;
@@ -195,9 +199,22 @@ gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__
                     }
                 }
                 tc_commit(bars + kEmptyBar + s * 8);
-                if (++s == C::kStages) { s = 0; ph ^= 1; }
+                s = next, ph = next_ph;
             }
             if (good) tc_commit(bars + kAccBar);
+        }
+        __syncwarp();
+    } else if (warp == kFp4GemmThreads / 32 - 1) {
+        // ---------------- relay: copies that have landed -> visible to the tensor core -> the MMAs ----------------
+        if (elect_one()) {
+            pdl_wait();
+            uint32_t s = 0, ph = 0;
+            for (int i = 0; i < rounds; ++i) {
+                if (!fp4_wait(bars + kFullBar + s * 8, ph, ctl, status, 5, s)) break;
+                fence_proxy_async_smem();
+                mbar_arrive(bars + kReadyBar + s * 8);
+                if (++s == C::kStages) { s = 0; ph ^= 1; }
+            }
         }
         __syncwarp();
     } else {
@@ -254,11 +271,11 @@ gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__
         cluster_arrive();  // every CTA of the tile has its sums: the stages are idle everywhere
         cluster_wait();
         tc_fence_after();
-        if (warp >= 1 && ok) cluster_send<TOK, kFp4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane);
+        if (epi && ok) cluster_send<TOK, kFp4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane);
         __syncwarp();
         cluster_arrive();  // and has received the others'
         cluster_wait();
-        if (warp >= 1)
+        if (epi)
             cluster_finish<TOK, kFp4Groups, kMode, YT>(tmem, smem, reinterpret_cast<const float *>(smem + C::kSlotOff), S, rank, group, quad, lane, ok, ops, y, M, N,
                                                        ldy, epilogue, n0, m0);
     }

@@ -1,19 +1,23 @@
 // The 4-bit by 4-bit forward (gemm_fp4_kernels.cuh) on CTA pairs, for batches whose tiles fill the machine: clusters of two CTAs compute
-// tiles of 256 weight rows by 256 tokens with tcgen05.mma.cta_group::2, one after the other.
+// tiles of 256 tokens by 256 weight rows with tcgen05.mma.cta_group::2, one after the other.
 //
 // Why: a single CTA's 128 x 256 tile needs 51 KB a stage of 256 k, which at the 64 to 67 bytes a cycle that an SM takes in last 780 cycles,
-// against 512 of matrix work.  In a pair each CTA brings its own 128 rows and only half of the tokens: 35 KB, 540 cycles.
+// against 512 of matrix work.  In a pair each CTA brings its own 128 tokens and only half of the weight rows: 35 KB (MX) or 38 KB (NV).
 //
-// Each CTA holds 128 rows of A with their scales, 128 of the 256 tokens of B, and the scales of all 256 tokens; the leader issues
-// tcgen05.cp and tcgen05.mma for both, and a stage is released to both CTAs (tcgen05.commit).
-// GATED: even rows of A are gate rows, odd ones the up rows of the same 64 channels, so that neighbouring lanes of the accumulator hold both
-// values of a channel.
+// A = tokens (128 in each CTA, with their scales), B = weight rows (128 in each CTA; the scales of all 256 in both); the leader issues
+// tcgen05.cp and tcgen05.mma for both, and a stage is released to both CTAs (tcgen05.commit).  GATED: the first CTA brings gate rows, the
+// second one the up rows of the same 128 channels.
+// Tokens are the lanes of the accumulator, so a thread holds neighbouring channels of one token, gate and up values alike: it packs 16
+// bytes of output at a time, and a warp turns its 32 x 32 piece into whole rows through 2 KB (4 KB for f32) of its own.  With channels as lanes, as the kernels for few
+// tokens have them, every output was a two-byte store to shared memory and gate and up values had to change lanes: some 370 instructions
+// for each warp and 16 columns, 7500 to 8400 cycles a tile, in which the tensor cores stood still.
 //
-// Warp roles: warp 0 = tensor-memory allocation, then in the leader the MMAs, in the other CTA the relay of its full stages to the leader;
-// 8 epilogue warps; 8 copying warps, two groups of 4 that take the stages in turn (a group's wait for its stage and its requests take some 400
-// cycles, nearly a stage).  Copies arrive on the stage's barrier by themselves (cp.async.mbarrier.arrive), and the thread that waits there
-// makes them visible to the tensor core.  The relay is one plain arrival a stage: with .release.cluster, by each copying warp, it took 1200
-// cycles a stage.  The copying warps run ahead into the next tile during an epilogue; the MMAs wait until the accumulators have been read.
+// Warp roles: warp 0 = tensor-memory allocation, and in the leader the MMAs; four groups of 4 warps = epilogue, the first two of them also
+// copies, taking the stages in turn; the last warp = relay.  Copies arrive on the stage's barrier by themselves
+// (cp.async.mbarrier.arrive); the relay of each CTA waits there, makes them visible to the tensor core (fence.proxy.async) and arrives at
+// the leader.  (Arrivals with .release.cluster by the copying warps took 1200 cycles a stage.)  The accumulators, 256 columns, and the stages' scales
+// fill tensor memory, so the MMAs of the next tile wait until the sums have been read: all warps that are free then take part, after the
+// next tile's first stages are under way.
 //
 // Device code only; also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once
@@ -23,8 +27,9 @@
 namespace shrewq {
 namespace {
 
-constexpr int kPairTok = 256, kPairHalf = 128;
-constexpr int kPairThreads = 32 + 256 + 256;
+constexpr int kPairTok = 256, kPairHalf = 128;  // tokens of a tile, and those that a CTA brings
+constexpr int kPairGroups = 4;                  // groups of 4 warps: two run the epilogue only, two also copy
+constexpr int kPairThreads = 32 + 128 * kPairGroups + 32;
 constexpr uint32_t kTimeoutFp4Pair = 8;  // DeviceStatus::timeout_flag of this kernel
 
 template <bool NV, bool GATED, typename YT>
@@ -33,82 +38,111 @@ struct Fp4PairCfg {
     static constexpr int kABytes = 128 * kFp4RowBytes, kBBytes = kPairHalf * kFp4RowBytes;
     static constexpr int kSfaBytes = kPieces * 512, kSfbBytes = 2 * kPieces * 512;
     static constexpr int kBOff = kABytes, kSfaOff = kBOff + kBBytes, kSfbOff = kSfaOff + kSfaBytes, kStageBytes = kSfbOff + kSfbBytes;
-    static constexpr int kAccCols = kPairTok, kSfCols = 3 * kPieces * 4;
-    static constexpr int kChannels = GATED ? 64 : 128;                                  // of a CTA
-    static constexpr int kOutBytes = kEpiChunk * kChannels * (int)sizeof(YT);           // a staging tile; two for each epilogue group
-    static constexpr int kMaxSmem = (225 * 1024 - 4 * kOutBytes) / kStageBytes, kMaxTmem = (512 - kAccCols) / kSfCols;
+    static constexpr int kSfCols = 3 * kPieces * 4;                                     // tensor memory: accumulators, then the stages' scales
+    static constexpr int kChannels = GATED ? 128 : 256;                                 // of a tile
+    static constexpr int kOutBytes = 32 * 32 * (int)sizeof(YT) + 512;                   // of a warp: a piece of the output, its columns' factors
+    static constexpr int kMaxSmem = (225 * 1024 - 4 * kPairGroups * kOutBytes) / kStageBytes, kMaxTmem = (512 - kPairTok) / kSfCols;
     static constexpr int kStages = kMaxSmem < kMaxTmem ? kMaxSmem : kMaxTmem;
-    static constexpr int kOutOff = kStages * kStageBytes, kBarOff = kOutOff + 4 * kOutBytes;
+    static constexpr int kOutOff = kStages * kStageBytes, kBarOff = kOutOff + 4 * kPairGroups * kOutBytes;
     static constexpr int kSmemBytes = kBarOff + 1024 + 1024;
     static_assert(kStages >= 4 && kSmemBytes <= 227 * 1024 && kStageBytes % 1024 == 0, "stages");
-    static_assert((2 * kStages + 2) * 8 <= 512, "barriers");
+    static_assert((3 * kStages + 2) * 8 <= 512, "barriers");
 };
 
-// 16 tokens at a time of this CTA's 128 rows: sums -> scale, bias, elementwise op -> staging tile -> whole rows of y.  The tile is written
-// while the one before is still being read, so one barrier a step is enough.  `step` counts them.
+// silu(g) * u = u g / (1 + 2^(-g log2 e)): four instructions less than with __expf and __fdividef, whose care for denormal results has
+// nothing to do here (0 for them is within 2^-126 |u g|).
+__device__ __forceinline__ float pair_silu(float g, float u) {
+    return g * recip_approx(1.0f + exp2_approx(-1.44269504f * g)) * u;
+}
+
+// This warp's 32 tokens: sums -> scale, bias, elementwise op -> rows of y.  Two steps of 32 sums a thread: 32 channels each (group, and 4 groups further),
+// or the gate and up sums of 16.  The second step's sums are read before the first one's rows are written, so that the next tile's MMAs
+// can begin.
 template <bool GATED, typename YT>
-__device__ __forceinline__ void pair_epilogue(uint32_t tmem_d, uint8_t *stages, uint32_t &step, uint32_t acc_free_leader, int group, int quad, int lane, bool ok,
-                                              const Operands &ops, YT *__restrict__ y, int M, int N, size_t ldy, int epilogue, int n0, int m0, bool vec_ok) {
-    constexpr int CW = kEpiChunk, CH = GATED ? 64 : 128, RB = CH * (int)sizeof(YT), EPV = 16 / (int)sizeof(YT), PPR = RB / 16, PIECES = CW * PPR;
-    const int row = quad * 32 + lane, ch = GATED ? row >> 1 : row, n = n0 + ch;
-    const uint32_t taddr = tmem_d + ((uint32_t)(quad * 32) << 16);
-    const bool is_up = GATED && (row & 1), n_ok = n < N;
-    const float *bias = is_up ? ops.bias2 : ops.bias;
-    const float sc = n_ok ? (is_up ? ops.scales2 : ops.scales)[n] : 0.0f, bs = n_ok && bias ? bias[n] : 0.0f;
-    uint32_t raw[CW];
-    tc_ld16(taddr + group * CW, raw);
-#pragma unroll 1
-    for (int c = group; c < kPairTok / CW; c += kFp4Groups, ++step) {
-        uint8_t *stage = stages + (group * 2 + (step & 1)) * (CW * RB);
-        YT *out_st = reinterpret_cast<YT *>(stage);
+struct PairEpilogue {
+    static constexpr int EPV = 16 / (int)sizeof(YT), SEGS = 32 / EPV;  // 16-byte pieces of a row of 32 channels
+    uint8_t *own;                                                       // [32 tokens][32 channels] of outputs, then the channels' factors
+    int group, quad, lane;
+
+    // piece j of row r, so that neither writing a piece of every row nor reading whole rows meets a bank twice
+    __device__ __forceinline__ uint8_t *at(int r, int j) const { return own + (r * SEGS + (j ^ (SEGS == 8 ? r & 7 : (r >> 1) & 3))) * 16; }
+    __device__ __forceinline__ float *factors() const { return reinterpret_cast<float *>(own + 32 * 32 * sizeof(YT)); }
+
+    // scale and bias of this warp's channels: asked for before the sums are waited for
+    __device__ __forceinline__ void begin(const Operands &ops, int n0, int N) const {
+        float4 f;
+        const int n = n0 + group * 32 + lane, n2 = GATED ? n : n + 128;
+        const float *scales2 = GATED ? ops.scales2 : ops.scales, *bias2 = GATED ? ops.bias2 : ops.bias;
+        f.x = n < N ? ops.scales[n] : 0.0f, f.y = n < N && ops.bias ? ops.bias[n] : 0.0f;
+        f.z = n2 < N ? scales2[n2] : 0.0f, f.w = n2 < N && bias2 ? bias2[n2] : 0.0f;
+        __syncwarp();  // the tile before has read its factors
+        if constexpr (GATED) reinterpret_cast<float4 *>(factors())[lane] = f;
+        else {
+            reinterpret_cast<float2 *>(factors())[lane] = float2{f.x, f.y};
+            reinterpret_cast<float2 *>(factors())[32 + lane] = float2{f.z, f.w};
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void load(uint32_t tmem_d, int step, uint32_t (&lo)[16], uint32_t (&hi)[16]) const {
+        const uint32_t at0 = tmem_d + ((uint32_t)(quad * 32) << 16) + (GATED ? group * 32 + step * 16 : step * 128 + group * 32);
+        tc_ld16(at0, lo);
+        tc_ld16(at0 + (GATED ? 128 : 16), hi);
         tc_wait_ld();
+    }
+    __device__ __forceinline__ void pack(int first_piece, const float (&v)[16]) const {
+#pragma unroll
+        for (int j = 0; j < 16 / EPV; ++j) {
+            union { uint4 q; YT e[EPV]; } o;
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) o.e[e] = to_out<YT>(v[j * EPV + e]);
+            *reinterpret_cast<uint4 *>(at(lane, first_piece + j)) = o.q;
+        }
+    }
+    __device__ __forceinline__ void compute(int step, const uint32_t (&lo)[16], const uint32_t (&hi)[16], bool relu) const {
+        float v[16];
         if constexpr (GATED) {
-            // the up lane finishes the second half of the tokens, the gate lane the first
-            float v[CW];
 #pragma unroll
-            for (int i = 0; i < CW; ++i) v[i] = __uint_as_float(raw[i]) * sc + bs;
-            const int keep0 = is_up ? CW / 2 : 0;
-#pragma unroll
-            for (int i = 0; i < CW / 2; ++i) {
-                const float other = __shfl_xor_sync(0xFFFFFFFFu, is_up ? v[i] : v[CW / 2 + i], 1), mine = is_up ? v[CW / 2 + i] : v[i];
-                out_st[(keep0 + i) * CH + ch] = to_out<YT>(silu_f(is_up ? other : mine) * (is_up ? mine : other));
+            for (int i = 0; i < 16; ++i) {
+                const float4 f = reinterpret_cast<const float4 *>(factors())[step * 16 + i];
+                v[i] = pair_silu(__uint_as_float(lo[i]) * f.x + f.y, __uint_as_float(hi[i]) * f.z + f.w);
             }
+            pack(step * (16 / EPV), v);
         } else {
-            const bool relu = epilogue == SHREWQ_EPILOGUE_RELU;
 #pragma unroll
-            for (int i = 0; i < CW; ++i) {
-                const float v = __uint_as_float(raw[i]) * sc + bs;
-                out_st[i * CH + ch] = to_out<YT>(relu ? fmaxf(v, 0.0f) : v);
-            }
-        }
-        if (c + kFp4Groups < kPairTok / CW) tc_ld16(taddr + (c + kFp4Groups) * CW, raw);
-        else {  // everything has been read: the next tile's MMAs may write
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_free_leader);
-        }
-        named_bar_sync(2 + group, 128);  // the staging tile is complete
-        if (!ok) continue;
-        const int mc = m0 + c * CW;
-        if (vec_ok) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int p = row; p < PIECES; p += 128) {
-                const int tr = p / PPR, seg = p % PPR, m = mc + tr, nn = n0 + seg * EPV;
-                if (m >= M || nn >= N) continue;
-                YT *dst = y + (size_t)m * ldy + nn;
-                if (nn + EPV <= N) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(stage + tr * RB + seg * 16);
-                else
-                    for (int e = 0; e < EPV && nn + e < N; ++e) dst[e] = out_st[tr * CH + seg * EPV + e];
-            }
-        } else {
-#pragma unroll 4
-            for (int e = row; e < CW * CH; e += 128) {
-                const int tr = e / CH, m = mc + tr, nn = n0 + e % CH;
-                if (m < M && nn < N) y[(size_t)m * ldy + nn] = out_st[e];
+                for (int i = 0; i < 16; i += 2) {  // two channels' factors at a time
+                    const float4 f = reinterpret_cast<const float4 *>(factors())[step * 16 + h * 8 + i / 2];
+                    v[i] = __uint_as_float(h ? hi[i] : lo[i]) * f.x + f.y;
+                    v[i + 1] = __uint_as_float(h ? hi[i + 1] : lo[i + 1]) * f.z + f.w;
+                }
+                if (relu) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = fmaxf(v[i], 0.0f);
+                }
+                pack(h * (16 / EPV), v);
             }
         }
     }
-}
+    __device__ __forceinline__ void store(YT *__restrict__ y, int M, int N, size_t ldy, int n, int m0, bool vec_ok) const {
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < SEGS; ++p) {
+            const int r = p * (32 / SEGS) + lane / SEGS, j = lane % SEGS, m = m0 + quad * 32 + r, nn = n + j * EPV;
+            if (m >= M || nn >= N) continue;
+            YT *dst = y + (size_t)m * ldy + nn;
+            union { uint4 q; YT e[EPV]; } o;
+            o.q = *reinterpret_cast<const uint4 *>(at(r, j));
+            if (vec_ok && nn + EPV <= N) *reinterpret_cast<uint4 *>(dst) = o.q;
+            else {
+#pragma unroll
+                for (int e = 0; e < EPV; ++e)
+                    if (nn + e < N) dst[e] = o.e[e];
+            }
+        }
+        __syncwarp();
+    }
+};
 
 // Grid: pairs * 2 CTAs; pair p takes the tiles p, p + pairs, ..., token tiles fastest.
 template <bool NV, bool GATED, typename YT>
@@ -126,17 +160,18 @@ gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restr
     const int pair = (int)(blockIdx.x >> 1), m_tiles = (M + kPairTok - 1) / kPairTok;
     const int rounds = (K + kFp4StageK - 1) / kFp4StageK;
     const size_t pieces = (size_t)rounds * C::kPieces;
-    constexpr uint32_t kFullBar = 0, kEmptyBar = C::kStages * 8, kAccFullBar = 2 * C::kStages * 8, kAccFreeBar = kAccFullBar + 8;
+    constexpr uint32_t kFullBar = 0, kEmptyBar = C::kStages * 8, kAccFullBar = 2 * C::kStages * 8, kAccFreeBar = kAccFullBar + 8, kReadyBar = kAccFreeBar + 8;
     const uint32_t bars = smem_u32(smem + C::kBarOff), smem_base = smem_u32(smem);
 
     if (threadIdx.x == 0) {
         ctl->abort_flag = 0;
         for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(bars + kFullBar + s * 8, 128 + (rank == 0 ? 1 : 0));  // a group's copies; in the leader also the relay
+            mbar_init(bars + kFullBar + s * 8, 128);  // a group's copies
+            mbar_init(bars + kReadyBar + s * 8, 2);   // the relays (the leader's are used)
             mbar_init(bars + kEmptyBar + s * 8, 1);
         }
         mbar_init(bars + kAccFullBar, 1);
-        mbar_init(bars + kAccFreeBar, 2 * 4 * kFp4Groups);  // (the leader's is used)
+        mbar_init(bars + kAccFreeBar, 2 * 4 * kPairGroups);  // (the leader's is used)
         mbar_fence_init();
     }
     if (warp == 0) {
@@ -152,33 +187,20 @@ gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restr
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, ctl->tmem_base, 0);  // (uniform to the compiler)
 
     if (warp == 0) {
-        if (rank == 1 && elect_one()) {
-            const uint32_t full_leader = map_to_cta(bars + kFullBar, 0);
-            uint32_t s = 0, ph = 0;
-            bool good = true;
-            pdl_wait();
-            for (int tile = pair; good && tile < tiles; tile += pairs)
-                for (int i = 0; i < rounds; ++i) {
-                    good = mbar_wait_close<kTimeoutFp4Pair>(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
-                    if (!good) break;
-                    fence_proxy_async_smem();
-                    mbar_arrive_cluster(full_leader + s * 8);
-                    if (++s == C::kStages) { s = 0; ph ^= 1; }
-                }
-        }
         if (rank == 0 && elect_one()) {
             pdl_wait();  // a stage is full only with its activations: the time limit of the waits starts when they exist
             uint32_t s = 0, ph = 0, done = 0;
-            bool good = true;
+            bool good = true, ready = false;
             for (int tile = pair; good && tile < tiles; tile += pairs, ++done) {
                 if (done > 0 && !mbar_wait_close<kTimeoutFp4Pair>(bars + kAccFreeBar, (done - 1) & 1u, ctl, status, 3, 0)) break;
-                tc_fence_after();
                 for (int i = 0; i < rounds; ++i) {
-                    good = mbar_wait_close<kTimeoutFp4Pair>(bars + kFullBar + s * 8, ph, ctl, status, 1, s);
+                    good = ready || mbar_wait_close<kTimeoutFp4Pair>(bars + kReadyBar + s * 8, ph, ctl, status, 1, s);
                     if (!good) break;
-                    fence_proxy_async_smem();
                     tc_fence_after();
-                    const uint32_t base = smem_base + s * C::kStageBytes, sf = tmem + C::kAccCols + s * C::kSfCols;
+                    // (a look takes 150 to 300 cycles here: the next stage's is under way while this one's MMAs are issued)
+                    const uint32_t next = s + 1 == C::kStages ? 0 : s + 1, next_ph = s + 1 == C::kStages ? ph ^ 1u : ph;
+                    ready = mbar_test(bars + kReadyBar + next * 8, next_ph);
+                    const uint32_t base = smem_base + s * C::kStageBytes, sf = tmem + kPairTok + s * C::kSfCols;
                     constexpr int kSfbCol = C::kPieces * 4;
                     const uint64_t adesc = make_b_desc(base), bdesc = make_b_desc(base + C::kBOff), sdesc = make_scale_desc(base + C::kSfaOff);
 #pragma unroll
@@ -195,102 +217,129 @@ gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restr
                         }
                     }
                     tc_commit_pair(bars + kEmptyBar + s * 8);
-                    if (++s == C::kStages) { s = 0; ph ^= 1; }
+                    s = next, ph = next_ph;
                 }
                 if (good) tc_commit_pair(bars + kAccFullBar);
             }
         }
         __syncwarp();
-    } else if (warp <= 4 * kFp4Groups) {
-        // ---------------- epilogue ----------------
+    } else if (warp == kPairThreads / 32 - 1) {
+        // ---------------- relay: copies that have landed -> visible to the tensor core -> the leader ----------------
+        if (elect_one()) {
+            const uint32_t ready_leader = map_to_cta(bars + kReadyBar, 0);
+            uint32_t s = 0, ph = 0;
+            bool good = true;
+            pdl_wait();
+            for (int tile = pair; good && tile < tiles; tile += pairs)
+                for (int i = 0; i < rounds; ++i) {
+                    good = mbar_wait_close<kTimeoutFp4Pair>(bars + kFullBar + s * 8, ph, ctl, status, 5, s);
+                    if (!good) break;
+                    fence_proxy_async_smem();
+                    mbar_arrive_cluster(ready_leader + s * 8);
+                    if (++s == C::kStages) { s = 0; ph ^= 1; }
+                }
+        }
+        __syncwarp();
+    } else {
         const int group = (warp - 1) >> 2, quad = warp & 3;
         const uint32_t acc_free_leader = map_to_cta(bars + kAccFreeBar, 0);
         const bool vec_ok = ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * sizeof(YT))) & 15) == 0;
-        uint32_t step = 0, done = 0;
-        pdl_wait();  // y may be in use by the previous kernel of the stream
-        for (int tile = pair; tile < tiles; tile += pairs, ++done) {
-            mbar_wait_all<kTimeoutFp4Pair>(bars + kAccFullBar, done & 1u, ctl, status, 4, 0);
+        uint32_t done = 0;
+        const PairEpilogue<GATED, YT> epi{smem + C::kOutOff + (warp - 1) * C::kOutBytes, group, quad, lane};
+        const bool relu = epilogue == SHREWQ_EPILOGUE_RELU;
+        auto finish = [&](int tile) {
+            const int n0 = tile / m_tiles * C::kChannels, m0 = tile % m_tiles * kPairTok + (int)rank * kPairHalf;
+            epi.begin(ops, n0, N);
+            mbar_wait_lane<kTimeoutFp4Pair, 40>(bars + kAccFullBar, done & 1u, ctl, status, 4, 0);
+            ++done;
             const bool ok = warp_ok(ctl);
             tc_fence_after();
-            pair_epilogue<GATED, YT>(tmem, smem + C::kOutOff, step, acc_free_leader, group, quad, lane, ok, ops, y, M, N, ldy, epilogue,
-                                     (tile / m_tiles * 2 + (int)rank) * C::kChannels, tile % m_tiles * kPairTok, vec_ok);
-        }
-    } else {
+            uint32_t lo[16], hi[16];
+            epi.load(tmem, 0, lo, hi);
+            epi.compute(0, lo, hi, relu);
+            epi.load(tmem, 1, lo, hi);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_free_leader);  // everything has been read: the next tile's MMAs may write
+            if (!GATED && ok) epi.store(y, M, N, ldy, n0 + group * 32, m0, vec_ok);
+            epi.compute(1, lo, hi, relu);
+            if (ok) epi.store(y, M, N, ldy, n0 + group * 32 + (GATED ? 0 : 128), m0, vec_ok);
+        };
+        if (group >= 2) {
+            pdl_wait();  // y may be in use by the previous kernel of the stream
+            for (int tile = pair; tile < tiles; tile += pairs) finish(tile);
+        } else {
         // ---------------- copies: 16 bytes a lane, swizzled as they land ----------------
-        constexpr int kInstr = 8;  // 4 rows each, of a warp: 32 rows of A, 32 of B
-        const int copier = warp - 1 - 4 * kFp4Groups, cgroup = copier >> 2, cw = copier & 3, t = cw * 32 + lane;
-        const size_t pitch = (size_t)((K + 31) >> 5) * 16;
-        const int seg = (lane & 7) * 16, last_tile = (M - 1) >> 7;
-        const uint8_t *wsrc[kInstr], *xsrc[kInstr], *sfa_src[C::kPieces], *sfb_src[2 * C::kPieces / 4];
-        uint32_t at[kInstr];
-#pragma unroll
-        for (int j = 0; j < kInstr; ++j) {
-            const int r = (cw * kInstr + j) * 4 + (lane >> 3);
-            at[j] = (uint32_t)(r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-        }
-        auto begin = [&](int tile) {
-            const int n0 = (tile / m_tiles * 2 + (int)rank) * C::kChannels, m0 = tile % m_tiles * kPairTok;
+        constexpr int kInstr = 8;  // of a warp, 4 rows each: 32 rows of each operand
+        const int cw = (warp - 1) & 3, t = cw * 32 + lane;
+        const uint32_t pitch = (uint32_t)((K + 31) >> 5) * 16;
+        const uint32_t seg = (lane & 7) * 16, last_m = (M - 1) >> 7, last_n = (N - 1) >> 7;
+        const uint8_t *wrows = GATED && rank ? w2_codes : w_codes, *wtile, *xtile, *sfw_src[C::kPieces / 2], *sfx_src;
+        int w_last = 0, x_last = 0;  // last rows of the tile that there are
+        // 16 bytes a lane of 4 rows at a time; the swizzle is by the row modulo 8; codes past the end of a row: zeros
+        auto rows = [&](uint32_t dst, const uint8_t *tile, int last, uint32_t byte) {
+            const bool in = byte + seg < pitch;
+            const uint8_t *src = tile + (in ? byte : 0);
+            const int r0 = cw * kInstr * 4 + (lane >> 3);
 #pragma unroll
             for (int j = 0; j < kInstr; ++j) {
-                const int r = (cw * kInstr + j) * 4 + (lane >> 3);
-                const int n = n0 + (GATED ? r >> 1 : r), m = m0 + (int)rank * kPairHalf + r;
-                wsrc[j] = (GATED && (r & 1) ? w2_codes : w_codes) + (size_t)(n < N ? n : N - 1) * pitch + seg;
-                xsrc[j] = x_codes + (size_t)(m < M ? m : M - 1) * pitch + seg;
+                const int r = r0 + j * 4;
+                copy_async_16(dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src + (size_t)(uint32_t)(r < last ? r : last) * pitch, in);
             }
-            if constexpr (GATED) {  // four bytes (a row's scales) at a time: gate and up rows are interleaved
-                const int r = (t & 3) * 32 + (t >> 2), n = n0 + (r >> 1) < N ? n0 + (r >> 1) : N - 1;
+        };
+        // (rows past the last one are read from it again: nothing of them is stored)
+        auto begin = [&](int tile) {
+            const int n0 = tile / m_tiles * C::kChannels, m0 = tile % m_tiles * kPairTok + (int)rank * kPairHalf;
+            const int nr = n0 + (GATED ? 0 : (int)rank * 128), nb = nr < N ? nr : N - 1, mb = m0 < M ? m0 : M - 1;
+            wtile = wrows + (size_t)nb * pitch + seg, w_last = N - 1 - nb;
+            xtile = x_codes + (size_t)mb * pitch + seg, x_last = M - 1 - mb;
 #pragma unroll
-                for (int p = 0; p < C::kPieces; ++p)
-                    sfa_src[p] = (r & 1 ? w2_pieces : w_pieces) + ((size_t)(n >> 7) * pieces + p) * 512 + (n & 31) * 16 + ((n & 127) >> 5) * 4;
-            } else {
-                const int wt = (n0 < N ? n0 : N - 1) >> 7;  // (rows past the end: any scales)
-                sfa_src[0] = w_pieces + (size_t)wt * pieces * 512 + t * 16;
+            for (int j = 0; j < C::kPieces / 2; ++j) {
+                const int c = j * 128 + t, half = c / (C::kPieces * 32), nt = (n0 >> 7) + (GATED ? 0 : half);
+                sfw_src[j] = (GATED && half ? w2_pieces : w_pieces) + (size_t)(nt < last_n ? nt : last_n) * pieces * 512 + (c % (C::kPieces * 32)) * 16;
             }
-#pragma unroll
-            for (int j = 0; j < 2 * C::kPieces / 4; ++j) {
-                const int c = j * 128 + t, half = c / (C::kPieces * 32), xt = (m0 >> 7) + half < last_tile ? (m0 >> 7) + half : last_tile;
-                sfb_src[j] = x_pieces + (size_t)xt * pieces * 512 + (c % (C::kPieces * 32)) * 16;
-            }
+            sfx_src = x_pieces + (size_t)((m0 >> 7) < last_m ? m0 >> 7 : last_m) * pieces * 512 + t * 16;
         };
         auto copy_w = [&](int i, int s) {
             const uint32_t dst = smem_base + s * C::kStageBytes;
-            const size_t byte = (size_t)i * kFp4RowBytes, sf = (size_t)i * C::kPieces * 512;
-            const bool in = byte + seg < pitch;  // (codes past the end of a row: zeros)
+            const size_t sf = (size_t)i * C::kPieces * 512;
+            rows(dst + C::kBOff, wtile, w_last, (uint32_t)i * kFp4RowBytes);
 #pragma unroll
-            for (int j = 0; j < kInstr; ++j) copy_async_16(dst + at[j], in ? wsrc[j] + byte : wsrc[j], in);
-            if constexpr (GATED) {
-#pragma unroll
-                for (int p = 0; p < C::kPieces; ++p) copy_async_4(dst + C::kSfaOff + p * 512 + t * 4, sfa_src[p] + sf, true);
-            } else {
-                if (t < C::kSfaBytes / 16) copy_async_16(dst + C::kSfaOff + t * 16, sfa_src[0] + sf, true);
-            }
+            for (int j = 0; j < C::kPieces / 2; ++j) copy_async_16(dst + C::kSfbOff + (j * 128 + t) * 16, sfw_src[j] + sf, true);
         };
         auto copy_x = [&](int i, int s) {
             const uint32_t dst = smem_base + s * C::kStageBytes;
-            const size_t byte = (size_t)i * kFp4RowBytes, sf = (size_t)i * C::kPieces * 512;
-            const bool in = byte + seg < pitch;
-#pragma unroll
-            for (int j = 0; j < kInstr; ++j) copy_async_16(dst + C::kBOff + at[j], in ? xsrc[j] + byte : xsrc[j], in);
-#pragma unroll
-            for (int j = 0; j < 2 * C::kPieces / 4; ++j) copy_async_16(dst + C::kSfbOff + (j * 128 + t) * 16, sfb_src[j] + sf, true);
+            const size_t sf = (size_t)i * C::kPieces * 512;
+            rows(dst, xtile, x_last, (uint32_t)i * kFp4RowBytes);
+            if (t < C::kSfaBytes / 16) copy_async_16(dst + C::kSfaOff + t * 16, sfx_src + sf, true);
         };
         begin(pair);
         const int pre = rounds < C::kStages ? rounds : C::kStages;
-        for (int i = cgroup; i < pre; i += 2) copy_w(i, i);
+        for (int i = group; i < pre; i += 2) copy_w(i, i);
         pdl_wait();
         int it = 0;  // stages so far, of both groups
         uint32_t s = 0, ph = 0;
-        for (int tile = pair; tile < tiles; tile += pairs) {
-            if (it > 0) begin(tile);
-            for (int i = 0; i < rounds; ++i, ++it) {
-                if ((it & 1) == cgroup) {
-                    if (it >= C::kStages) mbar_wait_all<kTimeoutFp4Pair>(bars + kEmptyBar + s * 8, ph ^ 1u, ctl, status, 0, s);
+        auto bring = [&](int first, int last) {
+            for (int i = first; i < last; ++i, ++it) {
+                if ((it & 1) == group) {
+                    if (it >= C::kStages) mbar_wait_lane<kTimeoutFp4Pair, 0>(bars + kEmptyBar + s * 8, ph ^ 1u, ctl, status, 0, s);
                     if (it >= pre) copy_w(i, s);
                     copy_x(i, s);
                     copy_async_arrive(bars + kFullBar + s * 8);
                 }
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
             }
+        };
+        // the next tile's first stages are requested before this tile is finished
+        bring(0, pre);
+        for (int tile = pair; tile < tiles; tile += pairs) {
+            bring(pre, rounds);
+            if (tile + pairs < tiles) {
+                begin(tile + pairs);
+                bring(0, pre);
+            }
+            finish(tile);
+        }
         }
     }
 

@@ -100,6 +100,17 @@ __device__ __forceinline__ void copy_async_16(uint32_t dst, const void *src, boo
 __device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
+// 2^x and 1/x, good to a few ulp; results below 2^-126 are 0
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float recip_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // this thread arrives on the barrier (of a count that includes it) when all of its copies so far have landed
 __device__ __forceinline__ void copy_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -39,6 +39,20 @@ __device__ __forceinline__ void mbar_wait_all(uint32_t bar, uint32_t parity, Ctl
     mbar_wait_close<CODE>(bar, parity, ctl, st, role, stage);
     __syncwarp();
 }
+// A whole warp beside others that must not be disturbed: one lane looks, PAUSE nanoseconds apart.  A look by 32 lanes keeps the SM's
+// shared-memory path busy for some 32 cycles, and 16 warps that look back to back slow every other access to it.
+template <uint32_t CODE, uint32_t PAUSE>
+__device__ __forceinline__ void mbar_wait_lane(uint32_t bar, uint32_t parity, Ctl *ctl, DeviceStatus *st, uint32_t role, uint32_t stage) {
+    if ((threadIdx.x & 31) == 0) {
+        bool done = mbar_test(bar, parity);
+        for (uint32_t i = 0; i < kSpinClose && !done; ++i) {
+            if (PAUSE) __nanosleep(PAUSE);
+            done = mbar_test(bar, parity);
+        }
+        if (!done) mbar_wait_slow(bar, parity, ctl, st, role, stage, CODE);
+    }
+    __syncwarp();
+}
 __device__ __forceinline__ bool warp_ok(Ctl *ctl) { return __all_sync(0xFFFFFFFFu, ctl->abort_flag == 0) != 0; }
 
 enum { kEpiPlain = 0, kEpiLanesPaired = 1, kEpiColumns = 2 };

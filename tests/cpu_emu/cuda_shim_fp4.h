@@ -101,6 +101,8 @@ static inline void copy_async_wait() {
     }
     v.resize(kept);
 }
+static inline float exp2_approx(float x) { return exp2f(x); }
+static inline float recip_approx(float x) { return 1.0f / x; }
 static inline void mbar_arrive(uint32_t bar);
 static inline void copy_async_arrive(uint32_t bar) {
     for (auto &c : emu::g_copies) memcpy(c.dst, c.data, c.bytes);

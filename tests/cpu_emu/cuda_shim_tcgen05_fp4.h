@@ -28,7 +28,7 @@ inline void cp_scales(Block *blk, uint32_t taddr, uint64_t desc) {
 // rows 128 r .. of A, its scales and D in block r of the pair (or the one block), rows 128 r .. of B there too, B's scales in every block
 inline void mma_fp4_pair(Block *leader, bool nv, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     const uint32_t N = ((idesc >> 17) & 0x3Fu) << 3, M = ((idesc >> 24) & 0x1Fu) << 4, sa = (idesc >> 29) & 3u, sb = (idesc >> 4) & 3u;
-    EMU_CHECK(leader->rank == 0 && M == 256 && N == 256 && ((idesc >> 7) & 7u) == 1 && ((idesc >> 10) & 7u) == 1, "E2M1 operands, 256 x 256, issued by the leader");
+    EMU_CHECK(leader->rank == 0 && M == 256 && N % 32 == 0 && N <= 256 && ((idesc >> 7) & 7u) == 1 && ((idesc >> 10) & 7u) == 1, "E2M1 operands, 256 rows, issued by the leader");
     EMU_CHECK(((idesc >> 23) & 1u) == (nv ? 0u : 1u) && (nv ? sa == 0 && sb == 0 : (sa & 1) == 0 && (sb & 1) == 0), "scale type and ids");
     const uint32_t dcol = d_tmem & 0xFFFF, ca = sfa & 0xFFFF, cb = sfb & 0xFFFF, per = nv ? 16 : 32;
     if (dcol + N > 512 || ca + 4 > 512 || cb + 8 > 512) { fail("block-scaled MMA outside tensor memory"); return; }
@@ -41,7 +41,7 @@ inline void mma_fp4_pair(Block *leader, bool nv, uint32_t d_tmem, uint64_t a_des
         for (uint32_t i = 0; i < 128; ++i)
             for (uint32_t k = 0; k < 64; ++k) a[i * 64 + k] = fp4_operand(blk, a_desc, i, k) * scale(ca, i, k / per, sa);
         for (uint32_t i = 0; i < N; ++i)
-            for (uint32_t k = 0; k < 64; ++k) b[i * 64 + k] = fp4_operand(leader->cluster[i >> 7], b_desc, i & 127, k) * scale(cb, i, k / per, sb);
+            for (uint32_t k = 0; k < 64; ++k) b[i * 64 + k] = fp4_operand(leader->cluster[i / (N / 2)], b_desc, i % (N / 2), k) * scale(cb, i, k / per, sb);
         for (uint32_t m = 0; m < 128; ++m)
             for (uint32_t n = 0; n < N; ++n) {
                 double acc = accumulate ? (double)__uint_as_float(blk->tmem[m * 512 + dcol + n]) : 0.0;

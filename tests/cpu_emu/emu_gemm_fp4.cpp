@@ -56,7 +56,7 @@ int run(const uint8_t *const *codes, const uint8_t *const *scales, const float *
     const Operands ops{alpha[0].data(), bias[0], alpha[GATED ? 1 : 0].data(), bias[GATED ? 1 : 0]};
     DeviceStatus status{0, 0, 0, 0};
     if (split == 2) {  // CTA pairs
-        const int per = GATED ? 128 : 256, tiles = (N + per - 1) / per * ((M + 255) / 256), pairs = tiles < 2 ? tiles : 2;
+        const int per = GATED ? 128 : 256, tiles = (N + per - 1) / per * ((M + kPairTok - 1) / kPairTok), pairs = tiles < 2 ? tiles : 2;
         emu::launch_cluster2((unsigned)(2 * pairs), 1, 1, kPairThreads, Fp4PairCfg<NV, GATED, float>::kSmemBytes, [&] {
             gemm_fp4_pair_kernel<NV, GATED, float>(codes[0], codes[GATED ? 1 : 0], xc, wp[0], wp[GATED ? 1 : 0], xp, ops, y, M, N, K, ldy, epilogue, tiles, pairs, &status);
         });
