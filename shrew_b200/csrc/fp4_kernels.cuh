@@ -79,6 +79,19 @@ __device__ __forceinline__ float fp4_tensor_scale(float amax) {
     return __uint_as_float(e << 23);
 }
 
+// a / 6 and 1 / s, rounded to nearest as the IEEE operations round them: an approximation and one step with its exact remainder (Markstein
+// 1990: right for every a whose quotient is a normal number, and smaller ones end at the least scale; s runs through the 126 values that a
+// scale can have, all of them checked against the division).  They cost 3 instructions each, without the branch for special operands that the
+// general operations carry.
+__device__ __forceinline__ float div6_rn(float a) {
+    const float r = 0.166666672f, q = a * r;  // r = 1/6 rounded to nearest
+    return __fmaf_rn(__fmaf_rn(-6.0f, q, a), r, q);
+}
+__device__ __forceinline__ float recip_e4m3_rn(float s) {
+    const float r = recip_approx(s);
+    return __fmaf_rn(__fmaf_rn(-s, r, 1.0f), r, r);
+}
+
 // One thread's part of a block: v[8] -> a word of codes and the block's scale byte (the same in all lanes of the block).  Every lane of
 // the warp takes part in the shuffles.
 template <bool NV>
@@ -94,10 +107,10 @@ __device__ __forceinline__ uint32_t fp4_encode(float *v, float inv_g, uint32_t &
     if constexpr (!NV) amax = max_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
     const bool bad = !(amax < __uint_as_float(0x7F800000u));
     if constexpr (NV) {
-        byte = amax == 0.0f ? kE4m3One : cvt_e4m3(fminf(fmaxf(__fdiv_rn(amax, 6.0f), 0.001953125f), 448.0f));
+        byte = amax == 0.0f ? kE4m3One : cvt_e4m3(fminf(fmaxf(div6_rn(amax), 0.001953125f), 448.0f));
         float s, unused;
         f32x2_of_f16x2(cvt_f16x2_e4m3(byte), s, unused);
-        const float r = __frcp_rn(s);
+        const float r = recip_e4m3_rn(s);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float q = v[i] * r;
@@ -231,7 +244,9 @@ __device__ __forceinline__ size_t scale_piece_offset(size_t row, size_t block, s
 
 // ---- quantize: any rows (strides, widths, alignments), and the activations of a 4-bit product ---------------------------------
 // A CTA a row at a time; PIECES: the scales go to the order of scale_piece_offset, out to `blocks_out` blocks a row (scale 1 beyond
-// the row's end).  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.
+// the row's end).  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.  The loads of four groups a thread are under way together: one
+// at a time left 4096 x 11008 bf16 at 30 us, and a byte at a time the scales.
+constexpr int kRowsUnroll = 4;
 template <typename T, bool NV, bool PIECES>
 __global__ void __launch_bounds__(kFp4Threads)
 fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size_t ld, int vec_ok, const float *g_in, const float *partials,
@@ -245,17 +260,30 @@ fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size
     const size_t groups = blocks_out << kShift;         // >= words
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *src = x + row * ld;
-        for (size_t i0 = 0; i0 < groups; i0 += blockDim.x) {  // (uniform: the shuffles need whole warps)
-            const size_t i = i0 + threadIdx.x;
-            float v[8];
-            if (vec_ok && i * 8 + 8 <= cols) load_vec8<T>(src + i * 8, v);
-            else load_guarded8<T>(src + i * 8, i * 8 < cols ? cols - i * 8 : 0, v);
-            uint32_t byte;
-            const uint32_t word = fp4_encode<NV>(v, inv_g, byte);
-            if (i < words) codes[row * words + i] = word;
-            if (i < groups && (i & ((1 << kShift) - 1)) == 0) {
-                const size_t b = i >> kShift;
-                scales[PIECES ? scale_piece_offset(row, b, blocks_out >> 2) : row * blocks_out + b] = (uint8_t)byte;
+        for (size_t i0 = 0; i0 < groups; i0 += kRowsUnroll * blockDim.x) {  // (uniform: the shuffles need whole warps)
+            float v[kRowsUnroll][8];
+#pragma unroll
+            for (int u = 0; u < kRowsUnroll; ++u) {
+                if (i0 + u * blockDim.x >= groups) continue;
+                const size_t i = i0 + u * blockDim.x + threadIdx.x;
+                if (vec_ok && i * 8 + 8 <= cols) load_vec8<T>(src + i * 8, v[u]);
+                else load_guarded8<T>(src + i * 8, i * 8 < cols ? cols - i * 8 : 0, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kRowsUnroll; ++u) {
+                if (i0 + u * blockDim.x >= groups) continue;
+                const size_t i = i0 + u * blockDim.x + threadIdx.x;
+                uint32_t byte;
+                const uint32_t word = fp4_encode<NV>(v[u], inv_g, byte);
+                if (i < words) codes[row * words + i] = word;
+                if constexpr (PIECES) {  // four blocks of a row are one word there, and `blocks_out` is a multiple of 4
+                    uint32_t four = byte | __shfl_xor_sync(0xFFFFFFFFu, byte, 1 << kShift) << 8;
+                    four |= __shfl_xor_sync(0xFFFFFFFFu, four, 2 << kShift) << 16;
+                    if (i < groups && (i & ((4 << kShift) - 1)) == 0)
+                        *reinterpret_cast<uint32_t *>(scales + scale_piece_offset(row, i >> kShift, blocks_out >> 2)) = four;
+                } else {
+                    if (i < groups && (i & ((1 << kShift) - 1)) == 0) scales[row * blocks_out + (i >> kShift)] = (uint8_t)byte;
+                }
             }
         }
     }
