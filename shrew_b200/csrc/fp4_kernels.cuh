@@ -98,7 +98,7 @@ template <bool NV>
 __device__ __forceinline__ uint32_t fp4_encode(float *v, float inv_g, uint32_t &byte) {
     if constexpr (NV) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inv_g;
+        for (int i = 0; i < 8; i += 2) mul_f32x2(v[i], v[i + 1], inv_g, v[i], v[i + 1]);
     }
     float amax = max_abs_nan(v[0], v[1]);
 #pragma unroll
@@ -112,9 +112,11 @@ __device__ __forceinline__ uint32_t fp4_encode(float *v, float inv_g, uint32_t &
         f32x2_of_f16x2(cvt_f16x2_e4m3(byte), s, unused);
         const float r = recip_e4m3_rn(s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q = v[i] * r;
-            v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
+        for (int i = 0; i < 8; i += 2) {
+            float q0, q1, e0, e1;
+            mul_f32x2(v[i], v[i + 1], r, q0, q1);
+            fma_f32x2(q0, q1, -s, v[i], v[i + 1], e0, e1);
+            fma_f32x2(e0, e1, r, q0, q1, v[i], v[i + 1]);
         }
         if (bad) byte = kE4m3Nan;
     } else {
@@ -152,21 +154,25 @@ fp4_amax_kernel(const T *__restrict__ x, size_t rows, size_t cols, size_t ld, fl
     const size_t step = (size_t)gridDim.x * kFp4Threads;
     size_t i = (size_t)blockIdx.x * kFp4Threads + threadIdx.x;
     if constexpr (FLAT) {
-        for (; i + 3 * step < total; i += 4 * step) {  // four loads in flight
-            float v[4][8];
+        constexpr int U = sizeof(T) == 2 ? 8 : 4;  // 128 bytes a thread under way, the end of the tensor included
+        for (; i < total; i += U * step) {
+            float v[U][8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) load_vec8<T>(x + (i + u * step) * 8, v[u]);
+            for (int u = 0; u < U; ++u) {
+                if (i + u * step < total) load_vec8<T>(x + (i + u * step) * 8, v[u]);
+                else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) take(v[u]);
+                    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) take(v[u]);
         }
     }
-    for (; i < total; i += step) {
+    for (; !FLAT && i < total; i += step) {
         float v[8];
-        if constexpr (FLAT) load_vec8<T>(x + i * 8, v);
-        else {
-            const size_t row = i / per_row, c = (i % per_row) * 8;
-            load_guarded8<T>(x + row * ld + c, cols - c, v);
-        }
+        const size_t row = i / per_row, c = (i % per_row) * 8;
+        load_guarded8<T>(x + row * ld + c, cols - c, v);
         take(v);
     }
     __shared__ float s_max[kFp4Threads / 32];
@@ -198,7 +204,8 @@ __device__ __forceinline__ float fp4_block_tensor_scale(const float *g_in, const
 }
 
 // ---- quantize: rows that are whole aligned 32s, one after the other: a flat stream of groups of 8 ------------------------------
-// U groups a thread, requested before the first is used.  The blocks go through the tensor from its end where a pass before this one
+// U groups a thread, requested before the first is used (and before the tensor's scale is made from the partial maxima: that costs a block
+// some 2000 cycles, so where there are partial maxima the grid is no more than what is resident).  The chunks go through the tensor from its end where a pass before this one
 // has read it from the front (BACK): what that pass left in L2 is read first.
 template <typename T, bool NV, int U>
 __global__ void __launch_bounds__(kFp4Threads)
@@ -206,33 +213,42 @@ fp4_quantize_flat_kernel(const T *__restrict__ x, size_t groups, const float *g_
                          uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
-    float inv_g = 1.0f;
-    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_block_tensor_scale(g_in, partials, n_partials, g_out, kFp4Threads));
-    const size_t block = partials ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-    const size_t base = block * (size_t)(kFp4Threads * U) + threadIdx.x;
+    const size_t chunks = (groups + kFp4Threads * U - 1) / (kFp4Threads * U);
     float v[U][8];
+    auto load = [&](size_t base) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const size_t i = base + (size_t)u * kFp4Threads;
-        if (i < groups) load_vec8<T>(x + i * 8, v[u]);
-        else {
+        for (int u = 0; u < U; ++u) {
+            const size_t i = base + (size_t)u * kFp4Threads;
+            if (i < groups) load_vec8<T>(x + i * 8, v[u]);
+            else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const size_t i = base + (size_t)u * kFp4Threads;
-        uint32_t byte;
-        const uint32_t word = fp4_encode<NV>(v[u], inv_g, byte);
-        if (i < groups) {
-            codes[i] = word;
-            if constexpr (NV) {
-                if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
-            } else {
-                if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+                for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
             }
         }
+    };
+    auto base_of = [&](size_t chunk) { return (partials ? chunks - 1 - chunk : chunk) * (size_t)(kFp4Threads * U) + threadIdx.x; };
+    load(base_of(blockIdx.x));
+    float inv_g = 1.0f;
+    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_block_tensor_scale(g_in, partials, n_partials, g_out, kFp4Threads));
+    for (size_t chunk = blockIdx.x;;) {
+        const size_t base = base_of(chunk);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t i = base + (size_t)u * kFp4Threads;
+            uint32_t byte;
+            const uint32_t word = fp4_encode<NV>(v[u], inv_g, byte);
+            if (i < groups) {
+                codes[i] = word;
+                if constexpr (NV) {
+                    if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
+                } else {
+                    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+                }
+            }
+        }
+        chunk += gridDim.x;
+        if (chunk >= chunks) break;
+        load(base_of(chunk));
     }
 }
 

@@ -100,6 +100,23 @@ __device__ __forceinline__ void copy_async_16(uint32_t dst, const void *src, boo
 __device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
+// two f32 operations an instruction, rounded as the single ones: (a0, a1) * s, (a0, a1) * s + (c0, c1)
+__device__ __forceinline__ void mul_f32x2(float a0, float a1, float s, float &d0, float &d1) {
+    asm("{\n\t.reg .b64 a, s, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\t"
+        "mul.rn.f32x2 d, a, s;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(s));
+}
+__device__ __forceinline__ void fma_f32x2(float a0, float a1, float s, float c0, float c1, float &d0, float &d1) {
+    asm("{\n\t.reg .b64 a, s, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 c, {%5, %6};\n\t"
+        "fma.rn.f32x2 d, a, s, c;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(s), "f"(c0), "f"(c1));
+}
 // 2^x and 1/x, good to a few ulp; results below 2^-126 are 0
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
