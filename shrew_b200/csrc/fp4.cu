@@ -38,7 +38,7 @@ int quantize_as(shrewq_ctx *ctx, const T *x, size_t rows, size_t cols, size_t ld
     } else {
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = aligned && (ld * sizeof(T)) % (8 * sizeof(T)) == 0;
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_rows_kernel<T, NV, false>, dim3((unsigned)(rows < 0x7FFFFFFF ? rows : 0x7FFFFFFF)),
+        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_rows_kernel<T, NV>, dim3((unsigned)(rows < 0x7FFFFFFF ? rows : 0x7FFFFFFF)),
                                               dim3((unsigned)(threads < kFp4Threads ? threads : kFp4Threads)), 0, ctx->stream, pdl, x, rows, cols, ld,
                                               vec_ok, (const float *)g, (const float *)partials, n_partials, g, blocks, codes, scales));
     }

@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t fp4_encode(float *v, float inv_g, uint32_t &
         byte = amax == 0.0f ? kE8m0One : (uint32_t)(e > 0 ? e : 0);
         const float inv = __uint_as_float((254u - byte) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inv;
+        for (int i = 0; i < 8; i += 2) mul_f32x2(v[i], v[i + 1], inv, v[i], v[i + 1]);
         if (bad) byte = kE8m0Nan;
     }
     return bad ? 0u : cvt_e2m1x8(v);
@@ -258,12 +258,9 @@ __device__ __forceinline__ size_t scale_piece_offset(size_t row, size_t block, s
     return ((row >> 7) * pieces + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-// ---- quantize: any rows (strides, widths, alignments), and the activations of a 4-bit product ---------------------------------
-// A CTA a row at a time; PIECES: the scales go to the order of scale_piece_offset, out to `blocks_out` blocks a row (scale 1 beyond
-// the row's end).  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.  The loads of four groups a thread are under way together: one
-// at a time left 4096 x 11008 bf16 at 30 us, and a byte at a time the scales.
-constexpr int kRowsUnroll = 4;
-template <typename T, bool NV, bool PIECES>
+// ---- quantize: any rows (strides, widths, alignments) ---------------------------------------------------------------------------
+// A CTA a row at a time.  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.
+template <typename T, bool NV>
 __global__ void __launch_bounds__(kFp4Threads)
 fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size_t ld, int vec_ok, const float *g_in, const float *partials,
                          int n_partials, float *g_out, size_t blocks_out, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
@@ -276,30 +273,57 @@ fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size
     const size_t groups = blocks_out << kShift;         // >= words
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *src = x + row * ld;
-        for (size_t i0 = 0; i0 < groups; i0 += kRowsUnroll * blockDim.x) {  // (uniform: the shuffles need whole warps)
-            float v[kRowsUnroll][8];
+        for (size_t i0 = 0; i0 < groups; i0 += blockDim.x) {  // (uniform: the shuffles need whole warps)
+            const size_t i = i0 + threadIdx.x;
+            float v[8];
+            if (vec_ok && i * 8 + 8 <= cols) load_vec8<T>(src + i * 8, v);
+            else load_guarded8<T>(src + i * 8, i * 8 < cols ? cols - i * 8 : 0, v);
+            uint32_t byte;
+            const uint32_t word = fp4_encode<NV>(v, inv_g, byte);
+            if (i < words) codes[row * words + i] = word;
+            if (i < groups && (i & ((1 << kShift) - 1)) == 0) scales[row * blocks_out + (i >> kShift)] = (uint8_t)byte;
+        }
+    }
+}
+
+// ---- quantize: the activations of a 4-bit product --------------------------------------------------------------------------------
+// As above, but the scales go to the order of scale_piece_offset, out to whole pieces (scale 1 beyond the row's end): `units` runs of 256
+// values a row, a warp a run, two of them requested together.  Four blocks of a row are one word of a piece.  Indices within a row are 32-bit and
+// whole runs take no guards: with the indexing of the kernel above 4096 x 11008 bf16 took 130 instructions for 8 values a lane and 37 us.
+template <typename T, bool NV>
+__global__ void __launch_bounds__(kFp4Threads)
+fp4_quantize_acts_kernel(const T *__restrict__ x, size_t rows, uint32_t cols, int vec_ok, const float *g_in, uint32_t units, uint32_t *__restrict__ codes,
+                         uint8_t *__restrict__ scales) {
+    pdl_launch_dependents();
+    pdl_wait();
+    float inv_g = 1.0f;
+    if constexpr (NV) inv_g = __fdiv_rn(1.0f, *g_in);
+    constexpr int kShift = NV ? 1 : 2, kPieces = NV ? 4 : 2;  // groups of 8 in a block, as a power of two; pieces that a run fills
+    const uint32_t words = (cols + 31) / 32 * 4, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const size_t pieces = (size_t)units * kPieces;
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *src = x + row * cols;
+        uint32_t *code_row = codes + row * words;
+        uint8_t *scale_row = scales + scale_piece_offset(row, 0, pieces) + (lane >> (kShift + 2)) * 512;
+        for (uint32_t u = threadIdx.x >> 5; u < units; u += 2 * warps) {
+            float v[2][8];
 #pragma unroll
-            for (int u = 0; u < kRowsUnroll; ++u) {
-                if (i0 + u * blockDim.x >= groups) continue;
-                const size_t i = i0 + u * blockDim.x + threadIdx.x;
-                if (vec_ok && i * 8 + 8 <= cols) load_vec8<T>(src + i * 8, v[u]);
-                else load_guarded8<T>(src + i * 8, i * 8 < cols ? cols - i * 8 : 0, v[u]);
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t i = (u + k * warps) * 32 + lane;
+                if (k == 1 && u + warps >= units) break;
+                if (vec_ok && (u + k * warps + 1) * 256 <= cols) load_vec8<T>(src + (size_t)i * 8, v[k]);
+                else load_guarded8<T>(src + (size_t)i * 8, i * 8 < cols ? cols - i * 8 : 0, v[k]);
             }
 #pragma unroll
-            for (int u = 0; u < kRowsUnroll; ++u) {
-                if (i0 + u * blockDim.x >= groups) continue;
-                const size_t i = i0 + u * blockDim.x + threadIdx.x;
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t run = u + k * warps, i = run * 32 + lane;
+                if (k == 1 && run >= units) break;
                 uint32_t byte;
-                const uint32_t word = fp4_encode<NV>(v[u], inv_g, byte);
-                if (i < words) codes[row * words + i] = word;
-                if constexpr (PIECES) {  // four blocks of a row are one word there, and `blocks_out` is a multiple of 4
-                    uint32_t four = byte | __shfl_xor_sync(0xFFFFFFFFu, byte, 1 << kShift) << 8;
-                    four |= __shfl_xor_sync(0xFFFFFFFFu, four, 2 << kShift) << 16;
-                    if (i < groups && (i & ((4 << kShift) - 1)) == 0)
-                        *reinterpret_cast<uint32_t *>(scales + scale_piece_offset(row, i >> kShift, blocks_out >> 2)) = four;
-                } else {
-                    if (i < groups && (i & ((1 << kShift) - 1)) == 0) scales[row * blocks_out + (i >> kShift)] = (uint8_t)byte;
-                }
+                const uint32_t word = fp4_encode<NV>(v[k], inv_g, byte);
+                if (i < words) code_row[i] = word;
+                uint32_t four = byte | __shfl_xor_sync(0xFFFFFFFFu, byte, 1 << kShift) << 8;
+                four |= __shfl_xor_sync(0xFFFFFFFFu, four, 2 << kShift) << 16;
+                if ((lane & ((4 << kShift) - 1)) == 0) *reinterpret_cast<uint32_t *>(scale_row + (size_t)run * (kPieces * 512)) = four;
             }
         }
     }

@@ -13,11 +13,11 @@ namespace {
 
 template <typename T, bool NV>
 cudaError_t quantize_acts(shrewq_ctx *ctx, const Fp4Forward &a, uint32_t *codes, uint8_t *pieces) {
-    const size_t blocks = fp4_pieces(a.K, NV) * 4, threads = blocks * (NV ? 2 : 4);
+    const uint32_t units = (uint32_t)((a.K + 255) / 256);
     const int vec_ok = (reinterpret_cast<uintptr_t>(a.x) % (8 * sizeof(T))) == 0 && a.K % 8 == 0;
-    return launch_maybe_pdl(fp4_quantize_rows_kernel<T, NV, true>, dim3((unsigned)(a.M < 0x7FFFFFFF ? a.M : 0x7FFFFFFF)),
-                            dim3((unsigned)(threads < kFp4Threads ? threads : kFp4Threads)), 0, ctx->stream, ctx->tuning.pdl != 0, static_cast<const T *>(a.x),
-                            a.M, a.K, a.K, vec_ok, (const float *)&a.w->params->x_scale, (const float *)nullptr, 0, (float *)nullptr, blocks, codes, pieces);
+    return launch_maybe_pdl(fp4_quantize_acts_kernel<T, NV>, dim3((unsigned)(a.M < 0x7FFFFFFF ? a.M : 0x7FFFFFFF)),
+                            dim3(units < kFp4Threads / 32 ? units * 32 : kFp4Threads), 0, ctx->stream, ctx->tuning.pdl != 0, static_cast<const T *>(a.x), a.M,
+                            (uint32_t)a.K, vec_ok, (const float *)&a.w->params->x_scale, units, codes, pieces);
 }
 
 size_t pair_tiles(const Fp4Forward &a) { return (a.N + (a.up ? 127 : 255)) / (a.up ? 128 : 256) * ((a.M + kPairTok - 1) / kPairTok); }

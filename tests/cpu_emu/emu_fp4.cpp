@@ -28,7 +28,7 @@ void quantize(const void *x, size_t rows, size_t cols, size_t ld, float *g, bool
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = (reinterpret_cast<uintptr_t>(p) % (8 * sizeof(T))) == 0 && ld % 8 == 0;
         emu::launch((unsigned)std::min<size_t>(rows, 3), (unsigned)std::min<size_t>(threads, kFp4Threads), [&] {
-            fp4_quantize_rows_kernel<T, NV, false>(p, rows, cols, ld, vec_ok, g, pp, (int)grid, g, blocks, c, s);
+            fp4_quantize_rows_kernel<T, NV>(p, rows, cols, ld, vec_ok, g, pp, (int)grid, g, blocks, c, s);
         });
     }
 }

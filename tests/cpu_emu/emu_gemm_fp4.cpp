@@ -51,7 +51,7 @@ int run(const uint8_t *const *codes, const uint8_t *const *scales, const float *
     uint8_t *xc = aligned(raw[2], M * pitch, 0xEE), *xp = aligned(raw[3], (M + 127) / 128 * pieces * 512, 0xFF);
     const size_t blocks = pieces * 4, threads = std::min<size_t>(blocks * (NV ? 2 : 4), kFp4Threads);
     emu::launch(M, (unsigned)threads, [&] {
-        fp4_quantize_rows_kernel<float, NV, true>(x, M, K, K, 0, &params[0].x_scale, nullptr, 0, nullptr, blocks, reinterpret_cast<uint32_t *>(xc), xp);
+        fp4_quantize_acts_kernel<float, NV>(x, M, K, (reinterpret_cast<uintptr_t>(x) & 31) == 0 && K % 8 == 0, &params[0].x_scale, (K + 255) / 256, reinterpret_cast<uint32_t *>(xc), xp);
     });
     const Operands ops{alpha[0].data(), bias[0], alpha[GATED ? 1 : 0].data(), bias[GATED ? 1 : 0]};
     DeviceStatus status{0, 0, 0, 0};
