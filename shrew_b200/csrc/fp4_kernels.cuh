@@ -138,7 +138,7 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
 // partials[block] = largest finite magnitude of the values that the block saw; the quantizing kernel takes the maximum of them.
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_amax_kernel(const T *__restrict__ x, size_t rows, size_t cols, size_t ld, float *__restrict__ partials) {
+fp4_amax_kernel(const T *x, size_t rows, size_t cols, size_t ld, float *__restrict__ partials) {
     pdl_launch_dependents();
     pdl_wait();
     float amax = 0.0f;
@@ -209,7 +209,7 @@ __device__ __forceinline__ float fp4_block_tensor_scale(const float *g_in, const
 // has read it from the front (BACK): what that pass left in L2 is read first.
 template <typename T, bool NV, int U>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_quantize_flat_kernel(const T *__restrict__ x, size_t groups, const float *g_in, const float *partials, int n_partials, float *g_out,
+fp4_quantize_flat_kernel(const T *x, size_t groups, const float *g_in, const float *partials, int n_partials, float *g_out,
                          uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
@@ -262,7 +262,7 @@ __device__ __forceinline__ size_t scale_piece_offset(size_t row, size_t block, s
 // A CTA a row at a time.  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size_t ld, int vec_ok, const float *g_in, const float *partials,
+fp4_quantize_rows_kernel(const T *x, size_t rows, size_t cols, size_t ld, int vec_ok, const float *g_in, const float *partials,
                          int n_partials, float *g_out, size_t blocks_out, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
@@ -292,7 +292,7 @@ fp4_quantize_rows_kernel(const T *__restrict__ x, size_t rows, size_t cols, size
 // whole runs take no guards: with the indexing of the kernel above 4096 x 11008 bf16 took 130 instructions for 8 values a lane and 37 us.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_quantize_acts_kernel(const T *__restrict__ x, size_t rows, uint32_t cols, int vec_ok, const float *g_in, uint32_t units, uint32_t *__restrict__ codes,
+fp4_quantize_acts_kernel(const T *x, size_t rows, uint32_t cols, int vec_ok, const float *g_in, uint32_t units, uint32_t *__restrict__ codes,
                          uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
@@ -375,7 +375,7 @@ __device__ __forceinline__ void from_f32(float v, __half *p) { *p = __float2half
 // flat: rows that are whole 32s and an aligned output; U groups of 8 a thread
 template <typename T, bool NV, int U>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_dequantize_flat_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, const float *g_in, size_t groups, T *__restrict__ out) {
+fp4_dequantize_flat_kernel(const uint32_t *codes, const uint8_t *scales, const float *g_in, size_t groups, T *__restrict__ out) {
     pdl_launch_dependents();
     pdl_wait();
     const float g = NV ? *g_in : 1.0f;
@@ -399,7 +399,7 @@ fp4_dequantize_flat_kernel(const uint32_t *__restrict__ codes, const uint8_t *__
 
 template <typename T, bool NV>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_dequantize_rows_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, const float *g_in, size_t rows, size_t cols,
+fp4_dequantize_rows_kernel(const uint32_t *codes, const uint8_t *scales, const float *g_in, size_t rows, size_t cols,
                            int vec_ok, T *__restrict__ out) {
     pdl_launch_dependents();
     pdl_wait();

@@ -93,7 +93,7 @@ __device__ __forceinline__ void e4m3_bf16x2(uint32_t two, uint32_t &first, uint3
 // f32 or bf16 activations of any width and alignment -> XT bf16 terms [XT][M][Kp], zeros beyond K
 template <typename T, int XT>
 __global__ void __launch_bounds__(256)
-stage_bf16_kernel(const T *__restrict__ x, size_t M, size_t K, size_t Kp, int vec_ok, uint16_t *__restrict__ terms) {
+stage_bf16_kernel(const T *x, size_t M, size_t K, size_t Kp, int vec_ok, uint16_t *__restrict__ terms) {
     pdl_launch_dependents();
     pdl_wait();
     const size_t per_row = Kp >> 3, total = M * per_row, plane = M * Kp;

@@ -32,7 +32,7 @@ int launch_one(shrewq_ctx *ctx, const Fp4Forward &a, const Staged &x) {
     const Fp4Operand w0{a.w->codes, a.w->pieces, a.w->params, a.bias};
     const Fp4Operand w1 = GATED ? Fp4Operand{a.up->codes, a.up->pieces, a.up->params, a.bias_up} : w0;
     SHREWQ_CUDA_TRY(ctx, launch_cluster(kern, (unsigned)(tiles * S), kH4Threads, (size_t)C::kSmemRequest, ctx->stream, a.pdl, S, tw, tw2, tx, w0, w1, a.alpha,
-                                        GATED ? a.alpha_up : a.alpha, x.exps, x.counts, x.octaves, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,
+                                        GATED ? a.alpha_up : a.alpha, (const int *)x.exps, (const int *)x.counts, x.most, x.octaves, static_cast<YT *>(a.y), (int)a.M, (int)a.N, (int)a.K, a.ldy,
                                         a.epilogue, S, per_cta, ctx->dev_status));
     ctx->launches += 1;
     SHREWQ_CUDA_TRY(ctx, cudaGetLastError());

@@ -67,12 +67,12 @@ __device__ __forceinline__ void widen32_f16(const uint4 c, uint32_t f_lo, uint32
     }
 }
 
-// x: terms of M rows, stacked (tmap_x); exps, counts: by token
+// x: terms of M rows, `most` of them stacked (tmap_x); exps, counts: by token
 template <int TOK, bool NV, bool GATED, typename YT>
 __global__ void __launch_bounds__(kH4Threads, 2)
 gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2, const __grid_constant__ CUtensorMap tmap_x, Fp4Operand w0,
-                   Fp4Operand w1, const float *__restrict__ alpha0, const float *__restrict__ alpha1, const int *__restrict__ exps, const int *__restrict__ counts,
-                   int octaves, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue, int S, int rounds_per_cta, DeviceStatus *status) {
+                   Fp4Operand w1, const float *__restrict__ alpha0, const float *__restrict__ alpha1, const int *exps, const int *counts,
+                   int most, int octaves, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue, int S, int rounds_per_cta, DeviceStatus *status) {
     using C = H4Cfg<TOK, NV, GATED>;
     constexpr int kChan = GATED ? 64 : 128, kMode = GATED ? kEpiLanesPaired : kEpiPlain;
     SHREWQ_DYNAMIC_SMEM(uint8_t, smem_raw);
@@ -140,8 +140,9 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 
     // passes: the terms that any token needs times the windows of the scales
     int n_terms = 1;
-    for (int m = lane; m < M; m += 32) n_terms = counts[m];
+    for (int m = lane; m < M; m += 32) n_terms = ld_written_s32(counts + m);
     n_terms = (int)warp_max((unsigned int)n_terms);
+    n_terms = n_terms < most ? n_terms : most;
     int top = 0, windows = 1;
     if constexpr (!NV) {
         top = w0.params->max_byte;

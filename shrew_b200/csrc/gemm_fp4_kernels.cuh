@@ -115,8 +115,8 @@ struct CopyRows {
 
 template <int TOK, bool NV, bool GATED, typename YT>
 __global__ void __launch_bounds__(kFp4GemmThreads, 1)
-gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__ w2_codes, const uint8_t *__restrict__ x_codes, const uint8_t *__restrict__ w_pieces,
-                const uint8_t *__restrict__ w2_pieces, const uint8_t *__restrict__ x_pieces, Operands ops, YT *__restrict__ y, int M, int N, int K, size_t ldy,
+gemm_fp4_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__ w2_codes, const uint8_t *x_codes, const uint8_t *__restrict__ w_pieces,
+                const uint8_t *__restrict__ w2_pieces, const uint8_t *x_pieces, Operands ops, YT *__restrict__ y, int M, int N, int K, size_t ldy,
                 int epilogue, int S, int rounds_per_cta, DeviceStatus *status) {
     using C = Fp4Cfg<TOK, NV, GATED>;
     pdl_launch_dependents();

@@ -147,8 +147,8 @@ struct PairEpilogue {
 // Grid: pairs * 2 CTAs; pair p takes the tiles p, p + pairs, ..., token tiles fastest.
 template <bool NV, bool GATED, typename YT>
 __global__ void __launch_bounds__(kPairThreads, 1)
-gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__ w2_codes, const uint8_t *__restrict__ x_codes,
-                     const uint8_t *__restrict__ w_pieces, const uint8_t *__restrict__ w2_pieces, const uint8_t *__restrict__ x_pieces, Operands ops,
+gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restrict__ w2_codes, const uint8_t *x_codes,
+                     const uint8_t *__restrict__ w_pieces, const uint8_t *__restrict__ w2_pieces, const uint8_t *x_pieces, Operands ops,
                      YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue, int tiles, int pairs, DeviceStatus *status) {
     using C = Fp4PairCfg<NV, GATED, YT>;
     pdl_launch_dependents();

@@ -115,7 +115,7 @@ __device__ __forceinline__ bool f16_terms(float *v, unsigned int top, uint4 *out
 // the token was divided by; counts[m]: terms in use.
 template <typename T>
 __global__ void __launch_bounds__(256)
-stage_f16_kernel(const T *__restrict__ x, int M, int K, int Kp, int vec_ok, uint4 *__restrict__ terms, int *__restrict__ exps, int *__restrict__ counts) {
+stage_f16_kernel(const T *x, int M, int K, int Kp, int vec_ok, uint4 *__restrict__ terms, int *__restrict__ exps, int *__restrict__ counts) {
     pdl_launch_dependents();
     __shared__ unsigned int s_max[8], s_more[8];
     const int m = blockIdx.x, threads = (int)blockDim.x, warps = threads >> 5, groups = Kp >> 3;
@@ -179,7 +179,7 @@ __device__ __forceinline__ int gemv4_row(int tile, int i) {
 // M <= kGemv4MaxStaged
 template <bool NV, bool GATED, typename T, typename YT>
 __global__ void __launch_bounds__(kGemv4Threads, 1)
-gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const T *__restrict__ x, int vec_ok, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
+gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const T *x, int vec_ok, YT *__restrict__ y, int M, int N, int K, size_t ldy, int epilogue) {
     constexpr int kRows = GATED ? 8 : 16;
     SHREWQ_DYNAMIC_SMEM(uint8_t, smem);  // ring, then the staged activations
     __shared__ float s_red[2][kGemv4Warps][4][32];
@@ -382,7 +382,7 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const T *__restrict__ x, int vec_o
 // channel n is multiplied by, the tensor scales of both operands.
 template <bool NV>
 __global__ void __launch_bounds__(256)
-fp4_scale_pieces_kernel(const uint8_t *__restrict__ scales, const float *g, size_t N, size_t blocks, size_t pieces, uint8_t *__restrict__ out,
+fp4_scale_pieces_kernel(const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, uint8_t *__restrict__ out,
                         Fp4Params *params, float x_scale, float *__restrict__ alpha) {
     const size_t total = (N + 127) / 128 * 128 * pieces;  // words
     int top = 0, low = 255;

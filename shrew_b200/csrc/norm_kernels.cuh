@@ -46,7 +46,7 @@ __device__ __forceinline__ void load_params8(const float *p, int c, int D, int v
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = otherwise;
     } else if (vec) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(p + c)), b = __ldg(reinterpret_cast<const float4 *>(p + c) + 1);
+        const float4 a = *reinterpret_cast<const float4 *>(p + c), b = *(reinterpret_cast<const float4 *>(p + c) + 1);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {

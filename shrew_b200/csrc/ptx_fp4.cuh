@@ -128,6 +128,13 @@ __device__ __forceinline__ float recip_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// A word that the kernel before in the stream has written, read where it stands in the program, from L2.  (Through a const __restrict__ pointer
+// it would be a load of data that never changes, which the compiler may move to before griddepcontrol.wait.)
+__device__ __forceinline__ int ld_written_s32(const int *p) {
+    int v;
+    asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
 // this thread arrives on the barrier (of a count that includes it) when all of its copies so far have landed
 __device__ __forceinline__ void copy_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

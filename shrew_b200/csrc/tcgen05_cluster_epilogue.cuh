@@ -15,6 +15,7 @@
 #pragma once
 
 #include "ptx_cluster.cuh"
+#include "ptx_fp4.cuh"
 #include "ptx_tcgen05_fp4.cuh"
 #include "tcgen05_common.cuh"
 #include "tcgen05_epilogue.cuh"
@@ -96,7 +97,7 @@ __device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_loc
 template <int NCOLS, int G, int MODE, typename YT, bool TOKENS = false>
 __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_base, const float *slots, int S, uint32_t rank, int group, int quad, int lane, bool ok,
                                                const Operands &ops, YT *__restrict__ y, int M, int N, size_t ldy, int epilogue, int n0, int m0,
-                                               const int *__restrict__ exps = nullptr, int back = 0) {
+                                               const int *exps = nullptr, int back = 0) {
     constexpr int CW = kEpiChunk, CH = MODE == kEpiLanesPaired ? 64 : 128, RB = CH * (int)sizeof(YT), EPV = 16 / (int)sizeof(YT), PPR = RB / 16, PIECES = CW * PPR;
     constexpr int ACCS = ClusterEpi<NCOLS, MODE>::kAccs;
     const int F = cluster_finishers<NCOLS>(S), tokens = NCOLS / F, row = quad * 32 + lane;
@@ -153,7 +154,7 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
             for (int i = 0; i < CW; ++i) {
                 if constexpr (TOKENS) {
                     const int m = m0 + first_col + c * CW + i;
-                    const int e = m < M ? exps[m] + back : 0;
+                    const int e = m < M ? ld_written_s32(exps + m) + back : 0;
 #pragma unroll
                     for (int a = 0; a < ACCS; ++a) v[a][i] = ldexpf(v[a][i], e);
                 }

@@ -105,6 +105,7 @@ static inline void mul_f32x2(float a0, float a1, float s, float &d0, float &d1) 
 static inline void fma_f32x2(float a0, float a1, float s, float c0, float c1, float &d0, float &d1) {
     d0 = fmaf(a0, s, c0), d1 = fmaf(a1, s, c1);
 }
+static inline int ld_written_s32(const int *p) { return *p; }
 static inline float exp2_approx(float x) { return exp2f(x); }
 static inline float recip_approx(float x) { return 1.0f / x; }
 static inline void mbar_arrive(uint32_t bar);

@@ -133,7 +133,7 @@ int run_h4(const uint8_t *const *codes, const uint8_t *const *scales, const floa
     DeviceStatus status{0, 0, 0, 0};
     const int rounds = (K + kH4StageK - 1) / kH4StageK, per_cta = split ? (rounds + 1) / 2 : rounds;
     launch_tiles((size_t)(N + box - 1) / box, split, kH4Threads, C::kSmemBytes, [&] {
-        gemm_w4_f16_kernel<TOK, NV, GATED, float>(tw, tw2, tx, w0, w1, alpha[0].data(), alpha[GATED ? 1 : 0].data(), exps.data(), counts.data(), XTerms<T>::kOctaves, y, M,
+        gemm_w4_f16_kernel<TOK, NV, GATED, float>(tw, tw2, tx, w0, w1, alpha[0].data(), alpha[GATED ? 1 : 0].data(), exps.data(), counts.data(), XTerms<T>::kMost, XTerms<T>::kOctaves, y, M,
                                                   N, K, ldy, epilogue, split ? 2 : 1, per_cta, &status);
     });
     return outcome(status);

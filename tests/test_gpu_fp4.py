@@ -285,6 +285,25 @@ def test_streams_graphs_and_repetition(rounded, m):
     gate.device.synchronize()
 
 
+@pytest.mark.parametrize("rounded", [False, True])
+@pytest.mark.parametrize("m", [4, 8, 16, 32, 64, 250])
+def test_layers_of_different_widths_in_turn(rounded, m):
+    """Two layers that share the context's workspace, laid out for another k each, over and over: the same bits each time."""
+    gate, _, _ = layer(384, 1024, Fp4Format.Nv, 1, quantize_activations=rounded)
+    up, _, _ = layer(384, 1024, Fp4Format.Nv, 2, quantize_activations=rounded)
+    down, _, _ = layer(1024, 384, Fp4Format.Nv, 3, quantize_activations=rounded)
+    xs = [acts(m, 1024, BF16, seed=s) * 0.01 for s in range(3)]
+    want = []
+    for x in xs:
+        h = gate.forward_gate_up_silu(up, x)
+        torch.cuda.synchronize()
+        want.append(down.forward(h))
+        torch.cuda.synchronize()
+    for _ in range(30):
+        got = [down.forward(gate.forward_gate_up_silu(up, x)) for x in xs]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_layer_surface_and_host_buffers():
     w = torch.randn(96, 160, device="cuda")
     b = torch.randn(96, device="cuda")
