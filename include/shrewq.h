@@ -89,7 +89,8 @@ SHREWQ_API int shrewq_ctx_set_stream(shrewq_ctx *ctx, void *stream);
 /* Streams: calls enqueued on different streams of one context are not ordered among each other.  Quantizing (per channel;
  * one tensor per tensor, up to eight calls in flight), dequantizing and forwards that are not split along K share nothing.
  * Forwards split along K, f32 forwards above 1024 features or with bf16 results, layers with zero points, packed INT4
- * above 4 tokens, batched per-tensor, f64 per-tensor and supplied-amax quantizing and the *_host calls use workspaces of the
+ * above 4 tokens, 4-bit floating-point layers as told at shrewq_linear_create_fp4, batched per-tensor, f64 per-tensor and supplied-amax
+ * quantizing and the *_host calls use workspaces of the
  * context: two of those must not overlap on different streams (order them by events, or use a context per stream). */
 /* Launch options of a context (no counterpart in the reference); the defaults are the measured choices and
  * need no setting.  name / value:
@@ -275,7 +276,8 @@ SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_
  *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens.
  *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
  *     positive number, as the tensor scale), and codes are multiplied by codes on the block-scaled tensor cores.
- * Both use the context's workspace (staged activations, partial sums): see shrewq_ctx_set_stream.
+ * Workspaces of the context (see shrewq_ctx_set_stream): quantize_activations = 1 always, for the codes; else 5 to 32 tokens, and above 32
+ * f32 activations and bf16 ones whose rows are not whole 16-byte pieces, for a staged copy.
  */
 SHREWQ_API int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev,
                                         const float *bias_dev, size_t out_features, size_t in_features, int format,
@@ -447,7 +449,8 @@ SHREWQ_API size_t shrewq_linear_out_features(const shrewq_linear *lin);
 SHREWQ_API size_t shrewq_linear_memory_savings_bytes(const shrewq_linear *lin);
 
 /* Name of the kernel family the calling thread's latest forward dispatched to ("gemv", "mma", "mma-ring",
- * "tcgen05", "tcgen05-2cta", "tcgen05-f32", "simt", "mma-w4"); for tests and benchmarks.  Kept per thread, not
+ * "tcgen05", "tcgen05-2cta", "tcgen05-f32", "simt", "mma-w4"; 4-bit floating-point weights: "mma-fp4", "tcgen05-w4-f16", "tcgen05-w4",
+ * "tcgen05-fp4"); for tests and benchmarks.  Kept per thread, not
  * in the handle: the one thing a forward writes to the handle it reads is an atomic flag saying that a
  * forward has been enqueued. */
 SHREWQ_API const char *shrewq_linear_last_kernel(const shrewq_linear *lin);

@@ -141,7 +141,6 @@ int launch_dequantize(shrewq_ctx *ctx, const int8_t *q, const double *scales, si
 int launch_scales_to_f32(shrewq_ctx *ctx, const double *scales, int granularity, size_t n, float *out);
 int launch_split_f32(shrewq_ctx *ctx, const float *x, size_t n, void *hi_bf16, void *lo_bf16);
 int ensure_xsplit(shrewq_ctx *ctx, size_t bytes);
-int ensure_ytmp(shrewq_ctx *ctx, size_t bytes);
 int launch_quantize_ex(shrewq_ctx *ctx, const float *w, size_t rows, size_t cols, int granularity, int bits, int mode,
                        int8_t *q, double *scales, double *zps);
 int launch_quantize_any(shrewq_ctx *ctx, const void *w, int w_dtype, size_t rows, size_t cols, int granularity, int bits,

@@ -18,6 +18,9 @@
 // the leader.  (Arrivals with .release.cluster by the copying warps took 1200 cycles a stage.)  The accumulators, 256 columns, and the stages' scales
 // fill tensor memory, so the MMAs of the next tile wait until the sums have been read: all warps that are free then take part, after the
 // next tile's first stages are under way.
+// Measured: 4096 x 11008 MX, 4096 tokens: 85 us of 114 to 118 for the call (quantizing the tokens is the rest; 3.1 PFLOP/s over all, at 1680 MHz under the
+// power limit); gated 11008 x 4096 NV, 512 tokens: 35 us, 36 to 39 for the call.  What is left: 256 tiles for 74 pairs are 3.5 rounds, and a stage
+// takes 540 to 600 cycles to bring for 512 of matrix work.
 //
 // Device code only; also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once

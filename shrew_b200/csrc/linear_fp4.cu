@@ -131,9 +131,9 @@ int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const ui
     }
     rc = launch_fp4_scale_pieces(ctx, scales_dev, tensor_scale_dev, out_features, (in_features + 31) / 32 * (nv ? 2 : 1), pieces, nv, w->pieces, w->params, w->x_scale,
                                  lin->scales_f32);
-    // boxes of the tensor-core kernels: 128 rows of 256 codes (codes by codes), or of 128 codes with 128 and, gated, 64 rows
-    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 128, w->round_x ? 128 : 64, lin->w_tmap);
-    if (rc == SHREWQ_OK) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, w->round_x ? 128 : 64, w->round_x ? 128 : 64, lin->w_tmap64);
+    // boxes of the tensor-core kernels that take activations as they come: 128 codes of 128 and, gated, 64 rows
+    if (rc == SHREWQ_OK && !w->round_x) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 128, 64, lin->w_tmap);
+    if (rc == SHREWQ_OK && !w->round_x) rc = encode_fp4_tmap(ctx, codes_dev, out_features, in_features, 64, 64, lin->w_tmap64);
     if (rc != SHREWQ_OK) {
         shrewq_linear_destroy(lin);
         return rc;

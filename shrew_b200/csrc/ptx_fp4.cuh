@@ -11,12 +11,6 @@
 namespace shrewq {
 namespace {
 
-// two f32 -> two E2M1 codes in a byte (lo in the low nibble), round to nearest even, saturating at 6
-__device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
-    uint32_t d;
-    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(d) : "f"(hi), "f"(lo));
-    return d;
-}
 // eight f32 -> eight E2M1 codes in a word, v[0] in the lowest nibble
 __device__ __forceinline__ uint32_t cvt_e2m1x8(const float *v) {
     uint32_t d;

@@ -25,7 +25,6 @@ static inline uint32_t emu_e2m1(float v) {
     const float lo = a - grid[c], hi = grid[c + 1] - a;
     return sign | (lo < hi || (lo == hi && (c & 1) == 0) ? c : c + 1);
 }
-static inline uint32_t cvt_e2m1x2(float lo, float hi) { return emu_e2m1(lo) | emu_e2m1(hi) << 4; }
 static inline uint32_t cvt_e2m1x8(const float *v) {
     uint32_t d = 0;
     for (int i = 0; i < 8; ++i) d |= emu_e2m1(v[i]) << (4 * i);
