@@ -285,6 +285,35 @@ def test_streams_graphs_and_repetition(rounded, m):
     gate.device.synchronize()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_wide_products_captured_and_repeated(fmt):
+    """Outputs that fill the machine, tile after tile: the same bits eagerly, on another stream and from a graph with new data."""
+    gate, _, _ = layer(4900, 608, fmt, 1, quantize_activations=True)
+    up, _, _ = layer(4900, 608, fmt, 2, quantize_activations=True)
+    down, _, _ = layer(608, 4900, fmt, 3, quantize_activations=True)
+    xs = [acts(700, 608, BF16, seed=s) * 0.01 for s in range(3)]
+
+    def run(x):
+        return down.forward(gate.forward_gate_up_silu(up, x))
+    want = [run(x) for x in xs]
+    for _ in range(20):
+        assert all(torch.equal(run(x), w) for x, w in zip(xs, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [run(x) for x in xs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    x, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run(x)
+    for x_new, w in zip(xs, want):
+        x.copy_(x_new)
+        graph.replay()
+        assert torch.equal(y, w)
+    gate.device.synchronize()
+
+
 @pytest.mark.parametrize("rounded", [False, True])
 @pytest.mark.parametrize("m", [4, 8, 16, 32, 64, 250])
 def test_layers_of_different_widths_in_turn(rounded, m):
