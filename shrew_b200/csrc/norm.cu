@@ -21,7 +21,10 @@ cudaError_t launch_typed(shrewq_ctx *ctx, const NormArgs &a) {
         return launch_maybe_pdl(residual_norm_kernel<TX, TB, TY, 4, true>, grid, block, 0, ctx->stream, pdl, a);
     }
     const int V = groups <= 2048 ? 2 : 4;
-    const dim3 grid((unsigned)(a.M < most ? a.M : most)), block((unsigned)(((groups + V - 1) / V + 31) / 32 * 32));
+    const dim3 block((unsigned)(((groups + V - 1) / V + 31) / 32 * 32));
+    // as many CTAs as are resident (64 registers a thread: 1024 threads an SM), row after row: 4096 rows of 4096 44.3 -> 43.8 us against a CTA a row
+    const size_t resident = (size_t)ctx->sm_count * (1024 / block.x);
+    const dim3 grid((unsigned)(a.M < resident ? a.M : resident));
     if (V == 2) return launch_maybe_pdl(residual_norm_kernel<TX, TB, TY, 2, false>, grid, block, 0, ctx->stream, pdl, a);
     return launch_maybe_pdl(residual_norm_kernel<TX, TB, TY, 4, false>, grid, block, 0, ctx->stream, pdl, a);
 }

@@ -16,6 +16,8 @@
 // Memory-bound: x and branch are read once and r and h written once.  A row lives in the registers of a warp (up to 1024 columns) or of a
 // CTA (V groups of 8 columns a thread), so the two statistics cost no second read.  The weights come through L1, which the rows' streaming
 // loads leave to them.
+// Measured: 4096 rows of 4096, f32 stream, bf16 branch and gate, norms before and after: 44 us, 4.6 TB/s of half reads and half writes; a
+// row is two sums of a CTA, one after the other, and four rows an SM are under way (more threads a row, or rows an SM, need registers that are not there).
 //
 // Device code only (no launch syntax; PTX behind ptx_fp4.cuh and ptx_small.cuh): also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once
@@ -115,6 +117,23 @@ __device__ __forceinline__ void load_row8(const T *row, int c, int D, int vec, f
     } else if (vec) load_vec8<T>(row + c, v);
     else load_guarded8<T>(row + c, (size_t)(D - c), v);
 }
+// eight values that every row uses again: through L1, which the rows' own loads pass by (a gate of channels from L2 for every row:
+// 4096 rows of 4096 in 47.7 us instead of 44.3)
+__device__ __forceinline__ void load_shared8(const float *p, float *v) {
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load_shared8(const __nv_bfloat16 *p, float *v) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(r[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void store_row8(T *row, int c, int D, int vec, const float *v) {
     if (c >= D) return;
@@ -152,7 +171,8 @@ residual_norm_kernel(NormArgs a) {
             for (int u = 0; u < V; ++u) {
                 float g[8];
                 const int c = (u * T + t) * 8;
-                if (a.gate_kind == kGateChannel) load_row8<TB>(gate, c, a.D, a.vec, g);
+                if (a.gate_kind == kGateChannel && a.vec && c < a.D) load_shared8(gate + c, g);
+                else if (a.gate_kind == kGateChannel) load_row8<TB>(gate, c, a.D, a.vec, g);
                 else if (a.gate_kind == kGateFull) load_row8<TB>(gate + m * a.ldg, c, a.D, a.vec, g);
                 else {
 #pragma unroll
