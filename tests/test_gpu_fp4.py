@@ -182,6 +182,26 @@ def test_wide_products_of_quantized_activations(fmt, gated, m, n, k):
     near(y, O.product(xq, w, b, **pair), O.product_bound(xq, w, k, bias=b, **pair))
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("off", [0, 8, 3])
+def test_column_slice_of_a_wide_product(gated, dtype, off):
+    n = 4801
+    lin, _, _ = layer(n, 320, Fp4Format.Nv, 3, quantize_activations=True)
+    up, _, _ = layer(n, 320, Fp4Format.Nv, 4, quantize_activations=True)
+    x = acts(300, 320, BF16) * 0.01
+
+    def run(out):
+        return lin.forward_gate_up_silu(up, x, out=out) if gated else lin.forward(x, out=out)
+    wide = torch.full((301, n + 23), -7.0, dtype=dtype, device="cuda")
+    out = wide[:300, off:off + n]
+    run(out)
+    assert torch.equal(out, run(torch.empty(300, n, dtype=dtype, device="cuda")))
+    mask = torch.ones_like(wide, dtype=torch.bool)
+    mask[:300, off:off + n] = False
+    assert (wide[mask] == -7.0).all()
+
+
 @pytest.mark.parametrize("rounded", [False, True])
 @pytest.mark.parametrize("m", [3, 40, 150])
 def test_column_slice_of_a_wider_buffer(rounded, m):
