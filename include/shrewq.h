@@ -86,8 +86,9 @@ typedef struct shrewq_linear shrewq_linear;
  * cudaStream_t (NULL = the default stream). */
 SHREWQ_API int shrewq_ctx_create(int device, void *stream, shrewq_ctx **out);
 SHREWQ_API int shrewq_ctx_set_stream(shrewq_ctx *ctx, void *stream);
-/* Streams: calls enqueued on different streams of one context are not ordered among each other.  Quantizing (per channel;
- * one tensor per tensor, up to eight calls in flight), dequantizing and forwards that are not split along K share nothing.
+/* Streams: calls enqueued on different streams of one context are not ordered among each other.  Quantizing (per channel; to 4-bit floating
+ * point; one tensor per tensor, up to eight calls in flight: calls take eight places in turn, and a captured call keeps its place, which every
+ * eighth later call takes too, for all of its replays), dequantizing and forwards that are not split along K share nothing.
  * Forwards split along K, f32 forwards above 1024 features or with bf16 results, layers with zero points, packed INT4
  * above 4 tokens, 4-bit floating-point layers as told at shrewq_linear_create_fp4, batched per-tensor, f64 per-tensor and supplied-amax
  * quantizing and the *_host calls use workspaces of the
@@ -223,7 +224,8 @@ SHREWQ_API int shrewq_dequantize_ex(shrewq_ctx *ctx, const int8_t *q_dev, const 
  * w_dev: [rows, cols] of w_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), rows ldw elements apart.  codes_dev must be 4-byte aligned.
  * tensor_scale_dev: NULL for MX; for NV one f32 on the device: read if find_tensor_scale is 0 (a positive number), else written: the
  * smallest power of two g with 2688 g >= the tensor's largest finite magnitude (1 for a tensor of zeros).  Finding it takes a pass over
- * the tensor of its own.  No workspace grows; up to eight calls that find a scale may be in flight on different streams.
+ * the tensor of its own.  find_tensor_scale is then the number of f32 that the call may use at tensor_scale_dev: 1, or more, of which those
+ * behind the first are workspace (1 + rows * ceil(cols / 8) / 1024, 2048 at most, spare a launch).  No workspace of the context: calls share nothing.
  */
 SHREWQ_API int shrewq_quantize_fp4(shrewq_ctx *ctx, const void *w_dev, int w_dtype, size_t rows, size_t cols, size_t ldw, int format,
                                    float *tensor_scale_dev, int find_tensor_scale, uint8_t *codes_dev, uint8_t *scales_dev);

@@ -12,35 +12,47 @@ size_t blocks_of(size_t threads_wanted, size_t cap) {
     return b < 1 ? 1 : (b > cap ? cap : b);
 }
 
+__global__ void fill_f32_kernel(float *p, float v) {
+    pdl_launch_dependents();
+    pdl_wait();
+    *p = v;
+}
+
+int fill_f32(shrewq_ctx *ctx, float *p, float v) {
+    SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fill_f32_kernel, dim3(1), dim3(1), 0, ctx->stream, ctx->tuning.pdl != 0, p, v));
+    ctx->launches += 1;
+    return SHREWQ_OK;
+}
+
 template <typename T, bool NV>
-int quantize_as(shrewq_ctx *ctx, const T *x, size_t rows, size_t cols, size_t ld, float *g, bool find_g, uint32_t *codes, uint8_t *scales) {
+int quantize_as(shrewq_ctx *ctx, const T *x, size_t rows, size_t cols, size_t ld, float *g, int find_g, uint32_t *codes, uint8_t *scales) {
     const bool pdl = ctx->tuning.pdl != 0;
     const bool aligned = (reinterpret_cast<uintptr_t>(x) % (8 * sizeof(T))) == 0;
     const bool flat = aligned && cols % 32 == 0 && (ld == cols || rows == 1);
-    float *partials = nullptr;
-    int n_partials = 0;
+    int source = kScaleGiven;
     if (NV && find_g) {
-        static_assert(kFp4MaxPartials * sizeof(float) <= kTensorSlotBytes, "a slot holds one call's words");
-        partials = reinterpret_cast<float *>(static_cast<char *>(ctx->tensor_slots) +
-                                             ctx->tensor_calls.fetch_add(1, std::memory_order_relaxed) % kTensorSlots * kTensorSlotBytes);
-        const size_t cap = (size_t)ctx->sm_count * 8 < (size_t)kFp4MaxPartials ? (size_t)ctx->sm_count * 8 : (size_t)kFp4MaxPartials;
-        n_partials = (int)blocks_of((flat ? rows * cols / 8 : rows * ((cols + 7) / 8)) / 4, cap);
-        auto kern = flat ? fp4_amax_kernel<T, true> : fp4_amax_kernel<T, false>;
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(kern, dim3((unsigned)n_partials), dim3(kFp4Threads), 0, ctx->stream, pdl, x, rows, cols, ld, partials));
+        const size_t grid = blocks_of((flat ? rows * cols / 8 : rows * ((cols + 7) / 8)) / 4, (size_t)ctx->sm_count * 8);
+        source = (size_t)find_g > grid ? (int)grid : kScaleFound;
+        if (source == kScaleFound && grid > 1) {
+            const int rc = fill_f32(ctx, g, 0.0f);
+            if (rc != SHREWQ_OK) return rc;
+        }
+        auto kern = flat ? fp4_tensor_scale_kernel<T, true> : fp4_tensor_scale_kernel<T, false>;
+        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(kern, dim3((unsigned)grid), dim3(kFp4Threads), 0, ctx->stream, pdl, x, rows, cols, ld, g, (int)(source > 0)));
         ctx->launches += 1;
     }
     constexpr int U = 4;
     const size_t groups = rows * cols / 8, want = (groups + kFp4Threads * U - 1) / (kFp4Threads * U);
     if (flat && want <= 0x7FFFFFFF) {
-        const size_t grid = partials && want > (size_t)ctx->sm_count * 6 ? (size_t)ctx->sm_count * 6 : want;
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_flat_kernel<T, NV, U>, dim3((unsigned)grid), dim3(kFp4Threads), 0, ctx->stream, pdl, x, groups,
-                                              (const float *)g, (const float *)partials, n_partials, g, codes, scales));
+        const size_t grid = source != kScaleGiven && want > (size_t)ctx->sm_count * 6 ? (size_t)ctx->sm_count * 6 : want;
+        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_flat_kernel<T, NV, U>, dim3((unsigned)grid), dim3(kFp4Threads), 0, ctx->stream, pdl, x, groups, g,
+                                              source, codes, scales));
     } else {
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = aligned && (ld * sizeof(T)) % (8 * sizeof(T)) == 0;
         SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_rows_kernel<T, NV>, dim3((unsigned)(rows < 0x7FFFFFFF ? rows : 0x7FFFFFFF)),
                                               dim3((unsigned)(threads < kFp4Threads ? threads : kFp4Threads)), 0, ctx->stream, pdl, x, rows, cols, ld,
-                                              vec_ok, (const float *)g, (const float *)partials, n_partials, g, blocks, codes, scales));
+                                              vec_ok, g, source, blocks, codes, scales));
     }
     ctx->launches += 1;
     SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
@@ -48,11 +60,11 @@ int quantize_as(shrewq_ctx *ctx, const T *x, size_t rows, size_t cols, size_t ld
 }
 
 template <typename T>
-int quantize_format(shrewq_ctx *ctx, const void *x, size_t rows, size_t cols, size_t ld, bool nv, float *g, bool find_g, void *codes, void *scales) {
+int quantize_format(shrewq_ctx *ctx, const void *x, size_t rows, size_t cols, size_t ld, bool nv, float *g, int find_g, void *codes, void *scales) {
     uint32_t *c = static_cast<uint32_t *>(codes);
     uint8_t *s = static_cast<uint8_t *>(scales);
     return nv ? quantize_as<T, true>(ctx, static_cast<const T *>(x), rows, cols, ld, g, find_g, c, s)
-              : quantize_as<T, false>(ctx, static_cast<const T *>(x), rows, cols, ld, nullptr, false, c, s);
+              : quantize_as<T, false>(ctx, static_cast<const T *>(x), rows, cols, ld, nullptr, 0, c, s);
 }
 
 template <typename T, bool NV>
@@ -80,23 +92,15 @@ int dequantize_format(shrewq_ctx *ctx, const void *codes, const void *scales, co
     return nv ? dequantize_as<T, true>(ctx, c, s, g, rows, cols, static_cast<T *>(out)) : dequantize_as<T, false>(ctx, c, s, nullptr, rows, cols, static_cast<T *>(out));
 }
 
-__global__ void fill_f32_kernel(float *p, float v) { *p = v; }
-
 }  // namespace
 
-int launch_fill_f32(shrewq_ctx *ctx, float *p, float v) {
-    fill_f32_kernel<<<1, 1, 0, ctx->stream>>>(p, v);
-    ctx->launches += 1;
-    SHREWQ_CUDA_TRY(ctx, cudaGetLastError());
-    return SHREWQ_OK;
-}
-
-// x: [rows][cols] with a row stride of ld elements.  g (NV): the tensor scale, read, or found and written where find_g is set
-int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows, size_t cols, size_t ld, bool nv, float *g, bool find_g,
+// x: [rows][cols] with a row stride of ld elements.  g (NV): the tensor scale, read, or found and written where find_g is set: the words at g, of
+// which those behind the first are workspace
+int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows, size_t cols, size_t ld, bool nv, float *g, int find_g,
                         void *codes, void *scales) {
     if (rows * cols == 0) {
         // an empty tensor has no largest value: the scale that a tensor of zeros gets
-        if (nv && find_g) return launch_fill_f32(ctx, g, 1.0f);
+        if (nv && find_g) return fill_f32(ctx, g, 1.0f);
         return SHREWQ_OK;
     }
     if (x_dtype == SHREWQ_F32) return quantize_format<float>(ctx, x, rows, cols, ld, nv, g, find_g, codes, scales);

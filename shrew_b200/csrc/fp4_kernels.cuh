@@ -30,7 +30,6 @@ namespace shrewq {
 namespace {
 
 constexpr int kFp4Threads = 256;
-constexpr int kFp4MaxPartials = 2048;  // blocks of the pass that finds a tensor's amax
 constexpr uint32_t kE4m3One = 0x38, kE4m3Nan = 0x7F, kE8m0One = 127, kE8m0Nan = 255;
 
 // Eight values of a thread.  load_vec8: 16-byte aligned (32 for f32); load_guarded8: element by element, zero beyond `left`.
@@ -134,11 +133,14 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
     return __uint_as_float(b == 0 ? 0x00400000u : b == 255u ? 0x7FFFFFFFu : b << 23);
 }
 
-// ---- the tensor's amax (NV without a given scale) --------------------------------------------------------------------------
-// partials[block] = largest finite magnitude of the values that the block saw; the quantizing kernel takes the maximum of them.
+// ---- the tensor's scale (NV where it is not given) ------------------------------------------------------------------------------
+// The scale that the largest finite magnitude asks for is the largest of the scales that the magnitudes of parts ask for, since it grows with the
+// magnitude; 0 stands for a part of zeros.  The memory is the call's own, so that calls on other streams and replays of captured ones cannot meet:
+// either a word behind g for every block, of which each block of the quantizing kernel takes the maximum, or g alone, which is 0 before and
+// which the blocks raise (positive floats are ordered as their words are): a launch more, for the zero.  One block writes g as it is.
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_amax_kernel(const T *x, size_t rows, size_t cols, size_t ld, float *__restrict__ partials) {
+fp4_tensor_scale_kernel(const T *x, size_t rows, size_t cols, size_t ld, float *g, int parts) {
     pdl_launch_dependents();
     pdl_wait();
     float amax = 0.0f;
@@ -182,35 +184,45 @@ fp4_amax_kernel(const T *x, size_t rows, size_t cols, size_t ld, float *__restri
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kFp4Threads / 32; ++w) amax = fmaxf(amax, s_max[w]);
-        partials[blockIdx.x] = amax;
+        const float mine = amax > 0.0f ? fp4_tensor_scale(amax) : 0.0f;
+        if (parts) g[1 + blockIdx.x] = mine;
+        else if (gridDim.x == 1) *g = mine;
+        else if (mine > 0.0f) atomicMax(reinterpret_cast<unsigned int *>(g), __float_as_uint(mine));
     }
 }
 
-// The tensor scale for every thread of a block: read, or from the partial maxima (block 0 then writes it to g_out)
-__device__ __forceinline__ float fp4_block_tensor_scale(const float *g_in, const float *partials, int n_partials, float *g_out, int threads) {
-    if (!partials) return *g_in;
+// The tensor scale for every thread of a block.  source: kScaleGiven, read; else found by the kernel before, and 1 where that found nothing but
+// zeros: kScaleFound in g itself (block 0 then writes the 1; who reads the word before and who reads it after takes it for 1 alike), else in as
+// many words behind g (block 0 writes g).
+constexpr int kScaleGiven = 0, kScaleFound = -1;
+__device__ __forceinline__ float fp4_read_tensor_scale(float *g, int source, int threads) {
+    if (source <= 0) {
+        const float v = __uint_as_float((uint32_t)ld_written_s32(reinterpret_cast<const int *>(g)));
+        if (source == kScaleGiven || v != 0.0f) return v;
+        if (blockIdx.x == 0 && threadIdx.x == 0) *g = 1.0f;
+        return 1.0f;
+    }
     __shared__ float s_part[32];
     float m = 0.0f;
-    for (int i = threadIdx.x; i < n_partials; i += threads) m = fmaxf(m, partials[i]);
+    for (int i = threadIdx.x; i < source; i += threads) m = fmaxf(m, g[1 + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = m;
     __syncthreads();
     m = s_part[0];
     for (int w = 1; w < threads / 32; ++w) m = fmaxf(m, s_part[w]);
-    const float g = fp4_tensor_scale(m);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *g_out = g;
-    return g;
+    m = m == 0.0f ? 1.0f : m;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g = m;
+    return m;
 }
 
 // ---- quantize: rows that are whole aligned 32s, one after the other: a flat stream of groups of 8 ------------------------------
-// U groups a thread, requested before the first is used (and before the tensor's scale is made from the partial maxima: that costs a block
-// some 2000 cycles, so where there are partial maxima the grid is no more than what is resident).  The chunks go through the tensor from its end where a pass before this one
-// has read it from the front (BACK): what that pass left in L2 is read first.
+// U groups a thread, requested before the first is used (and before the tensor's scale is put together, which costs a block some 2000 cycles where
+// it is in parts, so that the grid is no more than what is resident then).  Where a pass before this one has found the scale, reading the tensor
+// from the front, the chunks go through it from its end: what that pass left in L2 is read first.
 template <typename T, bool NV, int U>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_quantize_flat_kernel(const T *x, size_t groups, const float *g_in, const float *partials, int n_partials, float *g_out,
-                         uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+fp4_quantize_flat_kernel(const T *x, size_t groups, float *g, int source, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
     const size_t chunks = (groups + kFp4Threads * U - 1) / (kFp4Threads * U);
@@ -226,10 +238,10 @@ fp4_quantize_flat_kernel(const T *x, size_t groups, const float *g_in, const flo
             }
         }
     };
-    auto base_of = [&](size_t chunk) { return (partials ? chunks - 1 - chunk : chunk) * (size_t)(kFp4Threads * U) + threadIdx.x; };
+    auto base_of = [&](size_t chunk) { return (source != kScaleGiven ? chunks - 1 - chunk : chunk) * (size_t)(kFp4Threads * U) + threadIdx.x; };
     load(base_of(blockIdx.x));
     float inv_g = 1.0f;
-    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_block_tensor_scale(g_in, partials, n_partials, g_out, kFp4Threads));
+    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_read_tensor_scale(g, source, kFp4Threads));
     for (size_t chunk = blockIdx.x;;) {
         const size_t base = base_of(chunk);
 #pragma unroll
@@ -262,12 +274,12 @@ __device__ __forceinline__ size_t scale_piece_offset(size_t row, size_t block, s
 // A CTA a row at a time.  vec_ok: rows start on 16-byte (f32: 32-byte) boundaries.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(kFp4Threads)
-fp4_quantize_rows_kernel(const T *x, size_t rows, size_t cols, size_t ld, int vec_ok, const float *g_in, const float *partials,
-                         int n_partials, float *g_out, size_t blocks_out, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+fp4_quantize_rows_kernel(const T *x, size_t rows, size_t cols, size_t ld, int vec_ok, float *g, int source, size_t blocks_out,
+                         uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
     float inv_g = 1.0f;
-    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_block_tensor_scale(g_in, partials, n_partials, g_out, (int)blockDim.x));
+    if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_read_tensor_scale(g, source, (int)blockDim.x));
     constexpr int kShift = NV ? 1 : 2;                  // groups of 8 in a block, as a power of two
     const size_t words = (cols + 31) / 32 * 4;          // words of codes in a row
     const size_t groups = blocks_out << kShift;         // >= words

@@ -491,9 +491,13 @@ PyObject *quantize_fp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
         at::Tensor codes = empty(code_shape, at::kByte, device), scales = empty(scale_shape, at::kByte, device), whole;
         float *gp = nullptr;
         const bool find = nv && args[2] == Py_None;
-        if (find) {
-            whole = empty(1, at::kFloat, device);
+        int words = 0;
+        if (find) {  // (behind the scale a word for every 1024 groups of 8, where there are more: a launch less)
+            const int64_t parts = (rc_.rows * ((rc_.cols + 7) / 8) + 1023) / 1024;
+            words = parts > 1 ? (int)std::min<int64_t>(2048, parts + 1) : 1;
+            whole = empty(words, at::kFloat, device);
             gp = static_cast<float *>(whole.data_ptr());
+            if (words > 1) whole.unsafeGetTensorImpl()->set_sizes_contiguous(1);  // (the caller sees the scale)
         } else if (args[2] != Py_None) {
             gp = static_cast<float *>(tensor_scale_arg(args[2], device, "quantize_fp4"));
         }
@@ -502,7 +506,7 @@ PyObject *quantize_fp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
         uint8_t *cp = static_cast<uint8_t *>(codes.data_ptr()), *sp = static_cast<uint8_t *>(scales.data_ptr());
         int rc;
         Py_BEGIN_ALLOW_THREADS
-        rc = L.quantize_fp4(ctx, wp, wt, (size_t)rc_.rows, (size_t)rc_.cols, (size_t)ld, format, gp, find ? 1 : 0, cp, sp);
+        rc = L.quantize_fp4(ctx, wp, wt, (size_t)rc_.rows, (size_t)rc_.cols, (size_t)ld, format, gp, words, cp, sp);
         Py_END_ALLOW_THREADS
         check(rc, ctx);
         PyObject *go;

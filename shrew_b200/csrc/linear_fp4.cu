@@ -63,11 +63,12 @@ int shrewq_quantize_fp4(shrewq_ctx *ctx, const void *w_dev, int w_dtype, size_t 
     if (ldw < cols) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: ldw (%zu) smaller than cols (%zu)", ldw, cols);
     if (nv && !tensor_scale_dev) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: SHREWQ_FP4_NV needs tensor_scale_dev");
     if (!nv && tensor_scale_dev) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: SHREWQ_FP4_MX has no tensor scale");
+    if (find_tensor_scale < 0) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: find_tensor_scale is 0 or a number of f32");
     if (misaligned(tensor_scale_dev, 4) || misaligned(w_dev, size_of(w_dtype)) || misaligned(codes_dev, 4))
         return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: w_dev aligned to its elements, tensor_scale_dev and codes_dev to 4 bytes");
     if (rows * cols != 0 && (!w_dev || !codes_dev || !scales_dev)) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "quantize_fp4: NULL buffer");
     SHREWQ_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
-    return launch_quantize_fp4(ctx, w_dev, w_dtype, rows, cols, ldw, nv, tensor_scale_dev, find_tensor_scale != 0, codes_dev, scales_dev);
+    return launch_quantize_fp4(ctx, w_dev, w_dtype, rows, cols, ldw, nv, tensor_scale_dev, find_tensor_scale, codes_dev, scales_dev);
 }
 
 int shrewq_dequantize_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev, size_t rows, size_t cols,

@@ -68,8 +68,7 @@ inline int split_over_cluster(size_t tiles, int rounds, int room, int min_rounds
 // pieces of 128 rows by 4 blocks along a row, out to whole 256 columns
 inline size_t fp4_pieces(size_t K, bool nv) { return (K + 255) / 256 * (nv ? 4 : 2); }
 
-int launch_fill_f32(shrewq_ctx *ctx, float *p, float v);
-int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows, size_t cols, size_t ld, bool nv, float *g, bool find_g,
+int launch_quantize_fp4(shrewq_ctx *ctx, const void *x, int x_dtype, size_t rows, size_t cols, size_t ld, bool nv, float *g, int find_g,
                         void *codes, void *scales);
 int launch_dequantize_fp4(shrewq_ctx *ctx, const void *codes, const void *scales, const float *g, size_t rows, size_t cols, bool nv, int out_dtype, void *out);
 int launch_fp4_scale_pieces(shrewq_ctx *ctx, const uint8_t *scales, const float *g, size_t N, size_t blocks, size_t pieces, bool nv, uint8_t *out,

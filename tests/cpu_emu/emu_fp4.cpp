@@ -10,25 +10,25 @@ using namespace shrewq;
 namespace {
 
 template <typename T, bool NV>
-void quantize(const void *x, size_t rows, size_t cols, size_t ld, float *g, bool find, int route, unsigned grid, void *codes, void *scales) {
+void quantize(const void *x, size_t rows, size_t cols, size_t ld, float *g, int find, int route, unsigned grid, void *codes, void *scales) {
     const T *p = static_cast<const T *>(x);
     uint32_t *c = static_cast<uint32_t *>(codes);
     uint8_t *s = static_cast<uint8_t *>(scales);
-    std::vector<float> partials(grid);
-    const float *pp = NV && find ? partials.data() : nullptr;
-    if (pp) {
-        if (route == 0) emu::launch(grid, kFp4Threads, [&] { fp4_amax_kernel<T, true>(p, rows, cols, ld, partials.data()); });
-        else emu::launch(grid, kFp4Threads, [&] { fp4_amax_kernel<T, false>(p, rows, cols, ld, partials.data()); });
+    const int source = !(NV && find) ? kScaleGiven : (unsigned)find > grid ? (int)grid : kScaleFound;
+    if (source != kScaleGiven) {
+        if (source == kScaleFound && grid > 1) *g = 0.0f;
+        if (route == 0) emu::launch(grid, kFp4Threads, [&] { fp4_tensor_scale_kernel<T, true>(p, rows, cols, ld, g, source > 0); });
+        else emu::launch(grid, kFp4Threads, [&] { fp4_tensor_scale_kernel<T, false>(p, rows, cols, ld, g, source > 0); });
     }
     if (route == 0) {
         const size_t groups = rows * cols / 8;
         emu::launch((unsigned)((groups + kFp4Threads * 4 - 1) / (kFp4Threads * 4)), kFp4Threads,
-                    [&] { fp4_quantize_flat_kernel<T, NV, 4>(p, groups, g, pp, (int)grid, g, c, s); });
+                    [&] { fp4_quantize_flat_kernel<T, NV, 4>(p, groups, g, source, c, s); });
     } else {
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = (reinterpret_cast<uintptr_t>(p) % (8 * sizeof(T))) == 0 && ld % 8 == 0;
         emu::launch((unsigned)std::min<size_t>(rows, 3), (unsigned)std::min<size_t>(threads, kFp4Threads), [&] {
-            fp4_quantize_rows_kernel<T, NV>(p, rows, cols, ld, vec_ok, g, pp, (int)grid, g, blocks, c, s);
+            fp4_quantize_rows_kernel<T, NV>(p, rows, cols, ld, vec_ok, g, source, blocks, c, s);
         });
     }
 }

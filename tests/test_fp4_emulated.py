@@ -96,6 +96,21 @@ def test_a_given_tensor_scale(emu, g):
     np.testing.assert_array_equal(unsigned_zeros(codes.numpy()), unsigned_zeros(want[0]))
 
 
+@pytest.mark.parametrize("grid,words", [(1, 1), (3, 1), (3, 3), (1, 2), (3, 4), (40, 64)])
+@pytest.mark.parametrize("route", [0, 1])
+def test_the_scale_of_small_and_of_zero_tensors(emu, route, grid, words):
+    """In its own word and with words for the blocks' parts behind it."""
+    x = aligned((5, 64), torch.float32)
+    for top in (0.0, 1e-44, 2688.0, 2689.0, 3e38):
+        x[3, 7] = top
+        codes, scales, whole = aligned((5, 32), torch.uint8), aligned((5, 4), torch.uint8), torch.full((words + 1,), -5.0)
+        assert emu.emu_fp4_quantize(x.data_ptr(), 0, 5, 64, 64, 1, whole.data_ptr(), words, route, grid, codes.data_ptr(), scales.data_ptr()) == 0
+        want = O.quantize(x.double().numpy(), True)
+        assert float(whole[0]) == want[2] and float(whole[words]) == -5.0
+        np.testing.assert_array_equal(scales.numpy(), want[1])
+        np.testing.assert_array_equal(unsigned_zeros(codes.numpy()), unsigned_zeros(want[0]))
+
+
 def test_rows_with_a_stride(emu):
     wide = special(6, 200, torch.bfloat16, 3)
     for view in (wide[:, 8:72], wide[:, 1:100]):

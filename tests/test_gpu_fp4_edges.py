@@ -1,0 +1,90 @@
+"""GPU: calls of the 4-bit operators that meet other calls: other quantizers of the context, captured graphs beside eager calls, values at the
+ends of their ranges.  Through the package's public entry points, against the definitions in 64 bits (tests/fp4_oracle.py)."""
+import numpy as np
+import pytest
+import torch
+
+from shrew_b200 import Fp4Format, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor
+from shrew_b200 import _lib
+from shrew_b200.quantize import Device
+from tests import fp4_oracle as O
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def same(a, b):
+    return torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) and torch.equal(a.tensor_scale, b.tensor_scale)
+
+
+# ---- the tensor's scale ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("config", [QuantConfig.int8(), QuantConfig.int4()])
+def test_tensor_scales_leave_the_other_quantizers_alone(oracle, config):
+    """Large NV tensors, more of them than a context has slots for per-tensor quantizing, then per-tensor integers of several blocks each."""
+    g = torch.Generator().manual_seed(0)
+    big = torch.randn(512, 2048, generator=g).cuda()
+    small = [(torch.randn(300, 1000, generator=g) * (i + 1)).cuda() for i in range(9)]
+    before = [quantize_tensor(x, config) for x in small]
+    for i in range(17):
+        quantize_fp4(big * (i + 1), Fp4Format.Nv)
+    for x, b in zip(small, before):
+        q = quantize_tensor(x, config)
+        assert torch.equal(q.data, b.data) and torch.equal(q.scales, b.scales)
+        assert float(q.scales[0]) == float(x.abs().max().double()) / (127.0 if config.bits.name == "Int8" else 7.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_tensor_scales_of_calls_in_flight_together(dtype):
+    """A captured call replayed on one stream while eager calls run on another, and eager calls on many streams: every tensor gets its own scale."""
+    g = torch.Generator().manual_seed(1)
+    xs = [(torch.randn(300, 1024, generator=g) * 2.0 ** (3 * i - 12)).to(dtype).cuda() for i in range(9)]
+    want = [quantize_fp4(x, Fp4Format.Nv) for x in xs]
+    assert len({float(w.tensor_scale) for w in want}) == len(xs)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        captured = quantize_fp4(xs[-1], Fp4Format.Nv)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            for _ in range(40):
+                graph.replay()
+        got += [quantize_fp4(x, Fp4Format.Nv) for x in xs]
+    torch.cuda.synchronize()
+    assert same(captured, want[-1])
+    assert all(same(q, want[i % len(xs)]) for i, q in enumerate(got))
+    streams = [torch.cuda.Stream() for _ in range(24)]
+    got = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got.append(quantize_fp4(xs[i % len(xs)], Fp4Format.Nv))
+    torch.cuda.synchronize()
+    assert all(same(q, want[i % len(xs)]) for i, q in enumerate(got))
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (3, 40), (64, 64), (2000, 1024)])
+def test_the_scale_of_nothing_but_zeros(shape):
+    x = torch.zeros(shape, device="cuda")
+    x[0, 0] = float("nan")   # (finite values count)
+    q = quantize_fp4(x, Fp4Format.Nv)
+    assert float(q.tensor_scale) == 1.0
+    codes, scales, _, _ = O.quantize(x.double().cpu().numpy(), True)
+    np.testing.assert_array_equal(q.scales.cpu().numpy(), scales)
+    assert (dequantize_fp4(q).nan_to_num(0.0) == 0.0).all()
+
+
+@pytest.mark.parametrize("words", [1, 2, 30, 92, 93, 2048])
+def test_words_for_finding_a_scale(words):
+    """As many as the caller gives (at 93 the parts of all 92 blocks fit): the same result, and nothing behind them is written."""
+    x = torch.randn(367, 1024, generator=torch.Generator().manual_seed(3)).cuda()
+    x[200, 5] = 1e4
+    want = quantize_fp4(x, Fp4Format.Nv)
+    whole = torch.full((words + 3,), -5.0, device="cuda")
+    codes, scales = torch.empty_like(want.codes), torch.empty_like(want.scales)
+    dev = Device.get(x.device)
+    dev.bind_stream()
+    args = (dev.handle, x.data_ptr(), _lib.F32, 367, 1024, 1024, _lib.FP4_NV, whole.data_ptr())
+    assert _lib.lib().shrewq_quantize_fp4(*args, words, codes.data_ptr(), scales.data_ptr()) == _lib.OK
+    assert float(whole[0]) == float(want.tensor_scale) == O.quantize(x.double().cpu().numpy(), True)[2]
+    assert torch.equal(codes, want.codes) and torch.equal(scales, want.scales) and (whole[words:] == -5.0).all()
+    assert _lib.lib().shrewq_quantize_fp4(*args, -1, codes.data_ptr(), scales.data_ptr()) == _lib.ERR_INVALID_ARG
