@@ -277,7 +277,7 @@ SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_
  *   quantize_activations = 0: y = x . dequant(W)^T + bias with f32 sums of exact products.  bf16 activations smaller than 2^-64 of the
  *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens.
  *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
- *     positive number, as the tensor scale), and codes are multiplied by codes on the block-scaled tensor cores.
+ *     positive number, as the tensor scale, which is not used otherwise), and codes are multiplied by codes on the block-scaled tensor cores.
  * Workspaces of the context (see shrewq_ctx_set_stream): quantize_activations = 1 always, for the codes; else 5 to 32 tokens, and above 32
  * f32 activations and bf16 ones whose rows are not whole 16-byte pieces, for a staged copy.
  */

@@ -122,7 +122,7 @@ int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const ui
     w->codes = codes_dev;
     w->nv = nv;
     w->round_x = quantize_activations != 0;
-    w->x_scale = nv ? activation_scale : 1.0f;
+    w->x_scale = nv && w->round_x ? activation_scale : 1.0f;  // (activations as they come have none)
     const size_t pieces = fp4_pieces(in_features, nv), bytes = (out_features + 127) / 128 * pieces * 512;
     if (cudaMalloc(&w->pieces, bytes) != cudaSuccess || cudaMalloc(&w->params, sizeof(Fp4Params)) != cudaSuccess ||
         cudaMalloc(&lin->scales_f32, out_features * sizeof(float)) != cudaSuccess) {

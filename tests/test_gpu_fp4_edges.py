@@ -4,10 +4,11 @@ import numpy as np
 import pytest
 import torch
 
-from shrew_b200 import Fp4Format, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor
+from shrew_b200 import Fp4Format, Fp4Linear, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor
 from shrew_b200 import _lib
 from shrew_b200.quantize import Device
 from tests import fp4_oracle as O
+from tests.test_gpu_fp4 import acts, layer
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -88,3 +89,15 @@ def test_words_for_finding_a_scale(words):
     assert float(whole[0]) == float(want.tensor_scale) == O.quantize(x.double().cpu().numpy(), True)[2]
     assert torch.equal(codes, want.codes) and torch.equal(scales, want.scales) and (whole[words:] == -5.0).all()
     assert _lib.lib().shrewq_quantize_fp4(*args, -1, codes.data_ptr(), scales.data_ptr()) == _lib.ERR_INVALID_ARG
+
+
+# ---- layers -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [0.0, 0.5, -3.0, float("nan")])
+@pytest.mark.parametrize("m", [1, 4, 8, 20, 40, 200])
+def test_activations_as_they_come_have_no_scale(m, scale):
+    gate, _, _ = layer(136, 320, Fp4Format.Nv, 1)
+    up, _, _ = layer(136, 320, Fp4Format.Nv, 2)
+    gate_s, up_s = Fp4Linear(gate.weight_q, gate.bias, activation_scale=scale), Fp4Linear(up.weight_q, up.bias, activation_scale=scale + 1.0)
+    for x in (acts(m, 320, BF16), acts(m, 320, F32)):
+        assert torch.equal(gate_s.forward(x), gate.forward(x))
+        assert torch.equal(gate_s.forward_gate_up_silu(up_s, x), gate.forward_gate_up_silu(up, x))
