@@ -100,7 +100,7 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             mbar_init(bars + kAfreeBar + s * 8, 1);
         }
         mbar_init(bars + kAccBar, 1);
-        mbar_init(bars + kTakenBar, 4);
+        mbar_init(bars + kTakenBar, 4 * kH4Groups);
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -176,7 +176,7 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         bool good = true;
         if (elect_one()) {
             for (int pass = 0; pass < passes && good; ++pass) {
-                // the sums of the pass before have been taken out
+                // the sums of the pass before have been taken out, and every converter warp has seen them complete
                 if (pass > 0) good = mbar_wait_close<kTimeoutH4>(bars + kTakenBar, (uint32_t)(pass - 1) & 1u, ctl, status, 5, 0);
                 for (int i = 0; i < rounds && good; ++i) {
                     // (the converters have waited for the stage: its activations are there too)
@@ -210,7 +210,7 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
             const int first = top - (kMxWindow - 1) - kMxWindow * (pass % windows);  // MX: the byte of 2^-14 in this window
             for (int i = 0; i < rounds; ++i, ++item) {
                 // group g takes the items i % 3 == g, and so, the ring being a multiple, always the same stages and place: it passes through
-                // every phase of the barriers that it polls, so that a wait for a parity cannot take one phase for another
+                // every phase of their barriers, so that a wait for a parity cannot take one phase for another
                 const int slot = item % C::kSlots, s = item % C::kStages;
                 if (slot != group) continue;
                 mbar_wait_all<kTimeoutH4>(bars + kFullBar + s * 8, (uint32_t)(item / C::kStages) & 1u, ctl, status, 3, s);
@@ -263,8 +263,10 @@ gemm_w4_f16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0 && !last) mbar_arrive(bars + kTakenBar);
                 }
+                // Every warp, so that none can miss a phase of the accumulators' barrier: a group without an item in some passes (a round or
+                // two of them) would otherwise be held back by nothing, and two phases later its parity reads as if none had been.
+                if (lane == 0 && pass + 1 < passes) mbar_arrive(bars + kTakenBar);
                 if (pass + 1 == passes) {
                     named_bar_sync(1, 128 * kH4Groups);
                     tc_fence_after();

@@ -76,7 +76,21 @@ inline void mma_fp4(Block *blk, bool nv, uint32_t d_tmem, uint64_t a_desc, uint6
 }
 }  // namespace emu
 
-static inline bool mbar_test(uint32_t bar, uint32_t parity) { return mbar_try(bar, parity); }
+// Threads of the warps from this one on come so many milliseconds late to their first look at a barrier (-1 = none)
+namespace emu {
+inline std::atomic<int> g_late_warp{-1}, g_late_ms{0};
+inline void come_late() {
+    static thread_local bool been = false;
+    if (been || g_late_warp.load() < 0 || (int)(threadIdx.x >> 5) < g_late_warp.load()) return;
+    been = true;
+    std::this_thread::sleep_for(std::chrono::milliseconds(g_late_ms.load()));
+}
+}  // namespace emu
+extern "C" inline __attribute__((used, visibility("default"))) void emu_late_warps(int first, int ms) { emu::g_late_warp = first, emu::g_late_ms = ms; }
+static inline bool mbar_test(uint32_t bar, uint32_t parity) {
+    emu::come_late();
+    return mbar_try(bar, parity);
+}
 static inline void tc_cp_scales(uint32_t taddr, uint64_t desc) {
     if (emu::tc_deferred()) emu::tc_push([=] { emu::cp_scales(emu::g_block, taddr, desc); });
     else emu::cp_scales(emu::g_block, taddr, desc);

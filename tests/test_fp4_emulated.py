@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import fp4_oracle as O
-from tests.test_cpu_emulated_kernels import _build
+from tests.test_cpu_emulated_kernels import _build, _build_short_waits
 
 _vp, _sz, _ci, _cu, _cf = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint, ctypes.c_float
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -331,3 +331,36 @@ def test_four_bit_weights_on_the_tensor_cores(emu_gemm, nv, M, N, K, tok, x_dtyp
     up = wd[1] if gated else None
     want = O.product(xd, wd[0], biases[0].numpy(), up=up, relu=not gated and N % 2 == 1)
     assert (np.abs(y[:, :N].double().numpy() - want) <= O.product_bound(xd, wd[0], K, up=up, bias=biases[0].numpy())).all()
+
+
+@pytest.mark.parametrize("nv,K,x_dtype,spread", [(False, 96, torch.float32, 3), (True, 128, torch.float32, 0), (False, 256, torch.float32, 3), (False, 96, torch.bfloat16, 100),
+                                                 (False, 200, torch.float32, 40)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.timeout(120)
+def test_converters_that_come_late_to_a_pass(nv, K, x_dtype, spread, gated):
+    """Several passes (terms of f32 activations, windows of scales) of a round or two: the warps that have nothing to convert in the first passes
+    look at the accumulators' barrier long after those passes could be done."""
+    L = _build_short_waits("emu_gemm_fp4", ("-DSHREWQ_SPIN_FAST_LIMIT=64", "-DSHREWQ_SPIN_SLOW_LIMIT=10000"), "second_waits")
+    L.emu_gemm_w4_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _ci, _cu]
+    M, N = 9, 30
+    g = torch.Generator().manual_seed(K)
+    x = aligned((M, K), x_dtype)
+    x.copy_(torch.randn(M, K, generator=g))
+    ws = [stored(N, K, nv, i, spread=spread) for i in range(2 if gated else 1)]
+    for w in ws:
+        w[2].fill_(2.0 ** -9 if nv else 1.0)
+    bias = torch.randn(N, generator=g)
+    y = torch.full((M, N), -77.0)
+    table = lambda ts: (ctypes.c_void_p * 2)(*[None if t is None else t.data_ptr() for t in (list(ts) * 2)[:2]])  # noqa: E731
+    try:
+        for first in (10, 6, 2):   # the third group of converters, then more of them
+            L.emu_late_warps(first, 150)
+            rc = L.emu_gemm_w4_bf16(table([w[0] for w in ws]), table([w[1] for w in ws]), table([w[2] for w in ws]), table([bias]), x.data_ptr(), int(x_dtype is torch.float32),
+                                    M, N, K, 16, int(nv), int(gated), y.data_ptr(), N, 0, 0, 0)
+            assert rc == 0
+            xd, wd = x.double().numpy(), [O.dequantize(w[0].numpy(), w[1].numpy(), 2.0 ** -9, K, nv) for w in ws]
+            up = dict(up=wd[1], bias_up=bias.numpy()) if gated else {}
+            want, bound = O.product(xd, wd[0], bias.numpy(), **up), O.product_bound(xd, wd[0], K, bias=bias.numpy(), **up)
+            assert (np.abs(y.double().numpy() - want) <= bound).all()
+    finally:
+        L.emu_late_warps(-1, 0)
