@@ -44,7 +44,7 @@ __device__ __forceinline__ void load_vec8<float>(const float *p, float *v) {
 }
 template <>
 __device__ __forceinline__ void load_vec8<__nv_bfloat16>(const __nv_bfloat16 *p, float *v) {
-    const uint4 w = ld_stream_16(p);
+    const uint4 w = ld_once_16(p);
     const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -54,7 +54,7 @@ __device__ __forceinline__ void load_vec8<__nv_bfloat16>(const __nv_bfloat16 *p,
 }
 template <>
 __device__ __forceinline__ void load_vec8<__half>(const __half *p, float *v) {
-    const uint4 w = ld_stream_16(p);
+    const uint4 w = ld_once_16(p);
     f32x2_of_f16x2(w.x, v[0], v[1]);
     f32x2_of_f16x2(w.y, v[2], v[3]);
     f32x2_of_f16x2(w.z, v[4], v[5]);

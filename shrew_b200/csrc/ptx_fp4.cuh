@@ -62,7 +62,13 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
     return d;
 }
-// 32 bytes, read once / written once
+// 16 or 32 bytes, read once / written once.  Not through the read-only path: they may be what the kernel before in the stream writes, which may
+// still run when this one is launched early.
+__device__ __forceinline__ uint4 ld_once_16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ void ld_stream_32(const void *p, uint32_t *r) {
     asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])

@@ -293,7 +293,8 @@ static inline unsigned __byte_perm(unsigned x, unsigned y, unsigned sel) {
 }
 #define __expf expf
 static inline float __fdividef(float a, float b) { return a / b; }
-static inline uint4 ld_stream_16(const void *p) { uint4 v; memcpy(&v, p, 16); return v; }
+namespace emu { inline std::atomic<long> g_read_only_loads{0}; }  // through the read-only path: of data that nothing may write while the kernel is there
+static inline uint4 ld_stream_16(const void *p) { uint4 v; memcpy(&v, p, 16); emu::g_read_only_loads.fetch_add(1, std::memory_order_relaxed); return v; }
 static inline float ld_cg_ordered(const float *p) { return *p; }
 static inline void pdl_launch_dependents() {}   // launches are sequential here
 // Programmatic dependent launch: the previous kernel of the stream completes at this time of the steady clock

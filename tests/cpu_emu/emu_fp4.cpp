@@ -85,6 +85,8 @@ int outcome() { return emu::g_failed.exchange(false) ? -1 : 0; }
 
 }  // namespace
 
+extern "C" long emu_read_only_loads() { return emu::g_read_only_loads.exchange(0); }
+
 // route: 0 = whole aligned rows as one stream, 1 = any rows
 extern "C" int emu_fp4_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t ld, int nv, float *g, int find, int route, unsigned grid, void *codes,
                                 void *scales) {

@@ -364,3 +364,24 @@ def test_converters_that_come_late_to_a_pass(nv, K, x_dtype, spread, gated):
             assert (np.abs(y.double().numpy() - want) <= bound).all()
     finally:
         L.emu_late_warps(-1, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_inputs_of_a_stream_are_not_read_as_constant(emu, dtype):
+    """Tensors, activations, branches and gates may be the output of the kernel before, which may still run when these kernels are launched early: no
+    load of theirs goes through the read-only path, which is for data that nothing writes while the kernel is there."""
+    emu.emu_read_only_loads.restype = ctypes.c_long
+    emu.emu_read_only_loads()
+    x = special(9, 64, dtype, 1)
+    for nv in (False, True):
+        for route in (0, 1):
+            run_quantize(emu, x, nv, route=route)
+    assert emu.emu_read_only_loads() == 0
+    if dtype is torch.float16:
+        return
+    x, b, r, h = (aligned((3, 64), dtype) for _ in range(4))
+    which, w = int(dtype is torch.bfloat16), aligned((64,), torch.float32)
+    for gate_kind in (1, 3):
+        assert emu.emu_residual_norm(x.data_ptr(), b.data_ptr(), b.data_ptr(), 64, 64, 64, w.data_ptr(), None, w.data_ptr(), None, r.data_ptr(), h.data_ptr(), 3, 64, 1, 1, gate_kind,
+                                     1e-5, 1.0, 1.0, 1, which, which, which, 1, 2) == 0
+    assert emu.emu_read_only_loads() == 0
