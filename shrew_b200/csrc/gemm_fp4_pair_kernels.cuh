@@ -15,7 +15,9 @@
 // Warp roles: warp 0 = tensor-memory allocation, and in the leader the MMAs; four groups of 4 warps = epilogue, the first two of them also
 // copies, taking the stages in turn; the last warp = relay.  Copies arrive on the stage's barrier by themselves
 // (cp.async.mbarrier.arrive); the relay of each CTA waits there, makes them visible to the tensor core (fence.proxy.async) and arrives at
-// the leader.  (Arrivals with .release.cluster by the copying warps took 1200 cycles a stage.)  The accumulators, 256 columns, and the stages' scales
+// the leader, publishing them to the cluster (a fence for shared memory alone: with .release.cluster the relays' arrivals held the pair up, 165 us
+// instead of 117 for 4096 x 11008 with 4096 tokens, and by the copying warps, with copies in flight, they took 1200 cycles a stage).  The accumulators,
+// 256 columns, and the stages' scales
 // fill tensor memory, so the MMAs of the next tile wait until the sums have been read: all warps that are free then take part, after the
 // next tile's first stages are under way.
 // Measured: 4096 x 11008 MX, 4096 tokens: 85 us of 114 to 118 for the call (quantizing the tokens is the rest; 3.1 PFLOP/s over all, at 1680 MHz under the
@@ -197,12 +199,12 @@ gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restr
             for (int tile = pair; good && tile < tiles; tile += pairs, ++done) {
                 if (done > 0 && !mbar_wait_close<kTimeoutFp4Pair>(bars + kAccFreeBar, (done - 1) & 1u, ctl, status, 3, 0)) break;
                 for (int i = 0; i < rounds; ++i) {
-                    good = ready || mbar_wait_close<kTimeoutFp4Pair>(bars + kReadyBar + s * 8, ph, ctl, status, 1, s);
+                    good = ready || mbar_wait_close_cluster<kTimeoutFp4Pair>(bars + kReadyBar + s * 8, ph, ctl, status, 1, s);
                     if (!good) break;
                     tc_fence_after();
                     // (a look takes 150 to 300 cycles here: the next stage's is under way while this one's MMAs are issued)
                     const uint32_t next = s + 1 == C::kStages ? 0 : s + 1, next_ph = s + 1 == C::kStages ? ph ^ 1u : ph;
-                    ready = mbar_test(bars + kReadyBar + next * 8, next_ph);
+                    ready = mbar_test_acquire_cluster(bars + kReadyBar + next * 8, next_ph);
                     const uint32_t base = smem_base + s * C::kStageBytes, sf = tmem + kPairTok + s * C::kSfCols;
                     constexpr int kSfbCol = C::kPieces * 4;
                     const uint64_t adesc = make_b_desc(base), bdesc = make_b_desc(base + C::kBOff), sdesc = make_scale_desc(base + C::kSfaOff);
@@ -238,7 +240,7 @@ gemm_fp4_pair_kernel(const uint8_t *__restrict__ w_codes, const uint8_t *__restr
                     good = mbar_wait_close<kTimeoutFp4Pair>(bars + kFullBar + s * 8, ph, ctl, status, 5, s);
                     if (!good) break;
                     fence_proxy_async_smem();
-                    mbar_arrive_cluster(ready_leader + s * 8);
+                    mbar_arrive_release_cluster(ready_leader + s * 8);
                     if (++s == C::kStages) { s = 0; ph ^= 1; }
                 }
         }

@@ -47,6 +47,23 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uin
 }
 
 // ---- CTA pairs ----
+// Arrival on a barrier of the other CTA that publishes this CTA's shared memory, as this thread has seen it, to the cluster, and the look that goes
+// with it (an arrival without a scope orders within a CTA only).  The fence is for shared memory alone: a plain .release.cluster, which waits for
+// the thread's other memory operations too, made 4096 x 11008 with 4096 tokens 165 us instead of 117.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+    asm volatile("fence.release.sync_restrict::shared::cta.cluster;\n\tmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_test_acquire_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // tc_cp_scales in both CTAs of the pair, each from its own shared memory
 __device__ __forceinline__ void tc_cp_scales_pair(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");

@@ -32,6 +32,13 @@ __device__ __forceinline__ bool mbar_wait_close(uint32_t bar, uint32_t parity, C
         if (mbar_test(bar, parity)) return true;
     return mbar_wait_slow(bar, parity, ctl, st, role, stage, CODE);
 }
+// The same for a barrier on which the other CTA's threads arrive (mbar_arrive_release_cluster)
+template <uint32_t CODE>
+__device__ __forceinline__ bool mbar_wait_close_cluster(uint32_t bar, uint32_t parity, Ctl *ctl, DeviceStatus *st, uint32_t role, uint32_t stage) {
+    for (uint32_t i = 0; i < kSpinClose; ++i)
+        if (mbar_test_acquire_cluster(bar, parity)) return true;
+    return mbar_wait_slow(bar, parity, ctl, st, role, stage, CODE) && mbar_test_acquire_cluster(bar, parity);
+}
 // A whole warp: every lane looks (67 cycles where the phase is complete; one lane and a shuffle take 110, one lane, a shuffle and a second
 // look by all, as mbar_wait_warp_c has it, 270).  A wait that runs out raises the abort flag and the warp goes on, so that its lanes stay
 // together: what it computes then is not stored.  warp_ok() says afterwards whether anything gave up.

@@ -91,6 +91,8 @@ static inline bool mbar_test(uint32_t bar, uint32_t parity) {
     emu::come_late();
     return mbar_try(bar, parity);
 }
+static inline bool mbar_test_acquire_cluster(uint32_t bar, uint32_t parity) { return mbar_test(bar, parity); }
+static inline void mbar_arrive_release_cluster(uint32_t cluster_addr) { mbar_arrive(cluster_addr); }
 static inline void tc_cp_scales(uint32_t taddr, uint64_t desc) {
     if (emu::tc_deferred()) emu::tc_push([=] { emu::cp_scales(emu::g_block, taddr, desc); });
     else emu::cp_scales(emu::g_block, taddr, desc);
