@@ -222,7 +222,7 @@ SHREWQ_API int shrewq_dequantize_ex(shrewq_ctx *ctx, const int8_t *q_dev, const 
 #define SHREWQ_FP4_NV 1
 /*
  * w_dev: [rows, cols] of w_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), rows ldw elements apart.  codes_dev must be 4-byte aligned.
- * tensor_scale_dev: NULL for MX; for NV one f32 on the device: read if find_tensor_scale is 0 (a positive number), else written: the
+ * tensor_scale_dev: NULL for MX; for NV one f32 on the device: read if find_tensor_scale is 0 (2^-126 or more), else written: the
  * smallest power of two g with 2688 g >= the tensor's largest finite magnitude (1 for a tensor of zeros).  Finding it takes a pass over
  * the tensor of its own.  find_tensor_scale is then the number of f32 that the call may use at tensor_scale_dev: 1, or more, of which those
  * behind the first are workspace (1 + rows * ceil(cols / 8) / 1024, 2048 at most, spare a launch).  No workspace of the context: calls share nothing.

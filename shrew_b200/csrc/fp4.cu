@@ -45,8 +45,8 @@ int quantize_as(shrewq_ctx *ctx, const T *x, size_t rows, size_t cols, size_t ld
     const size_t groups = rows * cols / 8, want = (groups + kFp4Threads * U - 1) / (kFp4Threads * U);
     if (flat && want <= 0x7FFFFFFF) {
         const size_t grid = source != kScaleGiven && want > (size_t)ctx->sm_count * 6 ? (size_t)ctx->sm_count * 6 : want;
-        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(fp4_quantize_flat_kernel<T, NV, U>, dim3((unsigned)grid), dim3(kFp4Threads), 0, ctx->stream, pdl, x, groups, g,
-                                              source, codes, scales));
+        auto kern = NV && source != kScaleGiven ? fp4_quantize_flat_kernel<T, NV, !NV, U> : fp4_quantize_flat_kernel<T, NV, true, U>;
+        SHREWQ_CUDA_TRY(ctx, launch_maybe_pdl(kern, dim3((unsigned)grid), dim3(kFp4Threads), 0, ctx->stream, pdl, x, groups, g, source, codes, scales));
     } else {
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = aligned && (ld * sizeof(T)) % (8 * sizeof(T)) == 0;

@@ -92,20 +92,33 @@ __device__ __forceinline__ float recip_e4m3_rn(float s) {
 }
 
 // One thread's part of a block: v[8] -> a word of codes and the block's scale byte (the same in all lanes of the block).  Every lane of
-// the warp takes part in the shuffles.
-template <bool NV>
+// the warp takes part in the shuffles.  GIVEN (NV): a tensor scale that was not found from the tensor may take finite values beyond f32; they
+// saturate.  (A scale that was found does not, and the test for it costs 2 of 62 us in the round trip of 11008 x 4096.)
+template <bool NV, bool GIVEN>
 __device__ __forceinline__ uint32_t fp4_encode(float *v, float inv_g, uint32_t &byte) {
-    if constexpr (NV) {
+    auto scale_values = [&] {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) mul_f32x2(v[i], v[i + 1], inv_g, v[i], v[i + 1]);
-    }
+    };
+    if constexpr (NV && !GIVEN) scale_values();
     float amax = max_abs_nan(v[0], v[1]);
 #pragma unroll
     for (int i = 2; i < 8; i += 2) amax = max_abs_nan(amax, max_abs_nan(v[i], v[i + 1]));
     amax = max_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
     if constexpr (!NV) amax = max_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-    const bool bad = !(amax < __uint_as_float(0x7F800000u));
+    const float inf = __uint_as_float(0x7F800000u);
+    const bool bad = !(amax < inf);
     if constexpr (NV) {
+        if constexpr (GIVEN) {
+            amax *= inv_g;  // (what the largest of the products below is: rounding keeps their order)
+            scale_values();
+            if (amax == inf && !bad) {
+                const float most = __uint_as_float(0x7F7FFFFFu);
+                amax = most;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
+            }
+        }
         byte = amax == 0.0f ? kE4m3One : cvt_e4m3(fminf(fmaxf(div6_rn(amax), 0.001953125f), 448.0f));
         float s, unused;
         f32x2_of_f16x2(cvt_f16x2_e4m3(byte), s, unused);
@@ -219,8 +232,8 @@ __device__ __forceinline__ float fp4_read_tensor_scale(float *g, int source, int
 // ---- quantize: rows that are whole aligned 32s, one after the other: a flat stream of groups of 8 ------------------------------
 // U groups a thread, requested before the first is used (and before the tensor's scale is put together, which costs a block some 2000 cycles where
 // it is in parts, so that the grid is no more than what is resident then).  Where a pass before this one has found the scale, reading the tensor
-// from the front, the chunks go through it from its end: what that pass left in L2 is read first.
-template <typename T, bool NV, int U>
+// from the front (not GIVEN), the chunks go through it from its end: what that pass left in L2 is read first.
+template <typename T, bool NV, bool GIVEN, int U>
 __global__ void __launch_bounds__(kFp4Threads)
 fp4_quantize_flat_kernel(const T *x, size_t groups, float *g, int source, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     pdl_launch_dependents();
@@ -238,7 +251,7 @@ fp4_quantize_flat_kernel(const T *x, size_t groups, float *g, int source, uint32
             }
         }
     };
-    auto base_of = [&](size_t chunk) { return (source != kScaleGiven ? chunks - 1 - chunk : chunk) * (size_t)(kFp4Threads * U) + threadIdx.x; };
+    auto base_of = [&](size_t chunk) { return (GIVEN ? chunk : chunks - 1 - chunk) * (size_t)(kFp4Threads * U) + threadIdx.x; };
     load(base_of(blockIdx.x));
     float inv_g = 1.0f;
     if constexpr (NV) inv_g = __fdiv_rn(1.0f, fp4_read_tensor_scale(g, source, kFp4Threads));
@@ -248,7 +261,7 @@ fp4_quantize_flat_kernel(const T *x, size_t groups, float *g, int source, uint32
         for (int u = 0; u < U; ++u) {
             const size_t i = base + (size_t)u * kFp4Threads;
             uint32_t byte;
-            const uint32_t word = fp4_encode<NV>(v[u], inv_g, byte);
+            const uint32_t word = fp4_encode<NV, GIVEN>(v[u], inv_g, byte);
             if (i < groups) {
                 codes[i] = word;
                 if constexpr (NV) {
@@ -291,7 +304,7 @@ fp4_quantize_rows_kernel(const T *x, size_t rows, size_t cols, size_t ld, int ve
             if (vec_ok && i * 8 + 8 <= cols) load_vec8<T>(src + i * 8, v);
             else load_guarded8<T>(src + i * 8, i * 8 < cols ? cols - i * 8 : 0, v);
             uint32_t byte;
-            const uint32_t word = fp4_encode<NV>(v, inv_g, byte);
+            const uint32_t word = fp4_encode<NV, true>(v, inv_g, byte);
             if (i < words) codes[row * words + i] = word;
             if (i < groups && (i & ((1 << kShift) - 1)) == 0) scales[row * blocks_out + (i >> kShift)] = (uint8_t)byte;
         }
@@ -331,7 +344,7 @@ fp4_quantize_acts_kernel(const T *x, size_t rows, uint32_t cols, int vec_ok, con
                 const uint32_t run = u + k * warps, i = run * 32 + lane;
                 if (k == 1 && run >= units) break;
                 uint32_t byte;
-                const uint32_t word = fp4_encode<NV>(v[k], inv_g, byte);
+                const uint32_t word = fp4_encode<NV, true>(v[k], inv_g, byte);
                 if (i < words) code_row[i] = word;
                 uint32_t four = byte | __shfl_xor_sync(0xFFFFFFFFu, byte, 1 << kShift) << 8;
                 four |= __shfl_xor_sync(0xFFFFFFFFu, four, 2 << kShift) << 16;

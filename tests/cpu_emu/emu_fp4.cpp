@@ -22,8 +22,8 @@ void quantize(const void *x, size_t rows, size_t cols, size_t ld, float *g, int 
     }
     if (route == 0) {
         const size_t groups = rows * cols / 8;
-        emu::launch((unsigned)((groups + kFp4Threads * 4 - 1) / (kFp4Threads * 4)), kFp4Threads,
-                    [&] { fp4_quantize_flat_kernel<T, NV, 4>(p, groups, g, source, c, s); });
+        auto kern = NV && source != kScaleGiven ? fp4_quantize_flat_kernel<T, NV, !NV, 4> : fp4_quantize_flat_kernel<T, NV, true, 4>;
+        emu::launch((unsigned)((groups + kFp4Threads * 4 - 1) / (kFp4Threads * 4)), kFp4Threads, [&] { kern(p, groups, g, source, c, s); });
     } else {
         const size_t blocks = (cols + 31) / 32 * (NV ? 2 : 1), threads = (blocks * (NV ? 2 : 4) + 31) / 32 * 32;
         const int vec_ok = (reinterpret_cast<uintptr_t>(p) % (8 * sizeof(T))) == 0 && ld % 8 == 0;

@@ -111,6 +111,24 @@ def test_the_scale_of_small_and_of_zero_tensors(emu, route, grid, words):
         np.testing.assert_array_equal(unsigned_zeros(codes.numpy()), unsigned_zeros(want[0]))
 
 
+@pytest.mark.parametrize("route", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_far_above_a_given_tensor_scale_saturate(emu, dtype, route):
+    """x / g beyond f32 is still a finite x: the largest code and scale of its sign, not a NaN."""
+    x = aligned((4, 64), dtype)
+    x.copy_(torch.tensor([1e30, -1e30, 3e38, -1.0])[torch.arange(256) % 4].view(4, 64))
+    x[1, 17] = float("inf")
+    x[2, 40] = float("nan")
+    x[3, 16:] = 0.0
+    codes, scales, _ = run_quantize(emu, x, True, 2.0 ** -100, route=route)
+    want_codes, want_scales = np.full((4, 32), 0xF7), np.full((4, 4), 0x7E)
+    want_codes[1, 8:16], want_scales[1, 1] = 0, 0x7F
+    want_codes[2, 16:24], want_scales[2, 2] = 0, 0x7F
+    want_codes[3, 8:], want_scales[3, 1:] = 0, 0x38
+    np.testing.assert_array_equal(codes.numpy(), want_codes)
+    np.testing.assert_array_equal(scales.numpy(), want_scales)
+
+
 def test_rows_with_a_stride(emu):
     wide = special(6, 200, torch.bfloat16, 3)
     for view in (wide[:, 8:72], wide[:, 1:100]):

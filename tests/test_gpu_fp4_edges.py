@@ -101,3 +101,20 @@ def test_activations_as_they_come_have_no_scale(m, scale):
     for x in (acts(m, 320, BF16), acts(m, 320, F32)):
         assert torch.equal(gate_s.forward(x), gate.forward(x))
         assert torch.equal(gate_s.forward_gate_up_silu(up_s, x), gate.forward_gate_up_silu(up, x))
+
+
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_activations_far_above_their_scale_saturate(m, dtype):
+    """Finite activations that activation_scale takes beyond f32 are the largest value that the format has beside it, not NaN."""
+    lin, w, _ = layer(40, 96, Fp4Format.Nv, 1, bias=False, quantize_activations=True, activation_scale=1e-30)
+    x = torch.full((m, 96), 1e20, dtype=dtype, device="cuda")
+    x[1] = -1e20
+    x[2, 32:] = 1e-30
+    y = lin.forward(x, out_dtype=F32).double().cpu().numpy()
+    s = float(np.float32(1e-30))
+    xq = np.full((m, 96), 6.0 * 448.0 * s)
+    xq[1] *= -1.0
+    xq[2, 32:] = O.quantize(x[2:3, 32:].double().cpu().numpy(), True, s)[3][0]
+    want = O.product(xq, w)
+    assert (np.abs(y - want) <= O.product_bound(xq, w, 96) + 2.0 ** -24 * np.abs(want)).all()
