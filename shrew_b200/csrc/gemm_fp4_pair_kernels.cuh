@@ -123,7 +123,7 @@ struct PairEpilogue {
                 }
                 if (relu) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = fmaxf(v[i], 0.0f);
+                    for (int i = 0; i < 16; ++i) v[i] = relu_nan(v[i]);
                 }
                 pack(h * (16 / EPV), v);
             }

@@ -368,7 +368,7 @@ gemv_fp4_kernel(Fp4Operand w0, Fp4Operand w1, const T *x, int vec_ok, YT *__rest
                 if (w1.bias) u += w1.bias[n];
                 v = v / (1.0f + __expf(-v)) * u;
             } else if (epilogue == SHREWQ_EPILOGUE_RELU) {
-                v = fmaxf(v, 0.0f);
+                v = relu_nan(v);
             }
             store_out<YT>(y + (size_t)m * ldy + n, v);
         }

@@ -62,6 +62,12 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
     return d;
 }
+// max(v, 0), NaN for NaN
+__device__ __forceinline__ float relu_nan(float v) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(v), "f"(0.0f));
+    return d;
+}
 // 16 or 32 bytes, read once / written once.  Not through the read-only path: they may be what the kernel before in the stream writes, which may
 // still run when this one is launched early.
 __device__ __forceinline__ uint4 ld_once_16(const void *p) {

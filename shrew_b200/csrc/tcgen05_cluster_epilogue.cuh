@@ -184,7 +184,7 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
             } else {
                 const bool relu = epilogue == SHREWQ_EPILOGUE_RELU;
 #pragma unroll
-                for (int i = 0; i < CW; ++i) out_st[i * CH + ch] = to_out<YT>(relu ? fmaxf(v[0][i], 0.0f) : v[0][i]);
+                for (int i = 0; i < CW; ++i) out_st[i * CH + ch] = to_out<YT>(relu ? relu_nan(v[0][i]) : v[0][i]);
             }
         }
         named_bar_sync(2 + group, 128);  // the staging tile is complete

@@ -60,6 +60,7 @@ static inline uint32_t cvt_f16x2_e4m3(uint32_t two) { return emu_f16_bits(emu_e4
 static inline void f32x2_of_f16x2(uint32_t h, float &lo, float &hi) { lo = emu_f16_value(h & 0xFFFF); hi = emu_f16_value(h >> 16); }
 static inline uint32_t pack_f16x2_rn(float hi, float lo) { return emu_f16_bits(hi) << 16 | emu_f16_bits(lo); }
 static inline float max_abs_nan(float a, float b) { return a != a || b != b ? NAN : fmaxf(fabsf(a), fabsf(b)); }
+static inline float relu_nan(float v) { return v != v ? NAN : fmaxf(v, 0.0f); }
 static inline uint4 ld_once_16(const void *p) {
     EMU_CHECK((reinterpret_cast<uintptr_t>(p) & 15) == 0, "a 16-byte load off its boundary");
     uint4 v;

@@ -403,3 +403,13 @@ def test_inputs_of_a_stream_are_not_read_as_constant(emu, dtype):
         assert emu.emu_residual_norm(x.data_ptr(), b.data_ptr(), b.data_ptr(), 64, 64, 64, w.data_ptr(), None, w.data_ptr(), None, r.data_ptr(), h.data_ptr(), 3, 64, 1, 1, gate_kind,
                                      1e-5, 1.0, 1.0, 1, which, which, which, 1, 2) == 0
     assert emu.emu_read_only_loads() == 0
+
+
+@pytest.mark.parametrize("M", [3, 9])
+def test_relu_keeps_nan(emu, emu_gemm, M):
+    w = stored(20, 64, False, 4, spread=3)
+    x = aligned((M, 64), torch.bfloat16)
+    x.copy_(torch.randn(M, 64, generator=torch.Generator().manual_seed(1)))
+    x[2, 9] = float("nan")
+    y = forward(emu, emu_gemm, x, [w], [None], 64, False, relu=True)
+    assert np.isnan(y[2]).all() and (y[:2] >= 0).all() and (y[3:] >= 0).all()

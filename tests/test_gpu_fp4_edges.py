@@ -118,3 +118,14 @@ def test_activations_far_above_their_scale_saturate(m, dtype):
     xq[2, 32:] = O.quantize(x[2:3, 32:].double().cpu().numpy(), True, s)[3][0]
     want = O.product(xq, w)
     assert (np.abs(y - want) <= O.product_bound(xq, w, 96) + 2.0 ** -24 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("rounded", [False, True])
+@pytest.mark.parametrize("m,n", [(2, 150), (9, 150), (40, 150), (300, 150), (300, 9000)])
+@pytest.mark.parametrize("fmt", list(Fp4Format))
+def test_relu_keeps_nan(fmt, m, n, rounded):
+    lin, _, _ = layer(n, 256, fmt, 5, quantize_activations=rounded)
+    x = acts(m, 256, BF16)
+    x[1, 9] = float("nan")
+    y, r = lin.forward(x), lin.forward(x, epilogue=_lib.EPILOGUE_RELU)
+    assert r[1].isnan().all() and torch.equal(r[0], y[0].clamp(min=0.0)) and torch.equal(r[2:], y[2:].clamp(min=0.0))
