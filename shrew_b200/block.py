@@ -90,7 +90,7 @@ def run_blocks(blocks: Sequence[GatedMlp], x: torch.Tensor, final: Optional[Norm
     stream can feed bf16 products."""
     norms: List[Optional[Norm]] = [b.pre for b in blocks[1:]] + [final]
     if not blocks:
-        return residual_norm(x, pre=final)
+        return residual_norm(x, pre=final, out_dtype=act_dtype)
     _, h = residual_norm(x, pre=blocks[0].pre, out_dtype=act_dtype)
     for b, after in zip(blocks, norms):
         branch = b.block(h)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from shrew_b200 import Fp4Format, Fp4Linear, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor
+from shrew_b200 import Fp4Format, Fp4Linear, Norm, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor, run_blocks
 from shrew_b200 import _lib
 from shrew_b200.quantize import Device
 from tests import fp4_oracle as O
@@ -129,3 +129,10 @@ def test_relu_keeps_nan(fmt, m, n, rounded):
     x[1, 9] = float("nan")
     y, r = lin.forward(x), lin.forward(x, epilogue=_lib.EPILOGUE_RELU)
     assert r[1].isnan().all() and torch.equal(r[0], y[0].clamp(min=0.0)) and torch.equal(r[2:], y[2:].clamp(min=0.0))
+
+
+# ---- blocks -------------------------------------------------------------------------------------------------------------------
+def test_no_blocks_and_their_type():
+    x = acts(5, 64, F32)
+    r, h = run_blocks([], x, Norm(), act_dtype=BF16)
+    assert r is x and h.dtype is BF16 and torch.equal(h, run_blocks([], x, Norm())[1].to(BF16))
