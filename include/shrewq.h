@@ -229,7 +229,7 @@ SHREWQ_API int shrewq_dequantize_ex(shrewq_ctx *ctx, const int8_t *q_dev, const 
  */
 SHREWQ_API int shrewq_quantize_fp4(shrewq_ctx *ctx, const void *w_dev, int w_dtype, size_t rows, size_t cols, size_t ldw, int format,
                                    float *tensor_scale_dev, int find_tensor_scale, uint8_t *codes_dev, uint8_t *scales_dev);
-/* Codes and scales -> values of out_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), [rows, cols] without gaps. */
+/* Codes and scales -> values of out_dtype (SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16), [rows, cols] without gaps; tensor_scale_dev NULL for MX. */
 SHREWQ_API int shrewq_dequantize_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev,
                                      size_t rows, size_t cols, int format, int out_dtype, void *out_dev);
 

@@ -80,6 +80,7 @@ int shrewq_dequantize_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8
     if (!storage16or32(out_dtype)) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "dequantize_fp4: out_dtype must be SHREWQ_F32, SHREWQ_BF16 or SHREWQ_F16");
     if (sizes_overflow(rows, cols)) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "dequantize_fp4: rows*cols overflows");
     if (nv && !tensor_scale_dev) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "dequantize_fp4: SHREWQ_FP4_NV needs tensor_scale_dev");
+    if (!nv && tensor_scale_dev) return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "dequantize_fp4: SHREWQ_FP4_MX has no tensor scale");
     if (misaligned(tensor_scale_dev, 4) || misaligned(out_dev, size_of(out_dtype)) || misaligned(codes_dev, 4))
         return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "dequantize_fp4: out_dev aligned to its elements, tensor_scale_dev and codes_dev to 4 bytes");
     if (rows * cols == 0) return SHREWQ_OK;

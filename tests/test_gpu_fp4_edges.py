@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from shrew_b200 import Fp4Format, Fp4Linear, Norm, QuantConfig, dequantize_fp4, quantize_fp4, quantize_tensor, run_blocks
+from shrew_b200 import Fp4Format, Fp4Linear, Fp4Tensor, Norm, QuantConfig, ShrewError, dequantize_fp4, quantize_fp4, quantize_tensor, run_blocks
 from shrew_b200 import _lib
 from shrew_b200.quantize import Device
 from tests import fp4_oracle as O
@@ -89,6 +89,14 @@ def test_words_for_finding_a_scale(words):
     assert float(whole[0]) == float(want.tensor_scale) == O.quantize(x.double().cpu().numpy(), True)[2]
     assert torch.equal(codes, want.codes) and torch.equal(scales, want.scales) and (whole[words:] == -5.0).all()
     assert _lib.lib().shrewq_quantize_fp4(*args, -1, codes.data_ptr(), scales.data_ptr()) == _lib.ERR_INVALID_ARG
+
+
+def test_a_tensor_scale_beside_mx_is_refused():
+    """As the quantizer and the layers refuse it, not left out."""
+    q = quantize_fp4(torch.ones(4, 64, device="cuda"), Fp4Format.Mx)
+    with pytest.raises(ShrewError) as e:
+        dequantize_fp4(Fp4Tensor(q.codes, q.scales, torch.full((1,), 2.0, device="cuda"), q.shape, F32, Fp4Format.Mx))
+    assert e.value.code == _lib.ERR_INVALID_ARG
 
 
 # ---- layers -----------------------------------------------------------------------------------------------------------------
