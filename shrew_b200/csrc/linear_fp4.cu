@@ -23,6 +23,9 @@ bool sizes_overflow(size_t rows, size_t cols) { return cols > ((size_t)1 << 40) 
 }  // namespace
 
 int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
+    // (the kernels round the tokens up to whole tiles in 32 bits, and f32 ones above 32 stand in three terms one behind the other)
+    if (a.M > 0x7FFFFFFFu / (a.M > 32 && !a.w->round_x && a.x_dtype == SHREWQ_F32 ? 3 : 1) - 256)
+        return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "4-bit forward: %zu tokens are more than 32-bit indexes hold", a.M);
     if (a.w->round_x) {
         *kernel = "tcgen05-fp4";
         return launch_gemm_fp4(ctx, a);

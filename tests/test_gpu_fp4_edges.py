@@ -139,6 +139,16 @@ def test_relu_keeps_nan(fmt, m, n, rounded):
     assert r[1].isnan().all() and torch.equal(r[0], y[0].clamp(min=0.0)) and torch.equal(r[2:], y[2:].clamp(min=0.0))
 
 
+@pytest.mark.parametrize("rounded,x_dtype,most", [(True, _lib.BF16, 2 ** 31 - 257), (True, _lib.F32, 2 ** 31 - 257), (False, _lib.BF16, 2 ** 31 - 257),
+                                                  (False, _lib.F32, 715827626)])
+def test_more_tokens_than_indexes_hold_are_refused(rounded, x_dtype, most):
+    """On the host, before anything of them is read."""
+    lin, _, _ = layer(1, 32, Fp4Format.Mx, 1, quantize_activations=rounded)
+    x = torch.zeros(64, device="cuda")
+    for m in (most + 1, 2 ** 31 - 1):
+        assert _lib.lib().shrewq_linear_forward(lin._h, x.data_ptr(), x_dtype, m, x.data_ptr(), _lib.F32, 1, 0) == _lib.ERR_UNSUPPORTED
+
+
 # ---- blocks -------------------------------------------------------------------------------------------------------------------
 def test_no_blocks_and_their_type():
     x = acts(5, 64, F32)
