@@ -18,7 +18,6 @@ EPILOGUE_NONE, EPILOGUE_RELU = 0, 1
 EXCHANGE_FLAG_BYTES = 256
 FP4_MX, FP4_NV = 0, 1
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
-GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 
 # SHREWQ_LIB points at another build of the same library (e.g. the tracing build)
 LIB_PATH = os.environ.get("SHREWQ_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libshrewq.so")
@@ -70,15 +69,6 @@ SIGNATURES = {
     "shrewq_plan_forward": (_ci, [_sz, _sz, _sz, _ci, _ci, _ci, ctypes.c_char_p, _sz, ctypes.POINTER(_ci), ctypes.POINTER(_ci),
                                  ctypes.POINTER(_ci), ctypes.POINTER(_ci), ctypes.POINTER(_ci)]),
 }
-
-class ResidualNormArgs(ctypes.Structure):
-    """shrewq_residual_norm_args."""
-    _fields_ = [("M", _sz), ("D", _sz), ("x_dev", _vp), ("ldx", _sz), ("x_dtype", _ci), ("branch_dev", _vp), ("ldb", _sz),
-                ("branch_dtype", _ci), ("gate_dev", _vp), ("ldg", _sz), ("gate_kind", _ci), ("post_norm", _ci), ("post_eps", ctypes.c_float),
-                ("post_weight_dev", _vp), ("post_bias_dev", _vp), ("residual_scale", ctypes.c_float), ("branch_scale", ctypes.c_float),
-                ("pre_norm", _ci), ("pre_eps", ctypes.c_float), ("pre_weight_dev", _vp), ("pre_bias_dev", _vp), ("residual_dev", _vp),
-                ("normed_dev", _vp), ("normed_dtype", _ci)]
-
 
 class QuantItem(ctypes.Structure):
     """shrewq_quant_item: one tensor of shrewq_quantize_f32_batch."""
