@@ -278,8 +278,9 @@ SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_
  *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens.
  *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
  *     positive number, as the tensor scale, which is not used otherwise), and codes are multiplied by codes on the block-scaled tensor cores.
- * Workspaces of the context (see shrewq_ctx_set_stream): quantize_activations = 1 always, for the codes; else 5 to 32 tokens, and above 32
- * f32 activations and bf16 ones whose rows are not whole 16-byte pieces, for a staged copy.
+ * Workspaces of the context (see shrewq_ctx_set_stream): quantize_activations = 1 always, for the codes; else for a staged copy of x in the
+ * kernels "tcgen05-w4-f16" (see shrewq_linear_last_kernel; up to 32 tokens) and "tcgen05-w4", there with f32 activations or bf16 ones whose rows are not
+ * whole 16-byte pieces.
  */
 SHREWQ_API int shrewq_linear_create_fp4(shrewq_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, const float *tensor_scale_dev,
                                         const float *bias_dev, size_t out_features, size_t in_features, int format,

@@ -1,4 +1,4 @@
-// Launchers of the forward of 5 to 32 tokens with 4-bit weights (device code and its description: gemm_fp4_f16_kernels.cuh).
+// Launchers of the forward of up to 32 tokens with 4-bit weights in f16 (device code and its description: gemm_fp4_f16_kernels.cuh).
 #include <cuda_fp16.h>
 
 #include "gemm_tcgen05_launch.cuh"

@@ -1,4 +1,5 @@
-// Forward of a layer with 4-bit microscaled weights for 5 to 32 tokens, on the tensor cores (tcgen05.mma kind::f16 in f16), sm_100a only.
+// Forward of a layer with 4-bit microscaled weights for up to 32 tokens, on the tensor cores (tcgen05.mma kind::f16 in f16), sm_100a only.
+// (linear_fp4.cu says which calls take it: in the main 5 to 32 bf16 tokens over more tiles than SMs.)
 //
 //   y[m,n] = epi( alpha[n] * 2^e[m] * sum_k w[n,k] x'[m,k] + bias[n] ),   x' = x * 2^-e[m] in f16 terms
 //
@@ -10,8 +11,9 @@
 // activations where a token has values below 2^-32 of its largest (f32: three terms of 11 bits).  Each pass's sums are added in f32 with
 // their power of two to totals in tensor memory; with one pass (all ordinary tensors) nothing of that runs.
 //
-// Two CTAs share an SM (256 columns of tensor memory, half the shared memory): all tiles of a layer up to 296 CTAs are in flight at
-// once and share the stream evenly, whatever their number, and one CTA's prologue and epilogue hide behind the other's loads.
+// Two CTAs share an SM (256 columns of tensor memory, half the shared memory): up to 296 tiles are in flight at once, and one CTA's prologue and
+// epilogue hide behind the other's loads.  What an SM takes in bounds it, some 16 bytes a cycle for the 64-byte rows of its boxes, so the time is that
+// of the SMs with two tiles: 172 gated tiles (11008 x 4096, 16 tokens) 26 us, 296 tiles 27.7, 148 tiles 21.1, from cold HBM, staging included.
 // Mapping otherwise as gemm_fp4_bf16_kernels.cuh: D[128 x TOK] += A[128 x 16] B[TOK x 16]^T, stages of 128 codes a row, GATED tiles
 // interleave 64 gate and 64 up rows, k split over a cluster.  Codes and activations wait in a ring of kStages in shared memory; the
 // widened codes have kSlots places in tensor memory.

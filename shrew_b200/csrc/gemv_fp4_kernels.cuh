@@ -22,7 +22,7 @@
 // register holds a byte in flight, no barrier guards one, and an SM has some 60 KB on their way.  The rows of a tile are 4 neighbours
 // each from the 4 groups of 32 that share 16 bytes of scales in the handle's copy (scale_piece_offset): scale sectors are used whole.
 // Activations: every CTA stages them in its shared memory while its first codes are on their way: one launch, no workspace.  (From 5 tokens
-// on gemm_fp4_f16_kernels.cuh: an m16n8k16 of mma.sync holds its tensor pipe for 32 cycles, which one group of 8 tokens just allows.)
+// on the tcgen05 kernels: an m16n8k16 of mma.sync holds its tensor pipe for 32 cycles, which one group of 8 tokens just allows.)
 // The warps' sums of a tile meet in shared memory in a fixed order.
 //
 // Programmatic dependent launch: the ring is filled before the wait for the previous kernel.

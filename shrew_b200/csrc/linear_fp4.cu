@@ -20,6 +20,22 @@ bool misaligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 // rows * cols values at up to 4 bytes, and padded rows, stay within what a size_t and a kernel's index hold
 bool sizes_overflow(size_t rows, size_t cols) { return cols > ((size_t)1 << 40) || (cols != 0 && rows > ((size_t)1 << 48) / cols); }
 
+// Up to 32 tokens: the kernel in f16 (two CTAs an SM, a launch to stage the activations) or the one in bf16 (one CTA an SM, bf16 activations as they
+// are).  Measured on weights from cold HBM, us in f16 / in bf16:
+//   bf16, tiles for one CTA an SM, which may also share their k: bf16 wins (4096 x 4096, 16 tokens: 19.5 / 9.7; 4096 x 11008: 26.4 / 15.8; 8192 x
+//     4096 gated 20.2 / 18.5), but for fewer than 16 tokens of long rows in more than half as many tiles as SMs (11008 x 4096, 8 tokens: 18.0 / 19.0;
+//     16384 x 8192: 28.9 / 31.4);
+//   bf16, more tiles, which take bf16 another round: f16 wins (11008 x 4096 gated, 8 and 32 tokens: 24.9 / 35.3, 26.9 / 35.2), until the staging and
+//     16 tokens an epilogue chunk outweigh short rows (32768 x 512, 8, 16 and 32 tokens: 9.9 / 11.8, 11.5 / 11.5, 15.5 / 11.2);
+//   f32, three passes in f16, three products of one pass in bf16: bf16 wins (11008 x 4096, 8 tokens: 33.4 / 25.2; gated 54.5 / 49.7), but where many
+//     CTAs read the same few bytes of activations again and again, their three terms less than 128 KB (5 tokens: 32.8 / 43.3; 32768 x 2048, 8 and 12:
+//     31.3 / 43.4, 32.3 / 29.7).
+bool w4_f16_wins(const shrewq_ctx *ctx, const Fp4Forward &a) {
+    const size_t tiles = (a.N + (a.up ? 63 : 127)) / (a.up ? 64 : 128), sms = (size_t)ctx->sm_count;
+    if (a.x_dtype == SHREWQ_F32) return tiles > sms / 2 && a.K >= 1024 && a.M * a.K * 6 < 128 * 1024;
+    return tiles > sms ? a.K >= 32 * a.M : tiles > sms / 2 && a.K >= 4096 && a.M < 16;
+}
+
 }  // namespace
 
 int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
@@ -30,16 +46,16 @@ int forward_fp4(shrewq_ctx *ctx, const Fp4Forward &a, const char **kernel) {
         *kernel = "tcgen05-fp4";
         return launch_gemm_fp4(ctx, a);
     }
-    if (a.M > 32) {
-        *kernel = "tcgen05-w4";
-        return launch_gemm_w4_bf16(ctx, a);
-    }
     if (gemv_fp4_supported(a)) {
         *kernel = "mma-fp4";
         return launch_gemv_fp4(ctx, a);
     }
-    *kernel = "tcgen05-w4-f16";
-    return launch_gemm_w4_f16(ctx, a);
+    if (a.M <= 32 && w4_f16_wins(ctx, a)) {
+        *kernel = "tcgen05-w4-f16";
+        return launch_gemm_w4_f16(ctx, a);
+    }
+    *kernel = "tcgen05-w4";
+    return launch_gemm_w4_bf16(ctx, a);
 }
 
 void destroy_fp4(Fp4Weight *w) {

@@ -8,7 +8,7 @@ from shrew_b200 import Fp4Format, Fp4Linear, Fp4Tensor, Norm, QuantConfig, Shrew
 from shrew_b200 import _lib
 from shrew_b200.quantize import Device
 from tests import fp4_oracle as O
-from tests.test_gpu_fp4 import acts, layer
+from tests.test_gpu_fp4 import acts, layer, near
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -147,6 +147,39 @@ def test_more_tokens_than_indexes_hold_are_refused(rounded, x_dtype, most):
     x = torch.zeros(64, device="cuda")
     for m in (most + 1, 2 ** 31 - 1):
         assert _lib.lib().shrewq_linear_forward(lin._h, x.data_ptr(), x_dtype, m, x.data_ptr(), _lib.F32, 1, 0) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("m", [6, 20, 32])
+def test_gated_layers_of_many_tiles_in_turn_captured_and_on_streams(m):
+    """The kernels of 5 to 32 tokens over more tiles than SMs, and over few, one after the other: the same bits eagerly, on another stream and replayed."""
+    gate, wg, _ = layer(9600, 1056, Fp4Format.Nv, 1, bias=False)
+    up, wu, _ = layer(9600, 1056, Fp4Format.Nv, 2, bias=False)
+    down, wd, _ = layer(1056, 9600, Fp4Format.Nv, 3, bias=False)
+    xs = [acts(m, 1056, BF16, seed=s) * 0.01 for s in range(3)]
+
+    def run(x):
+        return down.forward(gate.forward_gate_up_silu(up, x))
+    h = gate.forward_gate_up_silu(up, xs[0])
+    assert gate.last_kernel() == "tcgen05-w4-f16"
+    xd = xs[0].double().cpu().numpy()
+    near(h, O.product(xd, wg, up=wu), O.product_bound(xd, wg, 1056, up=wu))
+    want = [run(x) for x in xs]
+    assert down.last_kernel() == "tcgen05-w4"
+    for _ in range(20):
+        assert all(torch.equal(run(x), w) for x, w in zip(xs, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [run(x) for x in xs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    x, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run(x)
+    for x_new, w in zip(xs, want):
+        x.copy_(x_new)
+        graph.replay()
+        assert torch.equal(y, w)
 
 
 # ---- blocks -------------------------------------------------------------------------------------------------------------------

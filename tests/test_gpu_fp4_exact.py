@@ -47,7 +47,7 @@ MS = [1, 2, 4, 5, 16, 17, 32, 33, 64, 65, 128, 129, 300]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("k,n", [(1, 3), (33, 40), (257, 130), (2049, 70), (4096, 130), (11008, 9)])
+@pytest.mark.parametrize("k,n", [(1, 3), (33, 40), (257, 130), (2049, 70), (4096, 130), (11008, 9), (1056, 19100)])
 @pytest.mark.parametrize("m", MS)
 def test_sums_are_exact(fmt, m, n, k):
     """Multiples of 1/4 below 36 k < 2^19: every partial sum has less than 24 bits, so f32 sums in any order are the exact sum."""
@@ -83,22 +83,23 @@ def test_gated_sums_are_exact(fmt, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("k", [96, 333, 1056])
+@pytest.mark.parametrize("k,times", [(96, 1), (333, 1), (1056, 1), (1056, 19)])
 @pytest.mark.parametrize("m", MS)
-def test_every_column_and_every_bit(fmt, k, m):
+def test_every_column_and_every_bit(fmt, k, times, m):
     """Each channel is one column of x with a factor of 2: f32 activations with all their 24 bits, the smallest 2^-12 of the largest."""
-    lin = Fp4Linear(stored(torch.eye(k, dtype=torch.uint8) * 4, fmt))
+    lin = Fp4Linear(stored((torch.eye(k, dtype=torch.uint8) * 4).repeat(times, 1), fmt))
     g = torch.Generator().manual_seed(m + k)
     x = (torch.rand(m, k, generator=g) + 1.0) * torch.exp2(-torch.randint(0, 13, (m, k), generator=g).float()) * torch.where(torch.rand(m, k, generator=g) < 0.5, -1.0, 1.0)
     x = x.cuda()
-    assert torch.equal(lin.forward(x), 2.0 * x)
-    assert torch.equal(lin.forward(x, out_dtype=BF16), (2.0 * x).to(BF16))
-    assert torch.equal(lin.forward(x.to(BF16), out_dtype=F32), 2.0 * x.to(BF16).float())
+    want, want16 = (2.0 * x).repeat(1, times), (2.0 * x.to(BF16).float()).repeat(1, times)
+    assert torch.equal(lin.forward(x), want)
+    assert torch.equal(lin.forward(x, out_dtype=BF16), want.to(BF16))
+    assert torch.equal(lin.forward(x.to(BF16), out_dtype=F32), want16)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rounded", [False, True])
-@pytest.mark.parametrize("m,n", [(1, 150), (8, 150), (40, 150), (200, 150), (300, 9500)])
+@pytest.mark.parametrize("m,n", [(1, 150), (8, 150), (8, 19100), (40, 150), (200, 150), (300, 9500)])
 def test_a_nan_block_stays_in_its_channel(fmt, rounded, m, n):
     code = codes(n, 320, 3)
     bad, clean = (Fp4Linear(stored(code, fmt, nan_block=b), quantize_activations=rounded) for b in ((77, 9), None))
@@ -107,6 +108,39 @@ def test_a_nan_block_stays_in_its_channel(fmt, rounded, m, n):
     assert y[:, 77].isnan().all()
     y[:, 77] = want[:, 77]
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("m", [1, 6, 20, 32, 40])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [50, 19100])
+def test_scales_far_apart(dtype, n, m):
+    """Block scales over 90 octaves: what stands in the blocks of small scales alone comes out as exactly as the rest."""
+    k = 1088
+    code = codes(n, k, 1)
+    w = stored(code, Fp4Format.Mx)
+    e = torch.randint(-90, 1, (n, k // 32), generator=torch.Generator().manual_seed(2))
+    e[:, 0] = 0
+    w.scales.copy_((127 + e).to(torch.uint8))
+    lin = Fp4Linear(w)
+    x = torch.zeros(m, k)
+    block = 1 + torch.arange(m) % (k // 32 - 1)
+    for i in range(m):   # (values of the grid, in one block each)
+        x[i, 32 * block[i]:32 * block[i] + 32] = values(codes(1, 32, i))[0]
+    y = lin.forward(x.to(dtype).cuda(), out_dtype=F32).double().cpu()
+    wd = values(code).double().view(n, -1, 32) * torch.exp2(e.double())[..., None]
+    assert torch.equal(y, x.double() @ wd.view(n, k).t())
+
+
+@pytest.mark.parametrize("m,n,k,dtype,gated,name", [
+    (4, 4096, 4096, BF16, False, "mma-fp4"), (4, 128, 11008, BF16, False, "tcgen05-w4"), (16, 4096, 4096, BF16, False, "tcgen05-w4"), (8, 9600, 4096, BF16, False, "tcgen05-w4-f16"),
+    (16, 9600, 4096, BF16, False, "tcgen05-w4"), (32, 9536, 1024, BF16, True, "tcgen05-w4-f16"), (32, 9472, 1024, BF16, True, "tcgen05-w4"),
+    (32, 19072, 992, BF16, False, "tcgen05-w4"), (5, 9600, 4096, F32, False, "tcgen05-w4-f16"), (6, 9600, 4096, F32, False, "tcgen05-w4"), (33, 19072, 4096, BF16, False, "tcgen05-w4")])
+def test_which_kernel_takes_a_call(m, n, k, dtype, gated, name):
+    """On the 148 SMs of a B200."""
+    lin = Fp4Linear(stored(torch.zeros(n, k, dtype=torch.uint8), Fp4Format.Mx))
+    x = torch.zeros(m, k, dtype=dtype, device="cuda")
+    y = lin.forward_gate_up_silu(lin, x) if gated else lin.forward(x)
+    assert lin.last_kernel() == name and (y == 0).all()
 
 
 # ---- the quantizer ------------------------------------------------------------------------------------------------------------
