@@ -208,7 +208,7 @@ SHREWQ_API int shrewq_dequantize_ex(shrewq_ctx *ctx, const int8_t *q_dev, const 
  * No counterpart in the reference (its 4-bit type is an integer, quantize.rs:51-58): weights, and activations if asked, as E2M1 codes
  * (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a scale for every block along a row:
  *   SHREWQ_FP4_MX  blocks of 32, a power of two as an E8M0 byte b (2^(b - 127), 255 = NaN): 2^(floor(log2 amax) - 2), at least 2^-127;
- *   SHREWQ_FP4_NV  blocks of 16, an E4M3 byte (448 at most, 0x7F = NaN), and one f32 scale g for the whole tensor:
+ *   SHREWQ_FP4_NV  blocks of 16, an E4M3 byte (448 at most, never negative, 0x7F = NaN), and one f32 scale g for the whole tensor:
  *                  e4m3(amax / (6 g)), at least 2^-9.
  * amax is the block's largest magnitude.  A block of zeros has the scale 1; a block with an infinity or a NaN has the scale NaN and
  * codes 0, so that it comes back as NaN.  code = x / scale (NV: (x / g) / scale, with x / g formed as x times the rounded reciprocal of g)
@@ -275,7 +275,8 @@ SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_
  * activations), shrewq_linear_forward_host and shrewq_mlp_forward_host; not through peer destinations or the no-allocation forward.  Any
  * in_features; activations and results f32 or bf16.
  *   quantize_activations = 0: y = x . dequant(W)^T + bias with f32 sums of exact products.  bf16 activations smaller than 2^-64 of the
- *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens.
+ *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens; there an infinite activation makes
+ *     NaN of an infinite result where the scales of an MX matrix span more than 28 octaves.  (NaN stays NaN everywhere, through ReLU too.)
  *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
  *     positive number, as the tensor scale, which is not used otherwise), and codes are multiplied by codes on the block-scaled tensor cores.
  * Workspaces of the context (see shrewq_ctx_set_stream): quantize_activations = 1 always, for the codes; else for a staged copy of x in the

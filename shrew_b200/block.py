@@ -25,7 +25,7 @@ class NormKind(enum.Enum):
 
 
 class Norm:
-    """The parameters of a norm over the last dimension; weight and bias (f32 copies are kept) may be left out.
+    """The parameters of a norm over the last dimension; weight and bias (kept as contiguous f32) may be left out.
 
     Rms:   v / sqrt(mean(v^2) + eps) * weight + bias
     Layer: (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias"""

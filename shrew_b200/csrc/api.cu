@@ -59,7 +59,6 @@ int ensure_scratch(shrewq_ctx *ctx, size_t bytes) {
 
 int ensure_xsplit(shrewq_ctx *ctx, size_t bytes) { return grow(ctx, &ctx->xsplit, &ctx->xsplit_bytes, bytes, false); }
 
-
 int ensure_stage(shrewq_ctx *ctx, size_t dev_bytes, size_t pinned_bytes) {
     int rc = grow(ctx, &ctx->stage_dev, &ctx->stage_dev_bytes, dev_bytes, false);
     if (rc != SHREWQ_OK) return rc;

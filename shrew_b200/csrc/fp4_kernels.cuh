@@ -78,10 +78,9 @@ __device__ __forceinline__ float fp4_tensor_scale(float amax) {
     return __uint_as_float(e << 23);
 }
 
-// a / 6 and 1 / s, rounded to nearest as the IEEE operations round them: an approximation and one step with its exact remainder (Markstein
-// 1990: right for every a whose quotient is a normal number, and smaller ones end at the least scale; s runs through the 126 values that a
-// scale can have, all of them checked against the division).  They cost 3 instructions each, without the branch for special operands that the
-// general operations carry.
+// a / 6 and 1 / s, rounded to nearest: an approximation and one step with its exact remainder (Markstein 1990: right for every a whose quotient is a
+// normal number, and smaller ones end at the least scale; s runs through the 126 values that a scale can have, and tests/test_gpu_fp4_exact.py
+// through all of them, with every border of their codes).  3 instructions each.
 __device__ __forceinline__ float div6_rn(float a) {
     const float r = 0.166666672f, q = a * r;  // r = 1/6 rounded to nearest
     return __fmaf_rn(__fmaf_rn(-6.0f, q, a), r, q);

@@ -16,13 +16,13 @@
 // copies, taking the stages in turn; the last warp = relay.  Copies arrive on the stage's barrier by themselves
 // (cp.async.mbarrier.arrive); the relay of each CTA waits there, makes them visible to the tensor core (fence.proxy.async) and arrives at
 // the leader, publishing them to the cluster (a fence for shared memory alone: with .release.cluster the relays' arrivals held the pair up, 165 us
-// instead of 117 for 4096 x 11008 with 4096 tokens, and by the copying warps, with copies in flight, they took 1200 cycles a stage).  The accumulators,
-// 256 columns, and the stages' scales
-// fill tensor memory, so the MMAs of the next tile wait until the sums have been read: all warps that are free then take part, after the
-// next tile's first stages are under way.
-// Measured: 4096 x 11008 MX, 4096 tokens: 85 us of 114 to 118 for the call (quantizing the tokens is the rest; 3.1 PFLOP/s over all, at 1680 MHz under the
-// power limit); gated 11008 x 4096 NV, 512 tokens: 35 us, 36 to 39 for the call.  What is left: 256 tiles for 74 pairs are 3.5 rounds, and a stage
-// takes 540 to 600 cycles to bring for 512 of matrix work.
+// instead of 117 for 4096 x 11008 with 4096 tokens, and by the copying warps, with copies in flight, they took 1200 cycles a stage).
+// The accumulators, 256 columns, and the stages' scales fill tensor memory, so the MMAs of the next tile wait until the sums have been read: all
+// warps that are free then take part, after the next tile's first stages are under way.
+// Measured: 4096 x 11008 MX, 4096 tokens: 85 us of 116 to 118 for the call (quantizing the tokens is the rest; 3.1 PFLOP/s over all, at 1680 MHz under
+// the power limit); gated 11008 x 4096 NV, 512 tokens: 35 us, 38.5 to 39.5 for the call.  A stage takes 540 to 600 cycles to bring for 512 of matrix
+// work, and 256 (172) tiles for 74 pairs are 3.5 (2.3) rounds that take 4 (3): together 66 and 25 us.  The rest is most likely the MMAs' wait for
+// the copying groups, which bring 4 or 5 stages of the next tile and are then in the epilogue of this one.
 //
 // Device code only; also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once
@@ -54,8 +54,8 @@ struct Fp4PairCfg {
     static_assert((3 * kStages + 2) * 8 <= 512, "barriers");
 };
 
-// silu(g) * u = u g / (1 + 2^(-g log2 e)): four instructions less than with __expf and __fdividef, whose care for denormal results has
-// nothing to do here (0 for them is within 2^-126 |u g|).
+// silu(g) * u = u g / (1 + 2^(-g log2 e)), by the approximate 2^x and 1 / x (results below 2^-126 are 0, within 2^-126 |u g| of theirs): four
+// instructions less than through __expf and __fdividef
 __device__ __forceinline__ float pair_silu(float g, float u) {
     return g * recip_approx(1.0f + exp2_approx(-1.44269504f * g)) * u;
 }

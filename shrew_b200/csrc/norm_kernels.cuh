@@ -14,10 +14,11 @@
 // centred values, which stay in registers: no cancellation for rows far from zero.
 //
 // Memory-bound: x and branch are read once and r and h written once.  A row lives in the registers of a warp (up to 1024 columns) or of a
-// CTA (V groups of 8 columns a thread), so the two statistics cost no second read.  The weights come through L1, which the rows' streaming
-// loads leave to them.
-// Measured: 4096 rows of 4096, f32 stream, bf16 branch and gate, norms before and after: 44 us, 4.6 TB/s of half reads and half writes; a
-// row is two sums of a CTA, one after the other, and four rows an SM are under way (more threads a row, or rows an SM, need registers that are not there).
+// CTA (V groups of 8 columns a thread), so the two statistics cost no second read; above 16384 columns (V = 4 with 64 registers a thread) 320 to 612
+// bytes a thread are spilled.  The weights come through L1, which the rows' streaming loads leave to them.
+// Measured (f32 stream, bf16 branch and gate of channels, norms before and after, bf16 out): 4096 rows of 4096 45 us, 4.5 TB/s of half reads and half
+// writes; 2048 rows of 16384 106 us, 3.8 TB/s; 1024 rows of 32768 127 us, 3.2 TB/s.  A row is two sums of a CTA, one after the other, with four
+// rows of 4096 an SM under way and no load of the next rows meanwhile (registers are taken; shared memory is not used for it).
 //
 // Device code only (no launch syntax; PTX behind ptx_fp4.cuh and ptx_small.cuh): also compiles for the CPU tests (tests/cpu_emu/).
 #pragma once

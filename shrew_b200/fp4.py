@@ -66,7 +66,7 @@ class Fp4Tensor:
 
 def quantize_fp4(tensor: torch.Tensor, format: Fp4Format = Fp4Format.Mx, tensor_scale: Optional[torch.Tensor] = None) -> Fp4Tensor:
     """An f32, bf16 or f16 CUDA tensor as 4-bit codes with block scales along its rows (shrewq_quantize_fp4).  `tensor_scale` (Nv
-    only): one positive float32 on the device; by default the smallest power of two that brings the largest block scale under E4M3's
+    only): one float32 on the device, 2^-126 or more; by default the smallest power of two that brings the largest block scale under E4M3's
     largest value, found in a pass of its own."""
     if not tensor.is_cuda:
         Device.get(tensor.device)    # raises: CUDA devices only
@@ -86,7 +86,10 @@ class Fp4Linear(QuantizedLinear):
 
     quantize_activations=False: x . dequant(W)^T + bias, products exact, sums in f32.
     quantize_activations=True: the rows of x are first quantized to the weights' format (Nv with `activation_scale` as their
-    tensor scale) and multiplied code by code on the block-scaled tensor cores."""
+    tensor scale, which nothing else uses) and multiplied code by code on the block-scaled tensor cores.
+
+    Most calls with more than a few tokens, and all that quantize activations, use a workspace of the device's context
+    (include/shrewq.h, shrewq_linear_create_fp4): calls on different streams, and replays of captured ones, have to be ordered."""
 
     def __init__(self, weight: Fp4Tensor, bias: Optional[torch.Tensor] = None, quantize_activations: bool = False,
                  activation_scale: float = 1.0):
