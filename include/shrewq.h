@@ -274,7 +274,8 @@ SHREWQ_API int shrewq_linear_create_int4(shrewq_ctx *ctx, const uint8_t *packed_
  * The handle goes through shrewq_linear_forward, shrewq_linear_forward_gate_up_silu (both layers of one format and one treatment of
  * activations), shrewq_linear_forward_host and shrewq_mlp_forward_host; not through peer destinations or the no-allocation forward.  Any
  * in_features; activations and results f32 or bf16.
- *   quantize_activations = 0: y = x . dequant(W)^T + bias with f32 sums of exact products.  bf16 activations smaller than 2^-64 of the
+ *   quantize_activations = 0: y = x . dequant(W)^T + bias with f32 sums of exact products (NV: before the tensor scale, so they are infinite
+ *     where they pass f32 without it).  bf16 activations smaller than 2^-64 of the
  *     largest in their token, and bits of f32 activations below 2^-46 of it, may be dropped up to 32 tokens; there an infinite activation makes
  *     NaN of an infinite result where the scales of an MX matrix span more than 28 octaves.  (NaN stays NaN everywhere, through ReLU too.)
  *   quantize_activations = 1: the rows of x are quantized to the layer's format first (rows are the tokens; NV with activation_scale, a
@@ -464,7 +465,7 @@ SHREWQ_API const char *shrewq_linear_last_kernel(const shrewq_linear *lin);
  * streamed through a shared-memory ring by bulk copies, M <= 32), "tcgen05" (single-CTA tensor-core kernel), "tcgen05-2cta" (CTA pairs,
  * tcgen05.mma.cta_group::2), "tcgen05-f32" (f32 activations as a bf16 hi/lo pair on the tensor cores),
  * "simt" (general f32 kernel), or "auto"/NULL to restore the built-in choice.  A forced kernel that
- * cannot take a shape makes the forward fail with SHREWQ_ERR_UNSUPPORTED (it never falls
+ * cannot take a shape, or 4-bit floating-point weights, makes the forward fail with SHREWQ_ERR_UNSUPPORTED (it never falls
  * back silently).  For tests and benchmarks; no counterpart in the reference. */
 SHREWQ_API int shrewq_force_kernel(const char *name);
 /* Which kernel family and launch plan a forward of this shape would get on a GPU with `sm_count` SMs

@@ -629,6 +629,7 @@ static int forward_impl(shrewq_linear *lin, shrewq_linear *up, const void *x_dev
         if (up && (!lin->fp4 || !up->fp4 || lin->fp4->nv != up->fp4->nv || lin->fp4->round_x != up->fp4->round_x || lin->fp4->x_scale != up->fp4->x_scale))
             return set_err(ctx, SHREWQ_ERR_INVALID_ARG, "%s: gate and up must both hold 4-bit weights of one format and treat activations alike", who);
         if (n_peers > 0) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "%s: 4-bit weights take no peer destinations", who);
+        if (g_forced_kernel != kAuto) return set_err(ctx, SHREWQ_ERR_UNSUPPORTED, "%s: a forced kernel cannot take 4-bit floating point weights", who);
         Fp4Forward f;
         f.w = lin->fp4; f.up = up ? up->fp4 : nullptr;
         f.bias = lin->bias; f.bias_up = up ? up->bias : nullptr;

@@ -182,6 +182,22 @@ def test_gated_layers_of_many_tiles_in_turn_captured_and_on_streams(m):
         assert torch.equal(y, w)
 
 
+@pytest.mark.parametrize("name", [b"gemv", b"mma", b"tcgen05", b"simt"])
+def test_forced_kernels_do_not_take_these_layers(name):
+    lin, _, _ = layer(32, 64, Fp4Format.Mx, 1)
+    x = acts(2, 64, BF16)
+    want = lin.forward(x)
+    assert _lib.lib().shrewq_force_kernel(name) == _lib.OK
+    try:
+        for call in (lambda: lin.forward(x), lambda: lin.forward_gate_up_silu(lin, x)):
+            with pytest.raises(ShrewError) as e:
+                call()
+            assert e.value.code == _lib.ERR_UNSUPPORTED
+    finally:
+        assert _lib.lib().shrewq_force_kernel(b"auto") == _lib.OK
+    assert torch.equal(lin.forward(x), want)
+
+
 # ---- blocks -------------------------------------------------------------------------------------------------------------------
 def test_no_blocks_and_their_type():
     x = acts(5, 64, F32)
