@@ -5,7 +5,9 @@
 //
 // code * scale is exact in bf16: an E2M1 code has two significant bits, an E8M0 scale is a power of two of bf16's own exponent range, an E4M3
 // scale has four bits.  bf16 activations are used as they are; f32 ones come as three bf16 terms (8 + 8 + 8 bits, truncated one after
-// the other: exact), three MMAs a step into one accumulator (XT = 3).
+// the other: exact), three MMAs a step (XT = 3).  Their sums keep four accumulators: the leading terms' go to three in turn, stage by stage, and those
+// of the two others, 2^-8 and less of them, to one of their own, where they do not drown in the sum of the leading ones; all are added in f32 at the
+// end.  (In one accumulator, which loses what is below its last place at every step, k = 11008 was 2.7e-5 off.)
 //
 // Mapping.  D[128 x TOK] += A[128 x 16] * B[TOK x 16]^T: A = 128 weight rows, widened by converter warps and written to TENSOR MEMORY with
 // tcgen05.st; B = a tile of tokens in shared memory (TMA, 128-byte swizzle); D = f32 accumulators in tensor memory (lane = channel).
@@ -51,7 +53,8 @@ struct W4Cfg {
     static constexpr int kStageBytes = (kScaleOff + kScaleBytes + 1023) / 1024 * 1024;
     static constexpr int kTxBytes = kCodeBytes + kXBytes + kScaleBytes;
     static constexpr int kACols = kW4StageK / 2;
-    static constexpr int kABase = (TOK + 31) / 32 * 32;
+    static constexpr int kLeading = XT == 3 ? 3 : 1, kAccs = XT == 3 ? 4 : 1;    // accumulators of the leading terms, and in all
+    static constexpr int kABase = (kAccs * TOK + 31) / 32 * 32;
     static constexpr int kMaxSmem = (224 * 1024) / kStageBytes, kMaxTmem = (512 - kABase) / kACols;
     static constexpr int kStagesRaw = kMaxSmem < kMaxTmem ? kMaxSmem : kMaxTmem;
     static constexpr int kStages = kStagesRaw > 12 ? 12 : kStagesRaw;
@@ -204,7 +207,7 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         if (elect_one()) {
             constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TOK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             pdl_wait();  // (as the converters)
-            uint32_t s = 0, ph = 0;
+            uint32_t s = 0, ph = 0, lead = 0;  // lead: the accumulator of this stage's leading terms
             bool good = true;
             for (int i = 0; i < rounds; ++i) {
                 // (the converters have waited for the stage: its activations are there too)
@@ -219,10 +222,12 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
                         for (int t = 0; t < XT; ++t)
-                            tc_mma_ts(tmem, a + j * 32 + q * 8, bdesc + (uint64_t)(((t * (kW4StageK / 64) + j) * C::kXBox + q * 32) >> 4), idesc,
-                                      (i > 0 || j > 0 || q > 0 || t > 0) ? 1u : 0u);
+                            tc_mma_ts(tmem + (t == 0 ? lead : C::kLeading) * TOK, a + j * 32 + q * 8,
+                                      bdesc + (uint64_t)(((t * (kW4StageK / 64) + j) * C::kXBox + q * 32) >> 4), idesc,
+                                      (i >= (t == 0 ? C::kLeading : 1) || j > 0 || q > 0 || t > 1) ? 1u : 0u);
                 tc_commit(bars + kEmptyBar + s * 8);  // frees the stage's shared memory and its A columns
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
+                if (C::kLeading > 1 && ++lead == C::kLeading) lead = 0;
             }
             if (good) tc_commit(bars + kAccBar);
         }
@@ -271,6 +276,25 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         mbar_wait_all<kTimeoutW4>(bars + kAccBar, 0, ctl, status, 4, 0);
         ok = warp_ok(ctl);
         tc_fence_after();
+        if constexpr (C::kAccs > 1) {  // all accumulators into the first, the small one first
+            const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+            for (int c = group * 16; c < TOK; c += kW4Groups * 16) {
+                uint32_t sum[16], r[16];
+                tc_ld16(at + C::kLeading * TOK + c, sum);
+                for (int n = 0; n < C::kLeading && n < rounds; ++n) {
+                    tc_ld16(at + n * TOK + c, r);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sum[e] = __float_as_uint(__uint_as_float(sum[e]) + __uint_as_float(r[e]));
+                }
+                tc_st16(at + c, sum);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            named_bar_sync(1, 128 * kW4Groups);
+            tc_fence_after();
+        }
         if (S == 1)
             cluster_finish<TOK, kW4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0);
     }

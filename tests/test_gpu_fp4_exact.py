@@ -98,6 +98,20 @@ def test_every_column_and_every_bit(fmt, k, times, m):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k", [32, 96, 256, 4096, 8192])
+@pytest.mark.parametrize("m,n", [(m, 70) for m in MS] + [(5, 9600), (20, 9600), (300, 9600)])
+def test_low_bits_of_f32_activations_survive_long_sums(fmt, m, n, k):
+    """x = 1 + 2^-12 + 2^-20 in every column and weights of 1 and -1: k times 21 bits, k one or three times a power of two, so that the sums of the
+    leading and of the low parts fit f32 and so does their sum (23 bits); added up together, the low parts fall below the last place."""
+    sign = torch.randint(0, 2, (n, 1), generator=torch.Generator().manual_seed(k), dtype=torch.uint8)
+    lin = Fp4Linear(stored((2 + 8 * sign).expand(n, k).contiguous(), fmt))
+    x = torch.full((m, k), 1.0 + 2.0 ** -12 + 2.0 ** -20, device="cuda")
+    want = ((1.0 - 2.0 * sign.double()) * k * (1.0 + 2.0 ** -12 + 2.0 ** -20)).view(1, n).expand(m, n)
+    assert torch.equal(want.float().double(), want)
+    assert torch.equal(lin.forward(x).double().cpu(), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rounded", [False, True])
 @pytest.mark.parametrize("m,n", [(1, 150), (8, 150), (8, 19100), (40, 150), (200, 150), (300, 9500)])
 def test_a_nan_block_stays_in_its_channel(fmt, rounded, m, n):
