@@ -7,7 +7,9 @@
 // scale has four bits.  bf16 activations are used as they are; f32 ones come as three bf16 terms (8 + 8 + 8 bits, truncated one after
 // the other: exact), three MMAs a step (XT = 3).  Their sums keep four accumulators: the leading terms' go to three in turn, stage by stage, and those
 // of the two others, 2^-8 and less of them, to one of their own, where they do not drown in the sum of the leading ones; all are added in f32 at the
-// end.  (In one accumulator, which loses what is below its last place at every step, k = 11008 was 2.7e-5 off.)
+// end.  (In one accumulator, which loses what is below its last place at every step, k = 11008 was 2.7e-5 off.)  bf16 activations have two accumulators in
+// turn in tiles of 64 tokens (sums of 11008 NV products 4.3e-6 -> 1.8e-6 off, and 4096 x 11008 16.1 -> 14.9 us; three: 1.0e-6, 15.4 us) and one in larger
+// ones, where a second costs a stage of the ring (128 tokens of gated 11008 x 4096: 34.9 -> 40.4 us).
 //
 // Mapping.  D[128 x TOK] += A[128 x 16] * B[TOK x 16]^T: A = 128 weight rows, widened by converter warps and written to TENSOR MEMORY with
 // tcgen05.st; B = a tile of tokens in shared memory (TMA, 128-byte swizzle); D = f32 accumulators in tensor memory (lane = channel).
@@ -53,7 +55,7 @@ struct W4Cfg {
     static constexpr int kStageBytes = (kScaleOff + kScaleBytes + 1023) / 1024 * 1024;
     static constexpr int kTxBytes = kCodeBytes + kXBytes + kScaleBytes;
     static constexpr int kACols = kW4StageK / 2;
-    static constexpr int kLeading = XT == 3 ? 3 : 1, kAccs = XT == 3 ? 4 : 1;    // accumulators of the leading terms, and in all
+    static constexpr int kLow = XT == 3 ? 1 : 0, kLeading = XT == 3 ? 3 : TOK == 64 ? 2 : 1, kAccs = kLow + kLeading;  // accumulators: of the low terms, then of the leading ones
     static constexpr int kABase = (kAccs * TOK + 31) / 32 * 32;
     static constexpr int kMaxSmem = (224 * 1024) / kStageBytes, kMaxTmem = (512 - kABase) / kACols;
     static constexpr int kStagesRaw = kMaxSmem < kMaxTmem ? kMaxSmem : kMaxTmem;
@@ -146,6 +148,7 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const int m0 = tile % m_tiles * TOK, n0 = tile / m_tiles * kChan;
     const int rounds_total = (K + kW4StageK - 1) / kW4StageK, r_begin = (int)rank * rounds_per_cta;
     const int rounds = min(rounds_total - r_begin, rounds_per_cta);  // >= 1 by construction of the grid
+    const int parts = C::kLow + min(rounds, C::kLeading);            // accumulators that hold something
     const size_t pieces = (size_t)((K + 255) >> 8) * (NV ? 4 : 2);
     constexpr uint32_t kFullBar = 0, kAreadyBar = C::kStages * 8, kEmptyBar = 2 * C::kStages * 8, kAccBar = 3 * C::kStages * 8;
     const uint32_t bars = smem_u32(bar_area), smem_base = smem_u32(smem);
@@ -222,7 +225,7 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
                         for (int t = 0; t < XT; ++t)
-                            tc_mma_ts(tmem + (t == 0 ? lead : C::kLeading) * TOK, a + j * 32 + q * 8,
+                            tc_mma_ts(tmem + (t == 0 ? C::kLow + lead : 0) * TOK, a + j * 32 + q * 8,
                                       bdesc + (uint64_t)(((t * (kW4StageK / 64) + j) * C::kXBox + q * 32) >> 4), idesc,
                                       (i >= (t == 0 ? C::kLeading : 1) || j > 0 || q > 0 || t > 1) ? 1u : 0u);
                 tc_commit(bars + kEmptyBar + s * 8);  // frees the stage's shared memory and its A columns
@@ -276,27 +279,8 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         mbar_wait_all<kTimeoutW4>(bars + kAccBar, 0, ctl, status, 4, 0);
         ok = warp_ok(ctl);
         tc_fence_after();
-        if constexpr (C::kAccs > 1) {  // all accumulators into the first, the small one first
-            const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
-#pragma unroll 1
-            for (int c = group * 16; c < TOK; c += kW4Groups * 16) {
-                uint32_t sum[16], r[16];
-                tc_ld16(at + C::kLeading * TOK + c, sum);
-                for (int n = 0; n < C::kLeading && n < rounds; ++n) {
-                    tc_ld16(at + n * TOK + c, r);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sum[e] = __float_as_uint(__uint_as_float(sum[e]) + __uint_as_float(r[e]));
-                }
-                tc_st16(at + c, sum);
-            }
-            tc_wait_st();
-            tc_fence_before();
-            named_bar_sync(1, 128 * kW4Groups);
-            tc_fence_after();
-        }
         if (S == 1)
-            cluster_finish<TOK, kW4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0);
+            cluster_finish<TOK, kW4Groups, kMode, YT>(tmem, smem, nullptr, 1, 0, group, quad, lane, ok, ops, y, M, N, ldy, epilogue, n0, m0, nullptr, 0, parts);
     }
     if (S > 1) {
         const int group = (warp - 2) >> 2, quad = warp & 3;
@@ -305,13 +289,13 @@ gemm_w4_bf16_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         cluster_arrive();  // every CTA of the tile has its sums: the stages are idle everywhere
         cluster_wait();
         tc_fence_after();
-        if (warp >= 2 && ok) cluster_send<TOK, kW4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane);
+        if (warp >= 2 && ok) cluster_send<TOK, kW4Groups, kMode>(tmem, smem_base + C::kSlotOff, S, rank, group, quad, lane, parts);
         __syncwarp();
         cluster_arrive();  // and has received the others'
         cluster_wait();
         if (warp >= 2)
             cluster_finish<TOK, kW4Groups, kMode, YT>(tmem, smem, reinterpret_cast<const float *>(smem + C::kSlotOff), S, rank, group, quad, lane, ok, ops, y, M, N,
-                                                      ldy, epilogue, n0, m0);
+                                                      ldy, epilogue, n0, m0, nullptr, 0, parts);
     }
 
     tc_fence_before();

@@ -77,10 +77,24 @@ struct ClusterEpi {
 template <int NCOLS>
 __device__ __forceinline__ int cluster_finishers(int S) { return S < NCOLS / kEpiChunk ? S : NCOLS / kEpiChunk; }
 
+// 16 columns of the first of `parts` accumulators, NCOLS columns apart, with the others' added in their order
+template <int NCOLS>
+__device__ __forceinline__ void load_sums(uint32_t taddr, int parts, uint32_t (&sum)[kEpiChunk]) {
+    tc_ld16(taddr, sum);
+    tc_wait_ld();
+    for (int n = 1; n < parts; ++n) {
+        uint32_t r[kEpiChunk];
+        tc_ld16(taddr + n * NCOLS, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < kEpiChunk; ++j) sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(r[j]));
+    }
+}
+
 // Sends this CTA's raw sums of the other CTAs' tokens to them.  One call per epilogue thread; the receivers' stages must be idle (a
 // cluster barrier before), the sums are there after the next cluster barrier.
 template <int NCOLS, int G, int MODE>
-__device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_local, int S, uint32_t rank, int group, int quad, int lane) {
+__device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_local, int S, uint32_t rank, int group, int quad, int lane, int parts = 1) {
     const int F = cluster_finishers<NCOLS>(S), tokens = NCOLS / F, row = quad * 32 + lane;
     const uint32_t taddr = tmem_d + ((uint32_t)(quad * 32) << 16);
     const int chunks = tokens / kEpiChunk, per_dest = ClusterEpi<NCOLS, MODE>::kAccs * chunks;
@@ -90,8 +104,11 @@ __device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_loc
         const uint32_t dest = (rank + 1 + step) % F;       // everybody starts with another receiver (a finisher never meets itself)
         const uint32_t source = rank < dest ? rank : rank - 1;
         uint32_t r[kEpiChunk];
-        tc_ld16(taddr + acc * NCOLS + dest * tokens + c * kEpiChunk, r);
-        tc_wait_ld();
+        if constexpr (ClusterEpi<NCOLS, MODE>::kAccs == 1) load_sums<NCOLS>(taddr + dest * tokens + c * kEpiChunk, parts, r);
+        else {
+            tc_ld16(taddr + acc * NCOLS + dest * tokens + c * kEpiChunk, r);
+            tc_wait_ld();
+        }
         const uint32_t at = map_to_cta(slots_local, dest) +
                             (uint32_t)((((int)source * ClusterEpi<NCOLS, MODE>::kAccs + acc) * tokens + c * kEpiChunk) * 512 + row * 4);
 #pragma unroll
@@ -100,11 +117,11 @@ __device__ __forceinline__ void cluster_send(uint32_t tmem_d, uint32_t slots_loc
 }
 
 // Finishes this CTA's share of the tokens, m0 the tile's first token.  One call per epilogue thread (G groups of 128).
-// TOKENS: the sums of token m are first multiplied by 2^(exps[m] + back).
+// TOKENS: the sums of token m are first multiplied by 2^(exps[m] + back).  parts: accumulators that a sum is kept in (one but for kEpiColumns' two).
 template <int NCOLS, int G, int MODE, typename YT, bool TOKENS = false>
 __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_base, const float *slots, int S, uint32_t rank, int group, int quad, int lane, bool ok,
                                                const Operands &ops, YT *__restrict__ y, int M, int N, size_t ldy, int epilogue, int n0, int m0,
-                                               const int *exps = nullptr, int back = 0) {
+                                               const int *exps = nullptr, int back = 0, int parts = 1) {
     constexpr int CW = kEpiChunk, CH = MODE == kEpiLanesPaired ? 64 : 128, RB = CH * (int)sizeof(YT), EPV = 16 / (int)sizeof(YT), PPR = RB / 16, PIECES = CW * PPR;
     constexpr int ACCS = ClusterEpi<NCOLS, MODE>::kAccs;
     const int F = cluster_finishers<NCOLS>(S), tokens = NCOLS / F, row = quad * 32 + lane;
@@ -128,9 +145,12 @@ __device__ __forceinline__ void cluster_finish(uint32_t tmem_d, uint8_t *stage_b
     for (int c = group; c < chunks; c += G) {
         if (ok) {
             uint32_t raw[ACCS][CW];
+            if constexpr (ACCS == 1) load_sums<NCOLS>(taddr + first_col + c * CW, parts, raw[0]);
+            else {
 #pragma unroll
-            for (int a = 0; a < ACCS; ++a) tc_ld16(taddr + a * NCOLS + first_col + c * CW, raw[a]);
-            tc_wait_ld();
+                for (int a = 0; a < ACCS; ++a) tc_ld16(taddr + a * NCOLS + first_col + c * CW, raw[a]);
+                tc_wait_ld();
+            }
             float v[ACCS][CW];
             if (S == 1) {
 #pragma unroll
