@@ -22,18 +22,18 @@ bool sizes_overflow(size_t rows, size_t cols) { return cols > ((size_t)1 << 40) 
 
 // Up to 32 tokens: the kernel in f16 (two CTAs an SM, a launch to stage the activations) or the one in bf16 (one CTA an SM, bf16 activations as they
 // are).  Measured on weights from cold HBM, us in f16 / in bf16:
-//   bf16, tiles for one CTA an SM, which may also share their k: bf16 wins (4096 x 4096, 16 tokens: 19.5 / 9.7; 4096 x 11008: 26.4 / 15.8; 8192 x
-//     4096 gated 20.2 / 18.5), but for fewer than 16 tokens of long rows in more than half as many tiles as SMs (11008 x 4096, 8 tokens: 18.0 / 19.0;
-//     16384 x 8192: 28.9 / 31.4);
-//   bf16, more tiles, which take bf16 another round: f16 wins (11008 x 4096 gated, 8 and 32 tokens: 24.9 / 35.3, 26.9 / 35.2), until the staging and
-//     16 tokens an epilogue chunk outweigh short rows (32768 x 512, 8, 16 and 32 tokens: 9.9 / 11.8, 11.5 / 11.5, 15.5 / 11.2);
-//   f32, three passes in f16, three products of one pass in bf16: bf16 wins (11008 x 4096, 8 tokens: 33.4 / 25.2; gated 54.5 / 49.7), but where many
-//     CTAs read the same few bytes of activations again and again, their three terms less than 128 KB (5 tokens: 32.8 / 43.3; 32768 x 2048, 8 and 12:
-//     31.3 / 43.4, 32.3 / 29.7).
+//   bf16, tiles for one CTA an SM, which may also share their k: bf16 wins (4096 x 4096, 16 tokens: 19.6 / 9.3; 4096 x 11008: 27.2 / 14.6; 8192 x
+//     4096 gated: 20.5 / 16.5), but where more than half of the SMs read the same activations of less than 128 KB again and again (11008 x 4096, 8
+//     tokens: 18.3 / 18.6; 16384 x 8192, 5 and 8: 28.4 / 39.4, 29.3 / 27.5);
+//   bf16, more tiles, which take bf16 another round: f16 wins (11008 x 4096 gated, 8 and 32 tokens: 25.0 / 33.9, 27.0 / 31.5), until the staging and
+//     16 tokens an epilogue chunk outweigh short rows (32768 x 512, 8, 16 and 32 tokens: 9.9 / 11.7, 11.6 / 11.6, 15.6 / 11.2; x 1024: 12.2 / 15.7,
+//     13.6 / 15.3, 17.4 / 14.9; 50257 x 256, 5 and 12: 14.5 / 16.4, 17.3 / 16.4);
+//   f32, three passes in f16, three products of one pass in bf16: bf16 wins (11008 x 4096, 8 tokens: 33.6 / 25.3; gated 55.0 / 49.8), but for activations
+//     of less than 128 KB in three terms, as above (5 tokens: 33.1 / 42.1; 32768 x 2048, 8 and 12: 31.8 / 43.4, 32.7 / 30.1).
 bool w4_f16_wins(const shrewq_ctx *ctx, const Fp4Forward &a) {
-    const size_t tiles = (a.N + (a.up ? 63 : 127)) / (a.up ? 64 : 128), sms = (size_t)ctx->sm_count;
-    if (a.x_dtype == SHREWQ_F32) return tiles > sms / 2 && a.K >= 1024 && a.M * a.K * 6 < 128 * 1024;
-    return tiles > sms ? a.K >= 32 * a.M : tiles > sms / 2 && a.K >= 4096 && a.M < 16;
+    const size_t tiles = (a.N + (a.up ? 63 : 127)) / (a.up ? 64 : 128), sms = (size_t)ctx->sm_count, few = 128 * 1024;
+    if (a.x_dtype == SHREWQ_F32) return tiles > sms / 2 && a.K >= 1024 && a.M * a.K * 6 < few;
+    return tiles > sms ? a.M < 8 || a.K >= 64 * a.M : tiles > sms / 2 && a.K >= 4096 && a.M * a.K * 2 < few;
 }
 
 }  // namespace

@@ -152,17 +152,17 @@ def test_more_tokens_than_indexes_hold_are_refused(rounded, x_dtype, most):
 @pytest.mark.parametrize("m", [6, 20, 32])
 def test_gated_layers_of_many_tiles_in_turn_captured_and_on_streams(m):
     """The kernels of 5 to 32 tokens over more tiles than SMs, and over few, one after the other: the same bits eagerly, on another stream and replayed."""
-    gate, wg, _ = layer(9600, 1056, Fp4Format.Nv, 1, bias=False)
-    up, wu, _ = layer(9600, 1056, Fp4Format.Nv, 2, bias=False)
-    down, wd, _ = layer(1056, 9600, Fp4Format.Nv, 3, bias=False)
-    xs = [acts(m, 1056, BF16, seed=s) * 0.01 for s in range(3)]
+    gate, wg, _ = layer(9600, 2080, Fp4Format.Nv, 1, bias=False)
+    up, wu, _ = layer(9600, 2080, Fp4Format.Nv, 2, bias=False)
+    down, wd, _ = layer(2080, 9600, Fp4Format.Nv, 3, bias=False)
+    xs = [acts(m, 2080, BF16, seed=s) * 0.01 for s in range(3)]
 
     def run(x):
         return down.forward(gate.forward_gate_up_silu(up, x))
     h = gate.forward_gate_up_silu(up, xs[0])
     assert gate.last_kernel() == "tcgen05-w4-f16"
     xd = xs[0].double().cpu().numpy()
-    near(h, O.product(xd, wg, up=wu), O.product_bound(xd, wg, 1056, up=wu))
+    near(h, O.product(xd, wg, up=wu), O.product_bound(xd, wg, 2080, up=wu))
     want = [run(x) for x in xs]
     assert down.last_kernel() == "tcgen05-w4"
     for _ in range(20):
